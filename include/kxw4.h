@@ -264,6 +264,83 @@ int kxw4_gemm_w4a4(const kxw4_weight_t *w, const uint8_t *q4, const float *scale
                    const int32_t *sum, int T, void *y, int y_dtype,
                    const float *residual, void *stream);
 
+/* ---- rows with a weight of their own --------------------------------------
+ * No counterpart in the reference, whose model is dense and has no adapters.
+ * The rows of a batch go to one of `groups` weights each: the experts that a
+ * router chose (k per token), or an adapter per request (k = 1). Slot t*k + j
+ * is choice j of token t; the plan sorts the N = T*k slots by group, stably,
+ * and is shared by every call of a step.
+ *   offsets  : [groups + 1] slots with a group below e; sorted places
+ *              [offsets[e], offsets[e+1]) are group e's rows
+ *   order    : [N] the slot at each sorted place; those without a group last
+ *   position : [N] the place of each slot, -1 without a group
+ * A slot has no group when its id lies outside [0, groups) (a dropped token,
+ * an expert of another GPU, a request without an adapter); one token may name
+ * a group twice. Buffers are the caller's; apart from kxw4_route_rows the
+ * calls read the plan and trust it. T may be 0: nothing is read or written
+ * (kxw4_route_rows still clears the offsets). Limits: groups 1..1024, T*k up
+ * to 2^30 slots. Row buffers of N rows are written up to offsets[groups];
+ * what lies behind stays as it was. Outputs must not overlap inputs unless
+ * said. Results do not depend on the order in which work-groups run. */
+typedef struct kxw4_route {
+    int32_t T, k, groups;
+    int32_t *offsets, *order, *position;
+} kxw4_route_t;
+
+/* ids[T][k]: int32, or int64 where ids_64 is set. workspace:
+ * kxw4_route_workspace bytes (0 up to 16,384 slots; then it may be NULL). */
+size_t kxw4_route_workspace(int T, int k, int groups);
+int kxw4_route_rows(const void *ids, int ids_64, const kxw4_route_t *route, void *workspace, void *stream);
+
+/* rows[p] = x[order[p] / k] for the places of a group. x [T][H], rows [N][H]
+ * of one type (KXW4_F32, KXW4_BF16); any H, and any alignment of the type's
+ * own size (16-byte pieces where pointers and rows allow). The gradient of x
+ * is kxw4_combine_rows without weights. */
+int kxw4_dispatch_rows(const void *x, int dtype, int H, const kxw4_route_t *route, void *rows, void *stream);
+
+/* y[t] = sum over j of weights[t][j] * rows[position[t][j]] (weights NULL: all
+ * 1), slots without a group adding nothing; summed in FP32 in the order of j,
+ * rounded once. rows [N][H] and y [T][H] have types of their own. */
+int kxw4_combine_rows(const void *rows, int rows_dtype, int H, const float *weights, const kxw4_route_t *route,
+                      void *y, int y_dtype, void *stream);
+
+/* The gradient of kxw4_combine_rows: drows[position[t][j]] = weights[t][j] *
+ * dy[t] (of rows' type), dweights[t][j] = <dy[t], rows[position[t][j]]> in
+ * FP32, 0 for a slot without a group. */
+int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, int rows_dtype, int H,
+                               const float *weights, const kxw4_route_t *route, void *drows, float *dweights,
+                               void *stream);
+
+/* The experts' projections: ys[i][p] = W_i,e x[order[p] / k], p a place of
+ * expert e. Each weight stacks the experts' rows: M = groups * rows, expert e
+ * the rows [e*rows, (e+1)*rows), rows a multiple of 16. Up to 4 weights share
+ * the activation (gate and up), with one K, group and encoding. a holds T rows,
+ * or with sorted_rows N rows that lie in the plan's order already (a down
+ * projection). ys[i]: [N][rows] of y_dtype. Tiers: per-token activations
+ * (block 0) with KXW4_SCALE_FP16 weights of group 64 or 128; block 32 with
+ * KXW4_SCALE_FP16_ZP4 of group 32 or 64, or with KXW4_SCALE_W8; else
+ * KXW4_ETIER. The arithmetic of a row is kxw4_gemm's under a split count that
+ * follows from the sizes alone (T, k, groups, rows, K). a's rows * K < 2^31. */
+int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count, const kxw4_act_t *a,
+                     const kxw4_route_t *route, int sorted_rows, int y_dtype, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection: out[t] = y[t]
+ * + scale[e] * B_e (A_e x[t]), e the group of token t in a plan with k = 1 and
+ * groups = n; out[t] = y[t] without one. a [n][r][K] and b [n][M][r] BF16,
+ * scale [n]. x [T][K], y and out [T][M] (one type); out may be y itself.
+ * Products are exact and summed in FP32, A x is held in FP32, out is rounded
+ * once. K % 128 == 0, M % 16 == 0 (as the projection's weight), r a multiple
+ * of 8 up to 256 (pad smaller ranks with zeros); 16-byte aligned pointers.
+ * workspace: kxw4_adapter_workspace bytes, this call's own while it runs. */
+typedef struct kxw4_adapters {
+    int32_t n, r, K, M;
+    const uint16_t *a, *b;
+    const float *scale;
+} kxw4_adapters_t;
+size_t kxw4_adapter_workspace(const kxw4_adapters_t *adapters, int T);
+int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, const kxw4_adapters_t *adapters,
+                     const kxw4_route_t *route, void *out, void *workspace, void *stream);
+
 /* No counterpart in the reference. For callers that cannot allocate (code
  * under HIP graph capture, tight serving loops): x[T][K] (KXW4_F32 or
  * KXW4_BF16) is quantized per K32 block into a fixed device array of this

@@ -33,10 +33,22 @@ class Act(C.Structure):
                 ("q", C.c_void_p), ("scale", C.c_void_p), ("sum", C.c_void_p)]
 
 
+class Route(C.Structure):
+    _fields_ = [("T", C.c_int32), ("k", C.c_int32), ("groups", C.c_int32),
+                ("offsets", C.c_void_p), ("order", C.c_void_p), ("position", C.c_void_p)]
+
+
+class AdapterSet(C.Structure):
+    _fields_ = [("n", C.c_int32), ("r", C.c_int32), ("K", C.c_int32), ("M", C.c_int32),
+                ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p)]
+
+
 # name -> (restype, argtypes); the exported C ABI, in header order
 P, I, F = C.c_void_p, C.c_int, C.c_float
 WP = C.POINTER(Weight)
 AP = C.POINTER(Act)
+RP = C.POINTER(Route)
+DP = C.POINTER(AdapterSet)
 SIGNATURES = {
     "kxw4_abi_version": (I, []),
     "kxw4_error_string": (C.c_char_p, [I]),
@@ -61,6 +73,14 @@ SIGNATURES = {
     "kxw4_gemm": (I, [WP, AP, P, I, P, C.POINTER(I), I, I, P]),
     "kxw4_gemm_fanout": (I, [C.POINTER(WP), C.POINTER(P), I, AP, I, C.POINTER(I), I, I, P]),
     "kxw4_gemm_w4a4": (I, [WP, P, P, P, I, P, I, P, P]),
+    "kxw4_route_workspace": (C.c_size_t, [I, I, I]),
+    "kxw4_route_rows": (I, [P, I, RP, P, P]),
+    "kxw4_dispatch_rows": (I, [P, I, I, RP, P, P]),
+    "kxw4_combine_rows": (I, [P, I, I, P, RP, P, I, P]),
+    "kxw4_combine_rows_backward": (I, [P, I, P, I, I, P, RP, P, P, P]),
+    "kxw4_expert_gemm": (I, [C.POINTER(WP), C.POINTER(P), I, AP, RP, I, I, P]),
+    "kxw4_adapter_workspace": (C.c_size_t, [DP, I]),
+    "kxw4_adapter_add": (I, [P, I, P, I, DP, RP, P, P, P]),
     "kxw4_gemv_x_noalloc": (I, [WP, P, I, I, P, I, P, P]),
     "kxw4_tqf_open": (I, [C.c_char_p, C.POINTER(P)]),
     "kxw4_tqf_close": (None, [P]),

@@ -214,6 +214,34 @@ int decode_uniform(const kxw4_weight_t *const *ws, void *const *ys, int count,
     return r == 1 ? KXW4_ESHAPE : r;
 }
 
+// ---- rows with a weight of their own -----------------------------------------
+
+bool valid_dtype(int d) { return d == KXW4_F32 || d == KXW4_BF16; }
+bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+constexpr int kMaxGroups = 1024;
+constexpr long long kMaxSlots = 1ll << 30;
+
+bool valid_plan(int T, int k, int groups) {
+    return T >= 0 && k > 0 && groups > 0 && groups <= kMaxGroups && (long long)T * k <= kMaxSlots;
+}
+
+// A plan that kxw4_route_rows filled. (With T = 0 only its sizes count.)
+int check_route(const kxw4_route_t *r) {
+    if (!r) return KXW4_EARG;
+    if (!valid_plan(r->T, r->k, r->groups)) return KXW4_ESHAPE;
+    if (r->T > 0 && (!r->offsets || !r->order || !r->position)) return KXW4_EPREP;
+    return KXW4_OK;
+}
+
+int check_rows(const kxw4_route_t *r, int H) {
+    const int rc = check_route(r);
+    if (rc) return rc;
+    return H <= 0 || H > (1 << 28) ? KXW4_ESHAPE : KXW4_OK;
+}
+
+int elem_bytes(int dtype) { return dtype == KXW4_BF16 ? 2 : 4; }
+
 }  // namespace
 
 extern "C" {
@@ -456,6 +484,171 @@ int kxw4_gemm_w4a4(const kxw4_weight_t *w, const uint8_t *q4, const float *scale
     args.T = T;
     args.y_bf16 = y_dtype == KXW4_BF16 ? 1 : 0;
     return launch_w4a4(args, as_stream(stream));
+}
+
+size_t kxw4_route_workspace(int T, int k, int groups) {
+    if (!valid_plan(T, k, groups)) return 0;
+    int per = 0;
+    const int blocks = route_blocks_of(T * k, &per);
+    return blocks > 1 ? (size_t)blocks * (groups + 1) * sizeof(int) : 0;
+}
+
+int kxw4_route_rows(const void *ids, int ids_64, const kxw4_route_t *route, void *workspace, void *stream) {
+    if (!route || !route->offsets) return KXW4_EARG;
+    if (!valid_plan(route->T, route->k, route->groups)) return KXW4_ESHAPE;
+    if (route->T > 0 && (!ids || !route->order || !route->position)) return KXW4_EARG;
+    if (!workspace && kxw4_route_workspace(route->T, route->k, route->groups)) return KXW4_EARG;
+    RouteArgs a{};
+    a.ids = ids;
+    a.ids64 = ids_64 ? 1 : 0;
+    a.offsets = route->offsets;
+    a.order = route->order;
+    a.position = route->position;
+    a.hist = static_cast<int *>(workspace);
+    a.N = route->T * route->k;
+    a.groups = route->groups;
+    return launch_route(a, as_stream(stream));
+}
+
+int kxw4_dispatch_rows(const void *x, int dtype, int H, const kxw4_route_t *route, void *rows, void *stream) {
+    const int rc = check_rows(route, H);
+    if (rc) return rc;
+    if (!valid_dtype(dtype)) return KXW4_ESHAPE;
+    if (route->T == 0) return KXW4_OK;
+    if (!x || !rows || !aligned(x, elem_bytes(dtype)) || !aligned(rows, elem_bytes(dtype))) return KXW4_EARG;
+    RowArgs a{};
+    a.x = x;
+    a.rows = rows;
+    a.position = route->position;
+    a.T = route->T;
+    a.k = route->k;
+    a.H = H;
+    return launch_dispatch(a, elem_bytes(dtype), as_stream(stream));
+}
+
+int kxw4_combine_rows(const void *rows, int rows_dtype, int H, const float *weights, const kxw4_route_t *route,
+                      void *y, int y_dtype, void *stream) {
+    const int rc = check_rows(route, H);
+    if (rc) return rc;
+    if (!valid_dtype(rows_dtype) || !valid_dtype(y_dtype)) return KXW4_ESHAPE;
+    if (route->T == 0) return KXW4_OK;
+    if (!rows || !y || !aligned(rows, elem_bytes(rows_dtype)) || !aligned(y, elem_bytes(y_dtype)) || !aligned(weights, 4))
+        return KXW4_EARG;
+    RowArgs a{};
+    a.rows = const_cast<void *>(rows);
+    a.y = y;
+    a.weights = weights;
+    a.position = route->position;
+    a.T = route->T;
+    a.k = route->k;
+    a.H = H;
+    return launch_combine(a, rows_dtype == KXW4_BF16, y_dtype == KXW4_BF16, as_stream(stream));
+}
+
+int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, int rows_dtype, int H,
+                               const float *weights, const kxw4_route_t *route, void *drows, float *dweights,
+                               void *stream) {
+    const int rc = check_rows(route, H);
+    if (rc) return rc;
+    if (!valid_dtype(dy_dtype) || !valid_dtype(rows_dtype)) return KXW4_ESHAPE;
+    if (route->T == 0) return KXW4_OK;
+    if (!dy || !rows || !weights || !drows || !dweights) return KXW4_EARG;
+    if (!aligned(dy, elem_bytes(dy_dtype)) || !aligned(rows, elem_bytes(rows_dtype)) ||
+        !aligned(drows, elem_bytes(rows_dtype)) || !aligned(weights, 4) || !aligned(dweights, 4))
+        return KXW4_EARG;
+    RowArgs a{};
+    a.x = dy;
+    a.rows = const_cast<void *>(rows);
+    a.y = drows;
+    a.weights = weights;
+    a.dweights = dweights;
+    a.position = route->position;
+    a.T = route->T;
+    a.k = route->k;
+    a.H = H;
+    return launch_combine_backward(a, dy_dtype == KXW4_BF16, rows_dtype == KXW4_BF16, as_stream(stream));
+}
+
+int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count, const kxw4_act_t *a,
+                     const kxw4_route_t *route, int sorted_rows, int y_dtype, void *stream) {
+    if (!ws || !ys || count <= 0 || count > kMaxWeights || !a) return KXW4_EARG;
+    int rc = check_route(route);
+    if (rc) return rc;
+    ExpertArgs x{};
+    for (int i = 0; i < count; ++i) {
+        const kxw4_weight_t *w = ws[i];
+        rc = check_weight(w);
+        if (rc) return rc;
+        if (w->K != ws[0]->K || w->group != ws[0]->group || w->scale_enc != ws[0]->scale_enc) return KXW4_ESHAPE;
+        if (w->M % route->groups || (w->M / route->groups) % 16) return KXW4_ESHAPE;
+        x.w[i] = StripWeight{w->codes, w->scales, ys[i], w->M / route->groups};
+        // 32-bit offsets inside one expert's codes
+        if ((long long)x.w[i].M * w->K >= (1ll << 31)) return KXW4_ESHAPE;
+    }
+    if (!valid_dtype(y_dtype)) return KXW4_ESHAPE;
+    const long long rows = sorted_rows ? (long long)route->T * route->k : route->T;
+    if (a->T != rows || a->K != ws[0]->K || (a->block != 0 && a->block != 32)) return KXW4_ESHAPE;
+    // the tiers of the strip kernel: per-token activations with plain FP16
+    // scales, K32 blocks with zero points or W8
+    if (a->block == 0 ? ws[0]->scale_enc != KXW4_SCALE_FP16 || (ws[0]->group != 64 && ws[0]->group != 128)
+                      : ws[0]->scale_enc == KXW4_SCALE_FP16 || ws[0]->group > 64 || ws[0]->group < 32)
+        return KXW4_ETIER;
+    if (!strip_takes(ws[0]->group, a->block, ws[0]->scale_enc, rows, ws[0]->K)) return KXW4_ESHAPE;
+    if (rows == 0) return KXW4_OK;
+    if (!a->q || !a->scale) return KXW4_EPREP;
+    for (int i = 0; i < count; ++i)
+        if (!ys[i]) return KXW4_EARG;
+    x.count = count;
+    x.q = a->q;
+    x.ascale = a->scale;
+    x.offsets = route->offsets;
+    x.order = sorted_rows ? nullptr : route->order;
+    x.N = route->T * route->k;
+    x.groups = route->groups;
+    x.k = route->k;
+    x.K = ws[0]->K;
+    x.group = ws[0]->group;
+    x.block = a->block;
+    x.scale_enc = ws[0]->scale_enc;
+    x.y_bf16 = y_dtype == KXW4_BF16 ? 1 : 0;
+    return launch_experts(x, as_stream(stream));
+}
+
+size_t kxw4_adapter_workspace(const kxw4_adapters_t *ad, int T) {
+    if (!ad || T <= 0 || ad->n <= 0 || ad->r <= 0 || ad->K <= 0) return 0;
+    return (size_t)adapter_splits(ad->n, T, ad->K) * T * ad->r * sizeof(float);
+}
+
+int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, const kxw4_adapters_t *ad,
+                     const kxw4_route_t *route, void *out, void *workspace, void *stream) {
+    if (!ad) return KXW4_EARG;
+    const int rc = check_route(route);
+    if (rc) return rc;
+    if (ad->n != route->groups || route->k != 1) return KXW4_ESHAPE;
+    if (ad->r <= 0 || ad->r % 8 || ad->r > 256 || ad->K <= 0 || ad->K % 128 || ad->M <= 0 || ad->M % 16)
+        return KXW4_ESHAPE;
+    if (!valid_dtype(y_dtype) || !valid_dtype(x_dtype)) return KXW4_ESHAPE;
+    if (route->T == 0) return KXW4_OK;
+    if (!y || !x || !out || !workspace || !ad->a || !ad->b || !ad->scale) return KXW4_EARG;
+    if (!aligned(y, 16) || !aligned(x, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(ad->a, 16) ||
+        !aligned(ad->b, 16) || !aligned(ad->scale, 4))
+        return KXW4_EARG;
+    AdapterArgs a{};
+    a.y = y;
+    a.x = x;
+    a.out = out;
+    a.a = ad->a;
+    a.b = ad->b;
+    a.scale = ad->scale;
+    a.low = static_cast<float *>(workspace);
+    a.offsets = route->offsets;
+    a.order = route->order;
+    a.T = route->T;
+    a.n = ad->n;
+    a.r = ad->r;
+    a.K = ad->K;
+    a.M = ad->M;
+    return launch_adapter(a, x_dtype == KXW4_BF16, y_dtype == KXW4_BF16, as_stream(stream));
 }
 
 int kxw4_partials(const kxw4_weight_t *w, const kxw4_act_t *a, int32_t *P, void *stream) {

@@ -84,6 +84,13 @@ __device__ __forceinline__ uint16_t float_to_bf16(float x) {
     return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
 }
 
+// The same in the low half of a word, for any value: a NaN stays a NaN (above,
+// one of low mantissa bits only is carried over to infinity or zero).
+__device__ __forceinline__ uint32_t round_bf16(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return x == x ? (b + 0x7fffu + ((b >> 16) & 1u)) >> 16 : (b >> 16) | 0x40u;
+}
+
 __device__ __forceinline__ float bf16_to_float(uint16_t b) {
     return __uint_as_float((uint32_t)b << 16);
 }

@@ -133,6 +133,10 @@ struct StripArgs {
     int waves, same_s;                // waves per work-group, whether every entry has one S (set by the launcher)
     int entries;
     StripEntry e[kMaxWeights * kMaxSegments];
+    // grouped rows (the entries are the weights, their blk first row blocks):
+    // M rows of each group, `row_blocks` work-groups per token tile
+    const int *offsets, *order;
+    int groups, k, row_blocks;
 };
 // the modes the strip kernel is built for
 bool strip_takes(int group, int block, int scale_enc, long long T, int K);
@@ -168,6 +172,60 @@ StripArgs strip_args(const A &a, int variant, int smin, int smax) {
     s.variant = variant;
     return s;
 }
+// The rows of `groups` groups, sorted by group, against the group's rows of
+// each weight (w[i].M: rows of one group); offsets [groups + 1], order NULL
+// where the activations lie in sorted order already, else row order[p] / k
+// belongs to place p. N: places, at most.
+struct ExpertArgs {
+    StripWeight w[kMaxWeights];
+    int count;
+    const int8_t *q;
+    const float *ascale;
+    const int *offsets, *order;
+    int N, groups, k, K, group, block, scale_enc, y_bf16;
+};
+int launch_experts(const ExpertArgs &a, hipStream_t st);
+
+// The plan that sorts N slots by group (kxw4_rows.hip); hist: scratch of the
+// large plans, [blocks][groups + 1].
+struct RouteArgs {
+    const void *ids;
+    int *offsets, *order, *position, *hist;
+    int ids64, N, groups;
+    int per_block;                    // (set by the launcher)
+};
+int route_blocks_of(int N, int *per_block);
+int launch_route(RouteArgs &a, hipStream_t st);
+
+// Rows of H elements: x by token, rows by sorted place.
+struct RowArgs {
+    const void *x;                    // dispatch: source; combine backward: dy
+    void *rows;                       // dispatch: written, else read
+    void *y;                          // combine: the sums; backward: drows
+    const float *weights;
+    float *dweights;
+    const int *position;
+    int T, k, H;
+    int pieces;                       // accesses per row (set by the launcher)
+};
+int launch_dispatch(RowArgs &a, int elem_bytes, hipStream_t st);
+int launch_combine(RowArgs &a, bool rows_bf16, bool y_bf16, hipStream_t st);
+int launch_combine_backward(RowArgs &a, bool dy_bf16, bool rows_bf16, hipStream_t st);
+
+// Low-rank adapters (kxw4_adapter.hip): a [n][r][K], b [n][M][r] BF16.
+struct AdapterArgs {
+    const void *y, *x;
+    void *out;
+    const uint16_t *a, *b;
+    const float *scale;
+    float *low;                       // scratch [splits][T][r]
+    const int *offsets, *order;
+    int T, n, r, K, M;
+    int splits;                       // (set by the launcher)
+};
+int adapter_splits(int n, int T, int K);
+int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st);
+
 // Returns 1 (nothing launched) outside the per-token, one-split-per-token mode.
 int launch_gemm3(GemmArgs &a, hipStream_t st);
 // Returns 1 (nothing launched) outside the reference mode (K32 activation

@@ -21,6 +21,12 @@ of the reference's library-global scratch:
     x_quantize_act_chunk_s4           quantize_act_s4
     x_gemm_w4a4                       gemm_w4a4
 
+Rows with a weight of their own have no counterpart there (one dense model
+without adapters): route_rows sorts the rows of a batch by expert or adapter,
+dispatch_rows and combine_rows (with their gradients) move rows there and back,
+expert_gemm[_fanout] projects each by its expert, adapter_add adds a low-rank
+adapter per request to a projection's output.
+
 Torch provides device memory and the current stream only; every kernel is
 the HIP code in libkxw4.so, reached through ctypes. Tensors must live on a
 GPU; nothing here falls back to the CPU.
@@ -482,6 +488,233 @@ def gemm_w4a4(w: W4Weight, a: QuantActS4, dtype=torch.float32, residual=None,
         C.byref(wc), _ptr(a.q4), _ptr(a.scale), _ptr(a.sum), a.T, _ptr(y), _dtype_code(dtype),
         _ptr(residual), _stream()))
     return y
+
+
+# ---- rows with a weight of their own -------------------------------------
+
+
+def _gpu(t, name: str) -> torch.device:
+    """The GPU of a call's first tensor, which the others have to share."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    return t.device
+
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """Call `name` on the current stream of `device`, which need not be the
+    current device."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        check(name, getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i)))
+    else:
+        with torch.cuda.device(i):
+            check(name, getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i)))
+
+
+_FLOATS = (torch.float32, torch.bfloat16)
+_IDS = (torch.int32, torch.int64)
+
+
+@dataclass
+class RowRoute:
+    """The plan that sorts a batch's slots (token t, choice j, slot t*k + j) by
+    the group each names: an expert, or an adapter (k = 1). Made by route_rows
+    and shared by every call of a step, its backward pass among them; the calls
+    trust its contents."""
+    T: int
+    k: int
+    groups: int
+    offsets: torch.Tensor    # int32 [groups + 1]: group e's places are offsets[e]:offsets[e + 1]
+    order: torch.Tensor      # int32 [T*k]: the slot at each place, those without a group last
+    position: torch.Tensor   # int32 [T][k]: the place of each slot, -1 without a group
+
+    def c(self) -> _lib.Route:
+        return _lib.Route(self.T, self.k, self.groups, self.offsets.data_ptr(), self.order.data_ptr(),
+                          self.position.data_ptr())
+
+    @classmethod
+    def empty(cls, T: int, k: int, groups: int, device="cuda") -> "RowRoute":
+        def ints(*shape):
+            return torch.empty(*shape, dtype=torch.int32, device=device)
+        return cls(T, k, groups, ints(groups + 1), ints(T * k), ints(T, k))
+
+
+def _check_route(r: RowRoute, device) -> RowRoute:
+    if not isinstance(r, RowRoute):
+        raise ValueError("route must be a RowRoute")
+    _need(r.offsets, "route offsets", torch.int32, (r.groups + 1,), device)
+    _need(r.order, "route order", torch.int32, (r.T * r.k,), device)
+    _need(r.position, "route position", torch.int32, (r.T, r.k), device)
+    return r
+
+
+def route_rows(ids: torch.Tensor, groups: int, out: Optional[RowRoute] = None) -> RowRoute:
+    """Sort the slots of ids ([T][k] or [T], int32 or int64) by group, stably.
+    An id outside [0, groups) names no group. `out` (same T, k, groups) is
+    reused when given."""
+    dev = _gpu(ids, "ids")
+    if ids.dim() not in (1, 2) or (ids.dim() == 2 and ids.shape[1] < 1):
+        raise ValueError(f"ids must have shape (T,) or (T, k), got {tuple(ids.shape)}")
+    _need(ids, "ids", _IDS, ids.shape, dev)
+    T, k = ids.shape if ids.dim() == 2 else (ids.shape[0], 1)
+    if not 1 <= groups <= 1024:
+        raise ValueError(f"groups must be 1 to 1024, got {groups}")
+    if out is not None:
+        if (out.T, out.k, out.groups) != (T, k, groups):
+            raise ValueError("out does not match the ids' shape / groups")
+        r = _check_route(out, dev)
+    else:
+        r = RowRoute.empty(T, k, groups, dev)
+    nbytes = lib().kxw4_route_workspace(T, k, groups)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = r.c()
+    _launch("kxw4_route_rows", dev, ids.data_ptr(), ids.dtype is torch.int64, C.byref(rc), _ptr(ws))
+    return r
+
+
+def dispatch_rows(x: torch.Tensor, route: RowRoute, out=None) -> torch.Tensor:
+    """The rows of x [T][H] (f32 / bf16) in the plan's order: [T*k][H], of
+    which the first offsets[groups] are written. For expert_gemm no such copy
+    is needed: it reads the tokens' rows where they are."""
+    dev = _gpu(x, "x")
+    _check_route(route, dev)
+    if x.dim() != 2:
+        raise ValueError("x must have shape (T, H)")
+    T, H = x.shape
+    _need(x, "x", _FLOATS, (route.T, H), dev)
+    N = route.T * route.k
+    rows = _need(out, "out", x.dtype, (N, H), dev) if out is not None else torch.empty(N, H, dtype=x.dtype, device=dev)
+    if N:
+        rc = route.c()
+        _launch("kxw4_dispatch_rows", dev, x.data_ptr(), _dtype_code(x.dtype), H, C.byref(rc), rows.data_ptr())
+    return rows
+
+
+def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Tensor] = None, dtype=None,
+                 out=None) -> torch.Tensor:
+    """y[t] = sum_j weights[t, j] * rows[position[t, j]] of rows [T*k][H] (f32
+    / bf16), summed in FP32; weights [T][k] f32, all 1 when None. y [T][H] is
+    of `dtype` (the rows' by default)."""
+    dev = _gpu(rows, "rows")
+    _check_route(route, dev)
+    if rows.dim() != 2:
+        raise ValueError("rows must have shape (T*k, H)")
+    H = rows.shape[1]
+    _need(rows, "rows", _FLOATS, (route.T * route.k, H), dev)
+    if weights is not None:
+        _need(weights, "weights", torch.float32, (route.T, route.k), dev)
+    y = _out(route.T, H, dtype or (out.dtype if out is not None else rows.dtype), dev, out)
+    if route.T:
+        rc = route.c()
+        _launch("kxw4_combine_rows", dev, rows.data_ptr(), _dtype_code(rows.dtype), H, _ptr(weights), C.byref(rc),
+                y.data_ptr(), _dtype_code(y.dtype))
+    return y
+
+
+def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, route: RowRoute, weights: torch.Tensor, out=None):
+    """The gradients of combine_rows: (of rows [T*k][H], in rows' type and, up
+    to offsets[groups], written to `out` when given; of weights [T][k], f32, 0
+    for a slot without a group)."""
+    dev = _gpu(rows, "rows")
+    _check_route(route, dev)
+    if rows.dim() != 2:
+        raise ValueError("rows must have shape (T*k, H)")
+    N, H = route.T * route.k, rows.shape[1]
+    _need(rows, "rows", _FLOATS, (N, H), dev)
+    _need(dy, "dy", _FLOATS, (route.T, H), dev)
+    _need(weights, "weights", torch.float32, (route.T, route.k), dev)
+    drows = _need(out, "out", rows.dtype, (N, H), dev) if out is not None else torch.empty_like(rows)
+    dweights = torch.empty(route.T, route.k, dtype=torch.float32, device=dev)
+    if N:
+        rc = route.c()
+        _launch("kxw4_combine_rows_backward", dev, dy.data_ptr(), _dtype_code(dy.dtype), rows.data_ptr(),
+                _dtype_code(rows.dtype), H, weights.data_ptr(), C.byref(rc), drows.data_ptr(), dweights.data_ptr())
+    return drows, dweights
+
+
+def dispatch_rows_backward(drows: torch.Tensor, route: RowRoute, dtype=None, out=None) -> torch.Tensor:
+    """The gradient of dispatch_rows: dx[t] = sum_j drows[position[t, j]]."""
+    return combine_rows(drows, route, None, dtype, out)
+
+
+def expert_gemm_fanout(ws: Sequence[W4Weight], a: QuantAct, route: RowRoute, dtype=torch.float32,
+                       sorted_rows: bool = False, outs=None):
+    """Up to 4 weights (an expert's gate and up) over one activation, each row
+    projected by its expert: outputs [T*k][rows] in the plan's order, of which
+    the first offsets[groups] rows are written. A weight stacks the experts'
+    rows: W4Weight.from_codes of [groups * rows][K] codes. `a` holds the T
+    tokens, or with sorted_rows the T*k rows in the plan's order (the hidden
+    rows of a down projection)."""
+    dev = ws[0].codes.device
+    for w in ws:
+        _check_weight(w, dev)
+        if w.M % route.groups:
+            raise ValueError(f"weight rows {w.M} are not a multiple of {route.groups} groups")
+    _check_route(route, dev)
+    _check_act(a, dev)
+    N = route.T * route.k
+    if a.T != (N if sorted_rows else route.T):
+        raise ValueError(f"the activation has {a.T} rows for {N if sorted_rows else route.T} of the plan")
+    if outs is not None and len(outs) != len(ws):
+        raise ValueError(f"outs has {len(outs)} tensors for {len(ws)} weights")
+    ys = [_out(N, w.M // route.groups, dtype, dev, None if outs is None else outs[i], f"outs[{i}]")
+          for i, w in enumerate(ws)]
+    keep, warr = _weight_array(ws)
+    yarr = (C.c_void_p * len(ws))(*[y.data_ptr() for y in ys])
+    ac, rc = a.c(), route.c()
+    _launch("kxw4_expert_gemm", dev, warr, yarr, len(ws), C.byref(ac), C.byref(rc), bool(sorted_rows),
+            _dtype_code(dtype))
+    return ys
+
+
+def expert_gemm(w: W4Weight, a: QuantAct, route: RowRoute, dtype=torch.float32, sorted_rows: bool = False,
+                out=None) -> torch.Tensor:
+    """One weight of expert_gemm_fanout."""
+    return expert_gemm_fanout([w], a, route, dtype, sorted_rows, None if out is None else [out])[0]
+
+
+@dataclass
+class Adapters:
+    """n low-rank adapters of one projection [M][K]: a [n][r][K] and b
+    [n][M][r] bfloat16, scale [n] float32. r is a multiple of 8, up to 256;
+    smaller ranks are padded with zeros."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: torch.Tensor
+
+    def c(self) -> _lib.AdapterSet:
+        n, r, K = self.a.shape
+        return _lib.AdapterSet(n, r, K, self.b.shape[1], self.a.data_ptr(), self.b.data_ptr(),
+                               self.scale.data_ptr())
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: RowRoute, out=None) -> torch.Tensor:
+    """y[t] + scale_e * b_e (a_e x[t]) for the adapter e of each token t (y[t]
+    for a token without one): y [T][M] the projection's output and x [T][K] its
+    input (f32 / bf16 each), route of one adapter id per token. `out` may be y
+    itself; else it must not overlap it."""
+    dev = _gpu(y, "y")
+    if adapters.a.dim() != 3 or adapters.b.dim() != 3:
+        raise ValueError("adapters must have shapes (n, r, K) and (n, M, r)")
+    n, r, K = adapters.a.shape
+    M = adapters.b.shape[1]
+    _check_route(route, dev)
+    if route.groups != n or route.k != 1:
+        raise ValueError(f"the plan has {route.groups} groups and k {route.k} for {n} adapters")
+    T = route.T
+    _need(y, "y", _FLOATS, (T, M), dev)
+    _need(x, "x", _FLOATS, (T, K), dev)
+    _need(adapters.a, "adapters.a", torch.bfloat16, (n, r, K), dev)
+    _need(adapters.b, "adapters.b", torch.bfloat16, (n, M, r), dev)
+    _need(adapters.scale, "adapters.scale", torch.float32, (n,), dev)
+    o = _need(out, "out", y.dtype, (T, M), dev) if out is not None else torch.empty_like(y)
+    ad, rc = adapters.c(), route.c()
+    ws = torch.empty(lib().kxw4_adapter_workspace(C.byref(ad), T), dtype=torch.uint8, device=dev)
+    _launch("kxw4_adapter_add", dev, y.data_ptr(), _dtype_code(y.dtype), x.data_ptr(), _dtype_code(x.dtype),
+            C.byref(ad), C.byref(rc), o.data_ptr(), ws.data_ptr())
+    return o
 
 
 class TqfFile:

@@ -1,0 +1,161 @@
+"""Refusals of the row routing, expert and adapter calls: argument checks of
+the C ABI and of the torch front end, made before any HIP call."""
+import ctypes as C
+
+import pytest
+import torch
+
+from knivesysl_xe_amd import _lib, ops
+
+P = C.c_void_p(64)
+
+
+def R(T=8, k=2, groups=4, offsets=64, order=64, position=64):
+    return _lib.Route(T, k, groups, offsets, order, position)
+
+
+def W(M=256, K=1024, group=128, enc=0, codes=64, scales=64):
+    return _lib.Weight(M, K, group, enc, codes, scales)
+
+
+def A(T=8, K=1024, block=0, q=64, scale=64, s=64):
+    return _lib.Act(T, K, block, q, scale, s)
+
+
+def D(n=4, r=16, K=1024, M=256, a=64, b=64, scale=64):
+    return _lib.AdapterSet(n, r, K, M, a, b, scale)
+
+
+def test_route_refuses_bad_plans():
+    f = _lib.lib().kxw4_route_rows
+    assert f(P, 0, None, None, None) == _lib.EARG
+    assert f(None, 0, C.byref(R()), None, None) == _lib.EARG
+    for missing in ("offsets", "order", "position"):
+        assert f(P, 0, C.byref(R(**{missing: None})), None, None) == _lib.EARG
+    for bad in (dict(T=-1), dict(k=0), dict(groups=0), dict(groups=1025), dict(T=1 << 30, k=2)):
+        assert f(P, 0, C.byref(R(**bad)), None, None) == _lib.ESHAPE
+    # a large plan needs its scratch
+    assert f(P, 0, C.byref(R(T=1 << 20)), None, None) == _lib.EARG
+
+
+def test_route_workspace_sizes():
+    size = _lib.lib().kxw4_route_workspace
+    assert size(8, 2, 4) == 0 and size(16384, 1, 4) == 0 and size(0, 1, 4) == 0
+    assert size(16385, 1, 4) == (16385 + 2047) // 2048 * 5 * 4
+    assert size(1 << 20, 8, 128) == 256 * 129 * 4
+    assert size(8, 2, 0) == 0 and size(-1, 2, 4) == 0 and size(1 << 30, 2, 4) == 0
+
+
+def test_row_calls_refuse_bad_arguments():
+    L = _lib.lib()
+
+    def dispatch(x=P, dtype=0, H=64, r=R(), rows=P):
+        return L.kxw4_dispatch_rows(x, dtype, H, None if r is None else C.byref(r), rows, None)
+
+    def combine(rows=P, rt=0, H=64, w=P, r=R(), y=P, yt=0):
+        return L.kxw4_combine_rows(rows, rt, H, w, None if r is None else C.byref(r), y, yt, None)
+
+    def backward(dy=P, dt=0, rows=P, rt=0, H=64, w=P, r=R(), drows=P, dw=P):
+        return L.kxw4_combine_rows_backward(dy, dt, rows, rt, H, w, None if r is None else C.byref(r), drows, dw, None)
+
+    for call in (dispatch, combine, backward):
+        assert call(r=None) == _lib.EARG
+        assert call(r=R(offsets=None)) == call(r=R(order=None)) == call(r=R(position=None)) == _lib.EPREP
+        assert call(r=R(k=0)) == call(r=R(T=-3)) == call(r=R(groups=2000)) == _lib.ESHAPE
+        assert call(H=0) == call(H=-8) == _lib.ESHAPE
+        # no tokens: nothing to read or write, whatever the pointers
+        assert call(r=R(T=0, offsets=None, order=None, position=None)) == 0
+    assert dispatch(dtype=2) == combine(rt=2) == combine(yt=-1) == backward(dt=3) == backward(rt=3) == _lib.ESHAPE
+    odd = C.c_void_p(65)
+    assert dispatch(x=None) == dispatch(rows=None) == dispatch(x=odd) == dispatch(rows=odd) == _lib.EARG
+    assert combine(rows=None) == combine(y=None) == combine(rows=odd) == combine(y=odd) == combine(w=odd) == _lib.EARG
+    for name in ("dy", "rows", "w", "drows", "dw"):
+        assert backward(**{name: None}) == backward(**{name: odd}) == _lib.EARG
+
+
+def test_expert_gemm_refuses_bad_arguments():
+    f = _lib.lib().kxw4_expert_gemm
+
+    def call(ws=(W(),), a=A(), r=R(), in_order=0, dtype=0, y=64, count=None):
+        arr = (C.POINTER(_lib.Weight) * len(ws))(*[C.pointer(w) for w in ws])
+        ys = (C.c_void_p * len(ws))(*[y] * len(ws))
+        return f(arr, ys, len(ws) if count is None else count, None if a is None else C.byref(a),
+                 None if r is None else C.byref(r), in_order, dtype, None)
+
+    assert f(None, None, 1, C.byref(A()), C.byref(R()), 0, 0, None) == _lib.EARG
+    assert call(count=0) == call(count=5) == call(a=None) == call(r=None) == call(y=None) == _lib.EARG
+    assert call(ws=(W(codes=None),)) == _lib.EARG
+    assert call(r=R(order=None)) == _lib.EPREP
+    assert call(a=A(q=None)) == call(a=A(scale=None)) == _lib.EPREP
+    # rows that the groups do not divide into 16-row slices, mixed weights
+    assert call(r=R(groups=3)) == call(ws=(W(M=32),)) == _lib.ESHAPE
+    assert call(ws=(W(), W(K=2048))) == call(ws=(W(), W(group=64))) == _lib.ESHAPE
+    # activation rows: T, or T * k in sorted order
+    assert call(a=A(T=16)) == call(in_order=1) == call(a=A(K=512)) == call(a=A(block=16)) == call(dtype=4) == _lib.ESHAPE
+    # offsets past 31 bits
+    assert call(a=A(T=1 << 22), r=R(T=1 << 22)) == _lib.ESHAPE
+    # tiers that are not built for experts
+    assert call(ws=(W(group=32),)) == call(ws=(W(enc=1),)) == call(a=A(block=32)) == _lib.ETIER
+    assert call(ws=(W(group=128, enc=1),), a=A(block=32)) == call(ws=(W(group=16, enc=1),), a=A(block=32)) == _lib.ETIER
+    assert call(ws=(W(group=32, enc=2),)) == _lib.ETIER                  # W8 has K32 activation blocks
+    assert call(r=R(T=0, offsets=None, order=None, position=None), a=A(T=0, q=None, scale=None), y=None) == 0
+
+
+def test_adapter_add_refuses_bad_arguments():
+    L = _lib.lib()
+
+    def call(y=P, yt=1, x=P, xt=1, ad=D(), r=R(k=1), out=P, ws=P):
+        return L.kxw4_adapter_add(y, yt, x, xt, None if ad is None else C.byref(ad), None if r is None else C.byref(r),
+                                  out, ws, None)
+
+    assert call(ad=None) == call(r=None) == _lib.EARG
+    assert call(r=R()) == call(r=R(k=1, groups=5)) == _lib.ESHAPE        # k = 2; another number of adapters
+    for bad in (dict(r=0), dict(r=12), dict(r=264), dict(K=1000), dict(K=0), dict(M=250), dict(M=0)):
+        assert call(ad=D(**bad)) == _lib.ESHAPE
+    assert call(yt=2) == call(xt=2) == _lib.ESHAPE
+    odd = C.c_void_p(72)
+    for name in ("y", "x", "out", "ws"):
+        assert call(**{name: None}) == call(**{name: odd}) == _lib.EARG
+    for name in ("a", "b", "scale"):
+        assert call(ad=D(**{name: None})) == _lib.EARG
+    assert call(ad=D(a=72)) == call(ad=D(b=72)) == call(ad=D(scale=66)) == _lib.EARG
+    assert call(r=R(T=0, k=1, offsets=None, order=None, position=None), y=None, x=None, out=None, ws=None) == 0
+    size = L.kxw4_adapter_workspace
+    assert size(None, 8) == 0 and size(C.byref(D()), 0) == 0
+    assert size(C.byref(D()), 8) % (8 * 16 * 4) == 0 and size(C.byref(D()), 8) >= 8 * 16 * 4
+
+
+def test_front_end_refuses_host_tensors():
+    x = torch.zeros(4, 64)
+    r = ops.RowRoute.empty(4, 2, 8, "cpu")
+    with pytest.raises(ValueError, match="ids must be on the GPU"):
+        ops.route_rows(torch.zeros(4, 2, dtype=torch.int32), 8)
+    with pytest.raises(ValueError, match="x must be on the GPU"):
+        ops.dispatch_rows(x, r)
+    with pytest.raises(ValueError, match="rows must be on the GPU"):
+        ops.combine_rows(x, r)
+    with pytest.raises(ValueError, match="rows must be on the GPU"):
+        ops.combine_rows_backward(x, x, r, torch.zeros(4, 2))
+    with pytest.raises(ValueError, match="y must be on the GPU"):
+        ops.adapter_add(x, x, None, r)
+    with pytest.raises(ValueError, match="must be a torch.Tensor"):
+        ops.route_rows([[1, 2]], 8)
+    w = ops.W4Weight(64, 128, 128, 0, torch.zeros(64 * 64, dtype=torch.uint8), torch.zeros(64, dtype=torch.int16))
+    with pytest.raises(ValueError, match="weights must be on the GPU"):
+        ops.expert_gemm(w, ops.QuantAct.empty(4, 128, 0, "cpu"), r)
+
+
+def test_route_buffers_are_checked():
+    r = ops.RowRoute.empty(4, 2, 8, "cpu")
+    assert ops._check_route(r, torch.device("cpu")) is r
+    with pytest.raises(ValueError, match="must be a RowRoute"):
+        ops._check_route(None, torch.device("cpu"))
+    short = ops.RowRoute(4, 2, 9, r.offsets, r.order, r.position)
+    with pytest.raises(ValueError, match="route offsets must have shape"):
+        ops._check_route(short, torch.device("cpu"))
+    wide = ops.RowRoute(4, 2, 8, r.offsets, r.order.long(), r.position)
+    with pytest.raises(ValueError, match="route order must be torch.int32"):
+        ops._check_route(wide, torch.device("cpu"))
+    flat = ops.RowRoute(4, 2, 8, r.offsets, r.order, r.position.view(-1))
+    with pytest.raises(ValueError, match="route position must have shape"):
+        ops._check_route(flat, torch.device("cpu"))
