@@ -288,14 +288,13 @@ typedef struct kxw4_route {
 } kxw4_route_t;
 
 /* ids[T][k]: int32, or int64 where ids_64 is set. workspace:
- * kxw4_route_workspace bytes (0 up to 16,384 slots; then it may be NULL). */
+ * kxw4_route_workspace bytes (0 up to 8,192 slots; then it may be NULL). */
 size_t kxw4_route_workspace(int T, int k, int groups);
 int kxw4_route_rows(const void *ids, int ids_64, const kxw4_route_t *route, void *workspace, void *stream);
 
 /* rows[p] = x[order[p] / k] for the places of a group. x [T][H], rows [N][H]
  * of one type (KXW4_F32, KXW4_BF16); any H, and any alignment of the type's
- * own size (16-byte pieces where pointers and rows allow). The gradient of x
- * is kxw4_combine_rows without weights. */
+ * own size. The gradient of x is kxw4_combine_rows without weights. */
 int kxw4_dispatch_rows(const void *x, int dtype, int H, const kxw4_route_t *route, void *rows, void *stream);
 
 /* y[t] = sum over j of weights[t][j] * rows[position[t][j]] (weights NULL: all

@@ -523,7 +523,7 @@ int kxw4_dispatch_rows(const void *x, int dtype, int H, const kxw4_route_t *rout
     a.T = route->T;
     a.k = route->k;
     a.H = H;
-    return launch_dispatch(a, elem_bytes(dtype), as_stream(stream));
+    return launch_dispatch(a, dtype == KXW4_BF16, as_stream(stream));
 }
 
 int kxw4_combine_rows(const void *rows, int rows_dtype, int H, const float *weights, const kxw4_route_t *route,

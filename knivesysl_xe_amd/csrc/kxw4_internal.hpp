@@ -206,9 +206,9 @@ struct RowArgs {
     float *dweights;
     const int *position;
     int T, k, H;
-    int pieces;                       // accesses per row (set by the launcher)
+    int pieces, lanes, per, chunks, past;       // (set by the launcher)
 };
-int launch_dispatch(RowArgs &a, int elem_bytes, hipStream_t st);
+int launch_dispatch(RowArgs &a, bool bf16, hipStream_t st);
 int launch_combine(RowArgs &a, bool rows_bf16, bool y_bf16, hipStream_t st);
 int launch_combine_backward(RowArgs &a, bool dy_bf16, bool rows_bf16, hipStream_t st);
 

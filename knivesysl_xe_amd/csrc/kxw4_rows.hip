@@ -21,27 +21,55 @@ namespace kxw4 {
 
 // ---- the plan --------------------------------------------------------------
 
-constexpr int kPlanWaves = 8, kPlanThreads = 64 * kPlanWaves;
+constexpr int kPlanWaves = 16, kPlanThreads = 64 * kPlanWaves;       // at most
+constexpr int kPlanAhead = 8;                                // keys of a lane requested together (one in plans of up to 1,024)
+constexpr int kPlanOne = kPlanThreads * kPlanAhead;          // slots of a plan in one block
 
-// Group of slot s, `groups` for none. (64-bit ids are compared before they
-// are narrowed.)
-__device__ __forceinline__ int slot_key(const RouteArgs &a, int s) {
-    if (a.ids64) {
-        const long long v = static_cast<const long long *>(a.ids)[s];
-        return v < 0 || v >= a.groups ? a.groups : (int)v;
-    }
-    const int v = static_cast<const int *>(a.ids)[s];
-    return v < 0 || v >= a.groups ? a.groups : v;
+// The keys of the AH 64-slot pieces from slot s0 < end on: a slot's
+// group, `groups` for none, -1 past the end. (64-bit ids are compared before
+// they are narrowed.)
+template <class Id, int AH>
+__device__ __forceinline__ void plan_keys_of(const Id *ids, int groups, int s0, int end, int lane, int (&key)[AH]) {
+    Id v[AH];
+#pragma unroll
+    for (int i = 0; i < AH; ++i) v[i] = ids[min(s0 + 64 * i + lane, end - 1)];
+#pragma unroll
+    for (int i = 0; i < AH; ++i)
+        key[i] = s0 + 64 * i + lane >= end ? -1 : v[i] < 0 || v[i] >= groups ? groups : (int)v[i];
 }
 
-// Counts of the keys in [b0, b1), by wave: wave w takes the w-th of kPlanWaves
-// consecutive runs of `per` slots. cnt: [waves][groups + 1], cleared here.
-__device__ __forceinline__ void plan_count(const RouteArgs &a, int b0, int b1, int per, int *cnt) {
+template <int AH>
+__device__ __forceinline__ void plan_keys(const RouteArgs &a, int s0, int end, int lane, int (&key)[AH]) {
+    if (s0 >= end) {
+#pragma unroll
+        for (int i = 0; i < AH; ++i) key[i] = -1;
+    } else if (a.ids64) {
+        plan_keys_of(static_cast<const long long *>(a.ids), a.groups, s0, end, lane, key);
+    } else {
+        plan_keys_of(static_cast<const int *>(a.ids), a.groups, s0, end, lane, key);
+    }
+}
+
+// Counts of the keys in [b0, b1), by wave: wave w takes the w-th of the block's
+// consecutive runs of `per` slots. cnt: [waves][groups + 1], cleared here; key:
+// the wave's last piece of its run.
+template <int AH>
+__device__ __forceinline__ void plan_count(const RouteArgs &a, int b0, int b1, int per, int *cnt, int (&key)[AH]) {
     const int G1 = a.groups + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < kPlanWaves * G1; i += kPlanThreads) cnt[i] = 0;
+    const int w0 = b0 + wave * per, w1 = min(b1, w0 + per);
+    plan_keys(a, w0, w1, lane, key);
+    for (int i = tid; i < (int)(blockDim.x / 64) * G1; i += blockDim.x) cnt[i] = 0;
     __syncthreads();
-    const int w1 = min(b1, b0 + (wave + 1) * per);
-    for (int s = b0 + wave * per + lane; s < w1; s += 64) atomicAdd(&cnt[wave * G1 + slot_key(a, s)], 1);
+    for (int s0 = w0;;) {
+#pragma unroll
+        for (int i = 0; i < AH; ++i) {
+            if (s0 + 64 * i >= w1) break;
+            if (key[i] >= 0) atomicAdd(&cnt[wave * G1 + key[i]], 1);
+        }
+        s0 += 64 * AH;
+        if (s0 >= w1) break;
+        plan_keys(a, s0, w1, lane, key);
+    }
     __syncthreads();
 }
 
@@ -49,10 +77,12 @@ __device__ __forceinline__ void plan_count(const RouteArgs &a, int b0, int b1, i
 __global__ __launch_bounds__(kPlanThreads) void plan_hist_kernel(const RouteArgs a) {
     extern __shared__ int cnt[];
     const int G1 = a.groups + 1, b0 = blockIdx.x * a.per_block, b1 = min(a.N, b0 + a.per_block);
-    plan_count(a, b0, b1, a.per_block / kPlanWaves, cnt);
+    int key[kPlanAhead];
+    plan_count(a, b0, b1, a.per_block / kPlanWaves, cnt, key);
     for (int g = threadIdx.x; g < G1; g += kPlanThreads) {
         int sum = 0;
-        for (int w = 0; w < kPlanWaves; ++w) sum += cnt[w * G1 + g];
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) sum += cnt[w * G1 + g];     // (kPlanWaves in a block of these)
         a.hist[(size_t)blockIdx.x * G1 + g] = sum;
     }
 }
@@ -61,29 +91,41 @@ __global__ __launch_bounds__(kPlanThreads) void plan_hist_kernel(const RouteArgs
 // its own run of slots again, adds up the blocks before it, and places its
 // slots. Within a wave the slots of one key find their rank by comparing keys
 // bit by bit over the lanes, so the sort is stable and no order of atomics
-// shows. A plan of 64 to 16,384 slots is a chain of a few memory and LDS
-// round trips.
+// shows. What bounds it is the chain of round trips to memory and LDS: a
+// lane's keys and a key's block counts are requested eight at a time.
+template <int AH>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const RouteArgs a) {
     extern __shared__ int cnt[];                             // [waves][groups + 1], then [groups + 1] totals
     const int G = a.groups, G1 = G + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int *tot = cnt + kPlanWaves * G1;
-    const int b0 = blockIdx.x * a.per_block, b1 = min(a.N, b0 + a.per_block), per = a.per_block / kPlanWaves;
-    plan_count(a, b0, b1, per, cnt);
+    const int waves = blockDim.x / 64;
+    int *tot = cnt + waves * G1;
+    const int b0 = blockIdx.x * a.per_block, b1 = min(a.N, b0 + a.per_block), per = a.per_block / waves;
+    int key[AH];
+    plan_count(a, b0, b1, per, cnt, key);
     // cnt becomes each wave's first place within its key's slots, tot the
     // key's slots over all blocks
-    for (int g = tid; g < G1; g += kPlanThreads) {
+    const int nb = gridDim.x;
+    for (int g = tid; g < G1; g += blockDim.x) {
         int before = 0, all = 0;
-        for (int b = 0; b < (int)gridDim.x && gridDim.x > 1; ++b) {
-            const int h = a.hist[(size_t)b * G1 + g];
-            before += b < (int)blockIdx.x ? h : 0;
-            all += h;
+        for (int q = 0; q < nb && nb > 1; q += 8) {
+            int h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = q + i < nb ? a.hist[(size_t)(q + i) * G1 + g] : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                before += q + i < (int)blockIdx.x ? h[i] : 0;
+                all += h[i];
+            }
         }
+        int c[kPlanWaves];
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) c[w] = w < waves ? cnt[w * G1 + g] : 0;
+#pragma unroll
         for (int w = 0; w < kPlanWaves; ++w) {
-            const int c = cnt[w * G1 + g];
-            cnt[w * G1 + g] = before;
-            before += c;
+            if (w < waves) cnt[w * G1 + g] = before;
+            before += c[w];
         }
-        tot[g] = gridDim.x > 1 ? all : before;
+        tot[g] = nb > 1 ? all : before;
     }
     __syncthreads();
     // exclusive scan of the totals: lane l takes a run of keys
@@ -105,164 +147,224 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const RouteArgs a) {
         }
     }
     __syncthreads();
-    int bits = 32 - __builtin_clz(G);                        // (keys run to G itself)
+    const int bits = 32 - __builtin_clz(G);                  // (keys run to G itself)
     volatile int *mine = cnt + wave * G1;
-    const int w1 = min(b1, b0 + (wave + 1) * per);
-    for (int s0 = b0 + wave * per; s0 < w1; s0 += 64) {
-        const int s = s0 + lane;
-        const bool on = s < w1;
-        const int key = on ? slot_key(a, s) : 0;
-        unsigned long long same = __ballot(on);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long one = __ballot(key >> b & 1);
-            same &= (key >> b & 1) ? one : ~one;
+    const int w0 = b0 + wave * per, w1 = min(b1, w0 + per);
+    for (int s0 = w0; s0 < w1; s0 += 64 * AH) {
+        if (per > 64 * AH) plan_keys(a, s0, w1, lane, key);      // (a run of one piece still holds its keys)
+#pragma unroll
+        for (int i = 0; i < AH; ++i) {
+            if (s0 + 64 * i >= w1) break;
+            const int s = s0 + 64 * i + lane, kk = key[i];
+            const bool on = kk >= 0;
+            unsigned long long same = __ballot(on);
+            for (int b = 0; b < bits; ++b) {
+                const unsigned long long one = __ballot(kk >> b & 1);
+                same &= (kk >> b & 1) ? one : ~one;
+            }
+            const unsigned long long below = same & ((1ull << lane) - 1);
+            if (on) {
+                const int place = tot[kk] + mine[kk] + __popcll(below);
+                a.order[place] = s;
+                a.position[s] = kk < G ? place : -1;
+            }
+            // (the wave's reads above come before this write: LDS accesses of
+            // one wave complete in order)
+            __builtin_amdgcn_wave_barrier();
+            if (on && below == 0) mine[kk] = mine[kk] + __popcll(same);
+            __builtin_amdgcn_wave_barrier();
         }
-        const unsigned long long below = same & ((1ull << lane) - 1);
-        if (on) {
-            const int first = mine[key], place = tot[key] + first + __popcll(below);
-            a.order[place] = s;
-            a.position[s] = key < G ? place : -1;
-        }
-        // (the wave's reads above come before this write: LDS accesses of one
-        // wave complete in order)
-        __builtin_amdgcn_wave_barrier();
-        if (on && below == 0) mine[key] = mine[key] + __popcll(same);
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
-// Slots per block: one block up to 16,384, else at most 256 blocks of a
-// multiple of 512.
+// Slots per block: one block up to kPlanOne, past which the scattered writes
+// of `order` by one CU cost more than a second launch; else blocks of 2,048 up
+// to 256 of them, then larger ones. A small plan's block has a wave for each
+// 64 slots.
+static int plan_round(long long v, int to) { return (int)((v + to - 1) / to * to); }
 int route_blocks_of(int N, int *per_block) {
-    constexpr int kOne = 16384, kLeast = 2048;
-    auto round = [](long long v) { return (int)((v + kPlanThreads - 1) / kPlanThreads * kPlanThreads); };
-    if (N <= kOne) {
-        *per_block = std::max(kPlanThreads, round(N));
+    if (N <= kPlanOne) {
+        *per_block = std::max(64, plan_round(N, N < kPlanThreads ? 64 : kPlanThreads));
         return 1;
     }
-    *per_block = std::max(kLeast, round((N + 255) / 256));
+    *per_block = std::max(2 * kPlanThreads, plan_round((N + 255) / 256, kPlanThreads));
     return (N + *per_block - 1) / *per_block;
 }
 
 int launch_route(RouteArgs &a, hipStream_t st) {
     const int nb = route_blocks_of(a.N, &a.per_block), G1 = a.groups + 1;
-    const size_t lds = (size_t)(kPlanWaves + 1) * G1 * sizeof(int);       // (at most 36.9 KB: 1,024 groups)
+    const int waves = std::min(a.per_block / 64, kPlanWaves);
+    const size_t lds = (size_t)(waves + 1) * G1 * sizeof(int);            // (at most 69.7 KB: 1,024 groups)
+    static bool attr[64] = {};                               // (the attribute is per device)
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return -6;
+    if (!attr[dev]) {
+        for (const void *k : {reinterpret_cast<const void *>(plan_hist_kernel), reinterpret_cast<const void *>(plan_kernel<1>),
+                              reinterpret_cast<const void *>(plan_kernel<kPlanAhead>)})
+            if (hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024) != hipSuccess) return -6;
+        attr[dev] = true;
+    }
     if (nb > 1) {
         if (!a.hist) return -1;
         hipLaunchKernelGGL(plan_hist_kernel, dim3(nb), dim3(kPlanThreads), lds, st, a);
     }
-    hipLaunchKernelGGL(plan_kernel, dim3(nb), dim3(kPlanThreads), lds, st, a);
+    hipLaunchKernelGGL(a.N <= kPlanThreads ? plan_kernel<1> : plan_kernel<kPlanAhead>, dim3(nb), dim3(64 * waves), lds, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 // ---- rows ------------------------------------------------------------------
+//
+// A thread owns a piece of a row: the 16 bytes that V elements of the rows'
+// type take. Rows of any length and alignment take the same instructions: the
+// hardware reads and writes 16 bytes at any address of whole elements, and the
+// last piece of a row ends at its end, over the piece before it (two threads
+// write the same values there). Only rows shorter than a piece go element by
+// element. H = 2049, float32, 8,000 rows: dispatch 27 -> 19 us, combine 27 ->
+// 19 (4 bytes a thread before).
 
 constexpr int kRowThreads = 256;
 
-template <int V>
-struct Raw;                                                  // V bytes moved as one
-template <> struct Raw<16> { typedef v4u type; };
-template <> struct Raw<8> { typedef v2u type; };
-template <> struct Raw<4> { typedef uint32_t type; };
-template <> struct Raw<2> { typedef uint16_t type; };
+// V elements at `at`; SHORT: of a row that may have only n of them.
+template <int V, bool BF, bool SHORT>
+struct Piece {
+    static constexpr int BYTES = V * (BF ? 2 : 4);
+    static constexpr int WORDS = BYTES / 4;
+    typedef uint32_t Words __attribute__((ext_vector_type(WORDS), aligned(BF ? 2 : 4)));
+    Words w;
+
+    __device__ __forceinline__ void load(const void *base, size_t at, int n) {
+        const uint8_t *p = static_cast<const uint8_t *>(base) + at * (BF ? 2 : 4);
+        if (!SHORT || n >= V) {
+            w = __builtin_nontemporal_load(reinterpret_cast<const Words *>(p));
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (i >= n) continue;
+                if constexpr (BF) w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[i] << 16 * (i & 1);
+                else w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void *base, size_t at, int n, int past) const {
+        uint8_t *p = static_cast<uint8_t *>(base) + at * (BF ? 2 : 4);
+        if (!SHORT || n >= V) {
+            if (past) {
+                // (the empty statements keep the compiler from making one
+                // plain store of the two)
+                asm volatile("");
+                __builtin_nontemporal_store(w, reinterpret_cast<Words *>(p));
+                asm volatile("");
+            } else {
+                *reinterpret_cast<Words *>(p) = w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (i >= n) continue;
+                if constexpr (BF) reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> 16 * (i & 1));
+                else reinterpret_cast<uint32_t *>(p)[i] = w[i];
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (BF) return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        else return __uint_as_float(w[i]);
+    }
+    __device__ __forceinline__ void set(const float (&v)[V]) {       // one rounding each
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (BF) w[i] = round_bf16(v[2 * i]) | round_bf16(v[2 * i + 1]) << 16;
+            else w[i] = __float_as_uint(v[i]);
+        }
+    }
+};
+
+// The thread's token and piece. WIDE: a row takes `a.chunks` blocks, so the
+// token is the block's and its plan entries come through scalar loads; else a
+// block takes `a.per` tokens of `a.lanes` threads each.
+struct RowAt {
+    int t, c;
+};
+template <bool WIDE>
+__device__ __forceinline__ RowAt row_at(const RowArgs &a) {
+    const int block = blockIdx.x;
+    if constexpr (WIDE) {
+        const int t = block / a.chunks;
+        return {t, (block - t * a.chunks) * a.lanes + (int)threadIdx.x};
+    } else {
+        const int sub = threadIdx.x / a.lanes;
+        return {block * a.per + sub, (int)threadIdx.x - sub * a.lanes};
+    }
+}
+template <int V, bool SHORT>
+__device__ __forceinline__ int piece_at(int H, int c) { return SHORT && H < V ? 0 : min(c * V, H - V); }
 
 // rows[position[t, j]] = x[t]: a thread reads one piece of a token's row and
 // writes it to each of the token's places, so x is read once. Bound by the
 // writes.
-template <int V>
-__global__ __launch_bounds__(kRowThreads) void dispatch_kernel(const RowArgs a) {
-    typedef typename Raw<V>::type P;
-    const int pieces = a.pieces, bpr = (pieces + kRowThreads - 1) / kRowThreads;
-    const int t = blockIdx.x / bpr, c = (blockIdx.x - t * bpr) * kRowThreads + threadIdx.x;
-    if (c >= pieces) return;
-    const P v = static_cast<const P *>(a.x)[(size_t)t * pieces + c];
-    const int *pos = a.position + (size_t)t * a.k;
-    for (int j = 0; j < a.k; ++j) {
-        const int p = pos[j];
-        if (p >= 0) static_cast<P *>(a.rows)[(size_t)p * pieces + c] = v;
+template <bool BF, bool WIDE>
+__global__ __launch_bounds__(512) void dispatch_kernel(const RowArgs a) {
+    constexpr int V = BF ? 8 : 4;
+    const RowAt r = row_at<WIDE>(a);
+    if (r.t >= a.T || r.c >= a.pieces) return;
+    const int n = min(a.H, V), at = piece_at<V, !WIDE>(a.H, r.c);
+    Piece<V, BF, !WIDE> v;
+    v.load(a.x, (size_t)r.t * a.H + at, n);
+    const int *pos = a.position + (size_t)r.t * a.k;
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+        int p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = j0 + i < a.k ? pos[j0 + i] : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p[i] >= 0) v.store(a.rows, (size_t)p[i] * a.H + at, n, a.past);
     }
 }
 
-// V consecutive elements of a row as FP32, and back with one rounding.
-template <int V, bool BF>
-__device__ __forceinline__ void load_row(const void *base, size_t at, float (&v)[V]) {
-    if constexpr (BF && V == 8) {
-        const v4u u = *reinterpret_cast<const v4u *>(static_cast<const uint16_t *>(base) + at);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(u[i] << 16);
-            v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-        }
-    } else if constexpr (!BF && V == 8) {
-        const v4f *p = reinterpret_cast<const v4f *>(static_cast<const float *>(base) + at);
-        const v4f lo = p[0], hi = p[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = lo[i];
-            v[4 + i] = hi[i];
-        }
-    } else {
-        static_assert(V == 1, "one or eight elements");
-        v[0] = BF ? bf16_to_float(static_cast<const uint16_t *>(base)[at]) : static_cast<const float *>(base)[at];
-    }
-}
-
-template <int V, bool BF>
-__device__ __forceinline__ void store_row(void *base, size_t at, const float (&v)[V]) {
-    if constexpr (BF && V == 8) {
-        v4u u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = round_bf16(v[2 * i]) | round_bf16(v[2 * i + 1]) << 16;
-        *reinterpret_cast<v4u *>(static_cast<uint16_t *>(base) + at) = u;
-    } else if constexpr (!BF && V == 8) {
-        v4f *p = reinterpret_cast<v4f *>(static_cast<float *>(base) + at);
-        p[0] = v4f{v[0], v[1], v[2], v[3]};
-        p[1] = v4f{v[4], v[5], v[6], v[7]};
-    } else if constexpr (BF) {
-        static_cast<uint16_t *>(base)[at] = (uint16_t)round_bf16(v[0]);
-    } else {
-        static_cast<float *>(base)[at] = v[0];
-    }
-}
-
-// y[t] = sum_j w[t, j] rows[position[t, j]] (w 1 where none is given): a
-// thread owns V elements of a token's row; up to kAhead choices' pieces are
-// requested before the first is added. Bound by the reads.
-constexpr int kAhead = 4;
-template <int V, bool RB, bool YB>
-__global__ __launch_bounds__(kRowThreads) void combine_kernel(const RowArgs a) {
-    const int pieces = a.pieces, bpr = (pieces + kRowThreads - 1) / kRowThreads;
-    const int t = blockIdx.x / bpr, c = (blockIdx.x - t * bpr) * kRowThreads + threadIdx.x;
-    if (c >= pieces) return;
-    const int *pos = a.position + (size_t)t * a.k;
-    const float *w = a.weights ? a.weights + (size_t)t * a.k : nullptr;
+// y[t] = sum_j w[t, j] rows[position[t, j]] (w 1 where none is given): AH
+// choices' pieces are requested before the first is added, those of slots
+// without a group from row 0 (a load under a branch waits for the one before
+// it). Bound by the reads.
+template <bool RB, bool YB, bool WIDE, int AH>
+__global__ __launch_bounds__(512) void combine_kernel(const RowArgs a) {
+    constexpr int V = RB ? 8 : 4;
+    const RowAt r = row_at<WIDE>(a);
+    if (r.t >= a.T || r.c >= a.pieces) return;
+    const int n = min(a.H, V), at = piece_at<V, !WIDE>(a.H, r.c);
+    const int *pos = a.position + (size_t)r.t * a.k;
+    const float *w = a.weights ? a.weights + (size_t)r.t * a.k : nullptr;
     float acc[V] = {};
-    for (int j0 = 0; j0 < a.k; j0 += kAhead) {
-        float v[kAhead][V], wj[kAhead];
-        int p[kAhead];
+    for (int j0 = 0; j0 < a.k; j0 += AH) {
+        Piece<V, RB, !WIDE> v[AH];
+        float wj[AH];
+        int p[AH];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            p[i] = j0 + i < a.k ? pos[j0 + i] : -1;
-            wj[i] = w && j0 + i < a.k ? w[j0 + i] : 1.0f;
-        }
+        for (int i = 0; i < AH; ++i) p[i] = j0 + i < a.k ? pos[j0 + i] : -1;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            if (p[i] >= 0) load_row<V, RB>(a.rows, (size_t)p[i] * a.H + (size_t)c * V, v[i]);
+        for (int i = 0; i < AH; ++i) wj[i] = w && j0 + i < a.k ? w[j0 + i] : 1.0f;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
+        for (int i = 0; i < AH; ++i)
+            v[i].load(a.rows, (size_t)max(p[i], 0) * a.H + at, n);
+#pragma unroll
+        for (int i = 0; i < AH; ++i)
             if (p[i] >= 0)
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[e] = __builtin_fmaf(wj[i], v[i][e], acc[e]);
+                for (int e = 0; e < V; ++e) acc[e] = __builtin_fmaf(wj[i], v[i].get(e), acc[e]);
     }
-    store_row<V, YB>(a.y, (size_t)t * a.H + (size_t)c * V, acc);
+    Piece<V, YB, !WIDE> y;
+    y.set(acc);
+    y.store(a.y, (size_t)r.t * a.H + at, n, a.past);
 }
 
 // drows[position[t, j]] = w[t, j] dy[t], dw[t, j] = <dy[t], rows[position[t,
 // j]]>: one block per token and run of kDots choices, which reads dy once for
 // all of them. Bound by the rows read and written.
 constexpr int kDots = 4;
-template <int V, bool DB, bool RB>
+template <bool DB, bool RB, bool SHORT>
 __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const RowArgs a) {
+    constexpr int V = RB ? 8 : 4;
     __shared__ float part[kRowThreads / 64][kDots];
     const int runs = (a.k + kDots - 1) / kDots;
     const int t = blockIdx.x / runs, j0 = (blockIdx.x - t * runs) * kDots;
@@ -275,21 +377,26 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Row
         w[i] = j0 + i < a.k ? a.weights[(size_t)t * a.k + j0 + i] : 0.0f;
     }
     for (int c = tid; c < a.pieces; c += kRowThreads) {
-        float dy[V], v[kDots][V];
-        load_row<V, DB>(a.x, (size_t)t * a.H + (size_t)c * V, dy);
+        const int n = min(a.H, V), at = piece_at<V, SHORT>(a.H, c), seen = c * V - at;
+        Piece<V, DB, SHORT> dy;
+        Piece<V, RB, SHORT> v[kDots];
+        dy.load(a.x, (size_t)t * a.H + at, n);
 #pragma unroll
         for (int i = 0; i < kDots; ++i)
-            if (p[i] >= 0) load_row<V, RB>(a.rows, (size_t)p[i] * a.H + (size_t)c * V, v[i]);
+            v[i].load(a.rows, (size_t)max(p[i], 0) * a.H + at, n);
 #pragma unroll
         for (int i = 0; i < kDots; ++i) {
             if (p[i] < 0) continue;
             float d[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                dot[i] = __builtin_fmaf(dy[e], v[i][e], dot[i]);
-                d[e] = w[i] * dy[e];
+                const float sum = __builtin_fmaf(dy.get(e), v[i].get(e), dot[i]);
+                dot[i] = e >= seen ? sum : dot[i];
+                d[e] = w[i] * dy.get(e);
             }
-            store_row<V, RB>(a.y, (size_t)p[i] * a.H + (size_t)c * V, d);
+            Piece<V, RB, SHORT> o;
+            o.set(d);
+            o.store(a.y, (size_t)p[i] * a.H + at, n, a.past);
         }
     }
 #pragma unroll
@@ -306,55 +413,77 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Row
     }
 }
 
-// Whether 16-byte pieces fit every row: aligned bases, eight elements or whole
-// 16 bytes at a time.
-static bool rows_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
-template <class K>
-static int launch_rows(K kernel, const RowArgs &a, long long blocks, hipStream_t st) {
+// Threads and blocks of a row kernel: rows of up to 32 pieces share a
+// 256-thread block, longer ones take a block each, or several of up to 512
+// threads.
+typedef void (*RowKernel)(const RowArgs);
+static int launch_rows(RowKernel wide, RowKernel narrow, RowArgs &a, hipStream_t st) {
+    long long blocks;
+    int threads;
+    if (a.pieces <= 32) {
+        a.lanes = 1;
+        while (a.lanes < a.pieces) a.lanes *= 2;
+        a.per = kRowThreads / a.lanes;
+        a.chunks = 1;
+        threads = kRowThreads;
+        blocks = ((long long)a.T + a.per - 1) / a.per;
+    } else {
+        a.per = 1;
+        a.chunks = (a.pieces + 511) / 512;
+        a.lanes = threads = ((a.pieces + a.chunks - 1) / a.chunks + 63) / 64 * 64;
+        blocks = (long long)a.T * a.chunks;
+    }
     if (blocks >= (1ll << 31)) return -2;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kRowThreads), 0, st, a);
+    hipLaunchKernelGGL(a.pieces <= 32 ? narrow : wide, dim3((unsigned)blocks), dim3(threads), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-int launch_dispatch(RowArgs &a, int elem_bytes, hipStream_t st) {
-    const long long bytes = (long long)a.H * elem_bytes;
-    const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.rows | (uintptr_t)bytes;
-    const int V = at % 16 == 0 ? 16 : at % 8 == 0 ? 8 : at % 4 == 0 ? 4 : 2;
-    a.pieces = (int)(bytes / V);
-    const long long blocks = (long long)a.T * ((a.pieces + kRowThreads - 1) / kRowThreads);
-    switch (V) {
-    case 16: return launch_rows(dispatch_kernel<16>, a, blocks, st);
-    case 8: return launch_rows(dispatch_kernel<8>, a, blocks, st);
-    case 4: return launch_rows(dispatch_kernel<4>, a, blocks, st);
-    default: return launch_rows(dispatch_kernel<2>, a, blocks, st);
-    }
+// Every row is read once, so the loads are marked as not to be kept. The
+// stores are where they write more than 64 MiB, a quarter of the last-level
+// cache, which would push out more than the next kernel finds there (us with /
+// without: a dispatch and a combine of 32,768 rows of 10 KB 148 / 157, the
+// gradients of 8,186 such rows 66.2 / 67.9, of 8,192 rows of 8 KB 40.7 / 37.5).
+static int past_cache(long long bytes) { return bytes > (64ll << 20); }
+
+static int pieces_of(int H, bool bf16) { return bf16 ? (H + 7) / 8 : (H + 3) / 4; }
+
+int launch_dispatch(RowArgs &a, bool bf16, hipStream_t st) {
+    a.pieces = pieces_of(a.H, bf16);
+    a.past = past_cache((long long)a.T * a.k * a.H * (bf16 ? 2 : 4));
+    return bf16 ? launch_rows(dispatch_kernel<true, true>, dispatch_kernel<true, false>, a, st)
+                : launch_rows(dispatch_kernel<false, true>, dispatch_kernel<false, false>, a, st);
 }
 
-template <int V>
-static int combine_typed(const RowArgs &a, bool rb, bool yb, hipStream_t st) {
-    const long long blocks = (long long)a.T * ((a.pieces + kRowThreads - 1) / kRowThreads);
-    if (rb) return yb ? launch_rows(combine_kernel<V, true, true>, a, blocks, st) : launch_rows(combine_kernel<V, true, false>, a, blocks, st);
-    return yb ? launch_rows(combine_kernel<V, false, true>, a, blocks, st) : launch_rows(combine_kernel<V, false, false>, a, blocks, st);
+template <bool RB, bool YB>
+static int combine_typed(RowArgs &a, hipStream_t st) {
+    const RowKernel narrow = combine_kernel<RB, YB, false, 2>;
+    if (a.k == 1) return launch_rows(combine_kernel<RB, YB, true, 1>, narrow, a, st);
+    if (a.k == 2) return launch_rows(combine_kernel<RB, YB, true, 2>, narrow, a, st);
+    if (a.k <= 4) return launch_rows(combine_kernel<RB, YB, true, 4>, narrow, a, st);
+    return launch_rows(combine_kernel<RB, YB, true, 8>, narrow, a, st);
 }
 
 int launch_combine(RowArgs &a, bool rows_bf16, bool y_bf16, hipStream_t st) {
-    const bool wide = a.H % 8 == 0 && rows_aligned(a.rows) && rows_aligned(a.y);
-    a.pieces = wide ? a.H / 8 : a.H;
-    return wide ? combine_typed<8>(a, rows_bf16, y_bf16, st) : combine_typed<1>(a, rows_bf16, y_bf16, st);
+    a.pieces = pieces_of(a.H, rows_bf16);
+    a.past = past_cache((long long)a.T * a.H * (y_bf16 ? 2 : 4));
+    if (rows_bf16) return y_bf16 ? combine_typed<true, true>(a, st) : combine_typed<true, false>(a, st);
+    return y_bf16 ? combine_typed<false, true>(a, st) : combine_typed<false, false>(a, st);
 }
 
-template <int V>
-static int backward_typed(const RowArgs &a, bool db, bool rb, hipStream_t st) {
-    const long long blocks = (long long)a.T * ((a.k + kDots - 1) / kDots);
-    if (db) return rb ? launch_rows(combine_backward_kernel<V, true, true>, a, blocks, st) : launch_rows(combine_backward_kernel<V, true, false>, a, blocks, st);
-    return rb ? launch_rows(combine_backward_kernel<V, false, true>, a, blocks, st) : launch_rows(combine_backward_kernel<V, false, false>, a, blocks, st);
+template <bool SHORT>
+static RowKernel backward_of(bool dy_bf16, bool rows_bf16) {
+    if (dy_bf16) return rows_bf16 ? combine_backward_kernel<true, true, SHORT> : combine_backward_kernel<true, false, SHORT>;
+    return rows_bf16 ? combine_backward_kernel<false, true, SHORT> : combine_backward_kernel<false, false, SHORT>;
 }
 
 int launch_combine_backward(RowArgs &a, bool dy_bf16, bool rows_bf16, hipStream_t st) {
-    const bool wide = a.H % 8 == 0 && rows_aligned(a.x) && rows_aligned(a.rows) && rows_aligned(a.y);
-    a.pieces = wide ? a.H / 8 : a.H;
-    return wide ? backward_typed<8>(a, dy_bf16, rows_bf16, st) : backward_typed<1>(a, dy_bf16, rows_bf16, st);
+    a.pieces = pieces_of(a.H, rows_bf16);
+    a.past = past_cache((long long)a.T * a.k * a.H * (rows_bf16 ? 2 : 4));
+    const long long blocks = (long long)a.T * ((a.k + kDots - 1) / kDots);
+    if (blocks >= (1ll << 31)) return -2;
+    const RowKernel k = a.pieces == 1 ? backward_of<true>(dy_bf16, rows_bf16) : backward_of<false>(dy_bf16, rows_bf16);
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kRowThreads), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 }  // namespace kxw4

@@ -40,8 +40,8 @@ def test_route_refuses_bad_plans():
 
 def test_route_workspace_sizes():
     size = _lib.lib().kxw4_route_workspace
-    assert size(8, 2, 4) == 0 and size(16384, 1, 4) == 0 and size(0, 1, 4) == 0
-    assert size(16385, 1, 4) == (16385 + 2047) // 2048 * 5 * 4
+    assert size(8, 2, 4) == 0 and size(8192, 1, 4) == 0 and size(0, 1, 4) == 0
+    assert size(8193, 1, 4) == (8193 + 2047) // 2048 * 5 * 4
     assert size(1 << 20, 8, 128) == 256 * 129 * 4
     assert size(8, 2, 0) == 0 and size(-1, 2, 4) == 0 and size(1 << 30, 2, 4) == 0
 
