@@ -606,6 +606,7 @@ int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count,
     x.N = route->T * route->k;
     x.groups = route->groups;
     x.k = route->k;
+    x.rows = (int)rows;
     x.K = ws[0]->K;
     x.group = ws[0]->group;
     x.block = a->block;

@@ -18,10 +18,19 @@ inline long long tiles_at_most(long long N, int groups, int TT) {
     return N / TT + (N < groups ? N : groups);
 }
 
+// What to count of a group's rows: all its tiles, those that are full, or the
+// one that is not.
+enum { kTilesAll = 0, kTilesFull = 1, kTilesPart = 2 };
+template <int WHICH>
+__device__ __forceinline__ int tiles_of(int rows, int TT) {
+    return WHICH == kTilesAll ? (rows + TT - 1) / TT : WHICH == kTilesFull ? rows / TT : (rows % TT != 0);
+}
+
 struct GroupTiles {
     int first, end, tiles_before, total;                     // this lane's run of groups, the tiles before it, all tiles
 };
 
+template <int WHICH = kTilesAll>
 __device__ __forceinline__ GroupTiles scan_tiles(const int *offsets, int groups, int TT, int lane) {
     const int run = (groups + 63) / 64;
     GroupTiles s;
@@ -31,7 +40,7 @@ __device__ __forceinline__ GroupTiles scan_tiles(const int *offsets, int groups,
     int lo = offsets[s.first];
     for (int e = s.first; e < s.end; ++e) {
         const int hi = offsets[e + 1];
-        sum += (hi - lo + TT - 1) / TT;
+        sum += tiles_of<WHICH>(hi - lo, TT);
         lo = hi;
     }
     int inc = sum;
@@ -50,6 +59,7 @@ struct GroupTile {
 };
 
 // Tile u < s.total.
+template <int WHICH = kTilesAll>
 __device__ __forceinline__ GroupTile tile_at(const GroupTiles &s, const int *offsets, int TT, int u) {
     // (the last lane whose run starts at or before u has the tile, since
     // every later one starts past it: lanes without tiles share their start)
@@ -60,7 +70,7 @@ __device__ __forceinline__ GroupTile tile_at(const GroupTiles &s, const int *off
     for (;;) {
         t.begin = offsets[t.e];
         t.end = offsets[t.e + 1];
-        t.count = (t.end - t.begin + TT - 1) / TT;
+        t.count = tiles_of<WHICH>(t.end - t.begin, TT);
         if (u < t.before + t.count) break;
         t.before += t.count;
         ++t.e;

@@ -63,6 +63,9 @@ struct GemmArgs {
     int seg_end[kMaxSegments];        // exclusive token end of each segment
     int n_tiles, t_tiles;             // set by the launcher
     int raster_tt;                    // token tiles per raster group (set by the launcher)
+    // grouped rows (w[i].M: rows of one group; `rows`: activation rows)
+    const int *offsets, *order;
+    int groups, k, rows;
 };
 
 int launch_pack(const int8_t *codes, const uint16_t *scales, int M, int K, int group,
@@ -182,7 +185,7 @@ struct ExpertArgs {
     const int8_t *q;
     const float *ascale;
     const int *offsets, *order;
-    int N, groups, k, K, group, block, scale_enc, y_bf16;
+    int N, groups, k, rows, K, group, block, scale_enc, y_bf16;     // rows: of the activations
 };
 int launch_experts(const ExpertArgs &a, hipStream_t st);
 

@@ -1,8 +1,9 @@
 // kxw4_route.hpp — which kernel a decode launch (at most 16 tokens) runs on:
 // the strip kernel (kxw4_strip.hip), the row-wave kernel (kxw4_rowwave.hip)
-// or the K-parallel kernel (kxw4_decode.hip); and, last, which packed prompts
-// run on the general GEMM kernel (kxw4_gemm.hip). Plain C++, so that the rules
-// can be checked without a GPU.
+// or the K-parallel kernel (kxw4_decode.hip); which packed prompts run on the
+// general GEMM kernel (kxw4_gemm.hip); and, last, the tiles of the experts'
+// projections (kxw4_experts.hip). Plain C++, so that the rules can be checked
+// without a GPU.
 //
 // Every kernel gives the same bits; the lines lie where the times cross. They
 // were measured over 256-73,728 rows (W8: 262,144) of 1,024-17,408 columns
@@ -196,6 +197,71 @@ inline bool packed_general(const PackedShape &s) {
                           k * ((1.0 * s.few + 1.5 * s.lots + 1.0 * s.strips) / 1000 + (s.strips ? 1.0 : 0.0) +
                                2.5 * s.tile_runs + (g64 ? 3.0 : 2.0) * s.tile_work / 1e5);
     return others > general;
+}
+
+// The experts' projections: strips of 16 weight rows x `tokens` places, or (per
+// token) tiles of the large-tile kernel.
+enum ExpertRoute {
+    kExpertStrip2 = 2, kExpertStrip8 = 8, kExpertStrip16 = 16, kExpertStrip32 = 32,
+    kExpertTile32 = 132,              // 32 places x 128 rows
+    kExpertTile64 = 164,              // 64 x 256
+    kExpertTile128 = 228              // 128 x 256, group 128
+};
+
+struct ExpertShape {
+    int cus;
+    long long N;                      // places, at most
+    int groups, group;
+    int rows128, rows256;             // 128- and 256-row tiles of one expert, over all weights
+    bool blocks;                      // activation scales per K32 block, else per token
+    bool w8;
+};
+
+// The rows of each expert are known on the device only, so the rule goes by
+// their number spread evenly over the experts. Swept over 120 shapes of 8-128
+// experts, 0.2-1,663 rows each, 256-2,048 weight rows, 512-5,120 columns
+// (launches of a graph replay, weights from HBM): 3 % (group 128) and 5 % (64)
+// behind the best of seven kernels on average.
+inline int expert_route(const ExpertShape &s) {
+    const long long experts = s.N < s.groups ? s.N : s.groups, each = (s.N + experts - 1) / experts;
+    auto tiles = [&](int places, int rows) { return experts * ((each + places - 1) / places) * rows; };
+    // Few rows: short strips, whose chains run on the real places alone where
+    // most experts have none (us for strips of 2 / 8: 8 rows over 64 experts,
+    // 2 x 1,024 rows, K = 5120 11.8 / 12.4; 6 over 128, K32 blocks, 2 x 1,216,
+    // K = 1408 8.0 / 9.2; 64 over 64 35.1 / 32.4).
+    if (2 * s.N <= s.groups) return kExpertStrip2;
+    // Tiles of the large-tile kernel share a weight's unpack between their
+    // token blocks, from twelve rows an expert on once they give every CU one:
+    // 32 places (strips of 16 / tiles: 64 experts of 31 rows, 2 x 1,152, K =
+    // 2048 57 / 44; 8 of 20, 2 x 320, K = 2560, 48 tiles: 8.7 / 12.5), 64 from
+    // 30 rows on (64 of 55, 2 x 1,024 111 / 90) unless their wider row tiles
+    // hang over by more than a quarter (16 of 134, 2 x 320 13.4 / 18.5), 128
+    // while three for each CU are left (64 of 256, 2 x 1,024, K = 5120 258 /
+    // 227; 16 of 370, 2 x 1,216 45 / 51). Full tiles come first and an expert's
+    // last one takes only the 32-token blocks it needs.
+    if (!s.blocks && !s.w8 && each >= 12 && tiles(32, s.rows128) >= s.cus) {
+        const bool fits = 2 * 4 * s.rows256 <= 5 * s.rows128;
+        if (each < 30 || !fits || tiles(64, s.rows256) < s.cus) return kExpertTile32;
+        return s.group == 128 && each >= 128 && tiles(128, s.rows256) >= 3 * s.cus ? kExpertTile128 : kExpertTile64;
+    }
+    // Strips: 8 places below four rows each (16 experts of 4, K32 blocks, 2 x
+    // 1,472 10.0 / 8.9 on 16; 64 of 2 per token, 2 x 1,024 46.7 / 50.4), 16
+    // places below 28 (32 of 24, K32 blocks, 2 x 512 14.6 / 15.1 on 32; of 33, 2
+    // x 832 21.8 / 21.2), W8, with no unpack to share, below 16 (64 of 13 9.8 /
+    // 11.4; 128 of 17, 2 x 768 99 / 93).
+    if (each < 4) return kExpertStrip8;
+    if (!s.blocks && !s.w8) return kExpertStrip16;
+    return each < (s.w8 ? 16 : 28) ? kExpertStrip16 : kExpertStrip32;
+}
+
+// Splits of K for the strips of the experts' projections (up to 8, of at least
+// a 128-column tile each): until there are 2,048 strips, eight a CU (one row
+// each of 8 experts, 2 x 1,024 rows, K = 5120, 1,024 strips: one split 14.6 us,
+// two 11.8, four 11.6, eight 13.0).
+inline int expert_splits(long long strips, int ktiles) {
+    int S = 1;
+    while (S < 8 && strips * S < 2048 && 2 * S <= ktiles) S *= 2;
+    return S;
 }
 
 }  // namespace kxw4

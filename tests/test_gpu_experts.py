@@ -136,6 +136,31 @@ def test_a_row_has_the_bits_of_its_experts_own_projection(mode, T, groups, K, M)
     assert any(same)
 
 
+@pytest.mark.parametrize("mode", ["token128", "token64"])
+@pytest.mark.parametrize("T,groups,K,Ms", [
+    (700, 40, 384, [144, 272]),                              # tiles of 32 places x 128 rows
+    (2100, 8, 256, [512, 496]),                              # 64 x 256
+    (4150, 16, 128, [1040, 1040]),                           # group 128: 128 x 256
+])
+def test_large_tiles(mode, T, groups, K, Ms):
+    # uneven experts: some with no rows, one row, and most of them; the bits of
+    # each expert's own projection in one split
+    rng = np.random.default_rng(T)
+    ids = make_ids(rng, T, 2, groups, 0.05)
+    ids[ids == 1] = 0
+    ids[ids == 2] = 0
+    ids[T // 2, 1] = 2
+    ws, a, r, ys, offsets, source = run(rng, mode, T, 2, groups, K, Ms, torch.float32, False, ids)
+    for (w, _), y in zip(ws, ys):
+        for e in range(groups):
+            p = np.arange(offsets[e], offsets[e + 1])
+            if not len(p):
+                continue
+            own = ops.gemm(slice_of(w, e, groups), rows_of(a, torch.from_numpy(source[p]).to(DEV)), forced_splits=1)
+            assert torch.equal(own, y[offsets[e]:offsets[e + 1]]), e
+    run(rng, mode, T, 2, groups, K, Ms, torch.bfloat16, True, ids)
+
+
 @pytest.mark.parametrize("T", [9, 200, 2500])
 def test_all_rows_to_one_expert_and_to_none(T):
     rng = np.random.default_rng(T)
