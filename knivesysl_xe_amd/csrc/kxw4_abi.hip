@@ -617,7 +617,7 @@ int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count,
 
 size_t kxw4_adapter_workspace(const kxw4_adapters_t *ad, int T) {
     if (!ad || T <= 0 || ad->n <= 0 || ad->r <= 0 || ad->K <= 0) return 0;
-    return (size_t)adapter_splits(ad->n, T, ad->K) * T * ad->r * sizeof(float);
+    return adapter_scratch(ad->n, T, ad->r, ad->K);
 }
 
 int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, const kxw4_adapters_t *ad,

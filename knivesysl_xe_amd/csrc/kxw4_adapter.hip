@@ -65,30 +65,50 @@ __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
     }
 }
 
-constexpr int kLowWaves = 4, kLowTile = 16;
+// An operand's 16 rows x 64 bytes are loaded with four lanes to a row, so that
+// sixteen lanes touch four rows, then go to the lanes that supply them: lane n
+// + 16 g takes row n's piece g from lane 4 n + g. (With a lane for each row
+// sixteen touched sixteen, and the L1 looks each up: 7.7 against 2.0 million
+// lookups for 3,965 tokens, r = 32, and 24 against 20 us; 61 tokens of 24
+// adapters, r = 64, K = 17408 25.9 / 24.9, r = 128 238 / 226 in all.)
+__device__ __forceinline__ uint32_t to_operand(uint32_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_ds_bpermute((4 * (lane & 15) + (lane >> 4)) * 4, (int)v);
+}
+__device__ __forceinline__ v4u to_operand(v4u v, int lane) {
+    return v4u{to_operand(v.x, lane), to_operand(v.y, lane), to_operand(v.z, lane), to_operand(v.w, lane)};
+}
+
+constexpr int kLowTile = 16, kFewWaves = 4;
+// 32-column chunks that r comes to, and BF16 elements of one chunk's three
+// parts of a tile in the order of the MFMA's operand: [part][lane][8]
+__host__ __device__ constexpr int chunks_of(int r) { return (r + 31) / 32; }
+constexpr int kCutChunk = 3 * 64 * 8;
 
 // low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
-// work-group takes 16 places of one adapter and part s, its waves consecutive
-// runs of 32-K steps, all r columns (CT tiles of 16). Operands come straight
-// from memory: a step's x piece is used by every column tile, an A piece once.
-template <int CT, bool XB>
-__global__ __launch_bounds__(64 * kLowWaves) void adapter_low_kernel(const AdapterArgs a) {
-    __shared__ float part[kLowWaves - 1][CT][256];
+// work-group takes 16 places of one adapter and part s, its WAVES waves
+// consecutive runs of 32-K steps, all r columns (CT tiles of 16). Operands come
+// straight from memory: a step's x piece is used by every column tile, an A
+// piece once. CUT: one part; scale * low is cut into its three BF16 parts here,
+// in the order the second launch's operand takes them.
+template <int CT, int WAVES, bool XB, bool CUT>
+__global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
+    __shared__ float part[WAVES - 1][CT][256];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
     if ((int)blockIdx.x >= tiles.total) return;
     const GroupTile tile = tile_at(tiles, a.offsets, kLowTile, blockIdx.x);
     const int p0 = tile.begin + tile.index * kLowTile;
-    const int steps = a.K / 32, ways = a.splits * kLowWaves, way = blockIdx.y * kLowWaves + wave;
+    const int steps = a.K / 32, ways = a.splits * WAVES, way = blockIdx.y * WAVES + wave;
     const int k0 = (int)((long long)steps * way / ways), k1 = (int)((long long)steps * (way + 1) / ways);
 
-    const int token = a.order[min(p0 + m, tile.end - 1)];
-    const size_t xrow = (size_t)token * a.K + 8 * g;
+    const int lr = lane >> 2, lk = 8 * (lane & 3);           // row and columns that this lane loads
+    const int token = a.order[min(p0 + lr, tile.end - 1)];
+    const size_t xrow = (size_t)token * a.K + lk;
     const uint16_t *arow[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
-        arow[c] = a.a + ((size_t)tile.e * a.r + min(c * 16 + m, a.r - 1)) * a.K + 8 * g;
+        arow[c] = a.a + ((size_t)tile.e * a.r + min(c * 16 + lr, a.r - 1)) * a.K + lk;
     v4f acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -107,7 +127,10 @@ __global__ __launch_bounds__(64 * kLowWaves) void adapter_low_kernel(const Adapt
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[c] = mfma_bf16(x[u], w[u][c], acc[c]);
+                for (int c = 0; c < CT; ++c) {
+                    if (c == 0) x[u] = to_operand(x[u], lane);
+                    acc[c] = mfma_bf16(x[u], to_operand(w[u][c], lane), acc[c]);
+                }
         } else {
             float v[U][8];
 #pragma unroll
@@ -119,11 +142,15 @@ __global__ __launch_bounds__(64 * kLowWaves) void adapter_low_kernel(const Adapt
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 v4u x[3];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] = __uint_as_float(to_operand(__float_as_uint(v[u][i]), lane));
                 split8(v[u], x);
 #pragma unroll
-                for (int c = 0; c < CT; ++c)
+                for (int c = 0; c < CT; ++c) {
+                    const v4u b = to_operand(w[u][c], lane);
 #pragma unroll
-                    for (int q = 2; q >= 0; --q) acc[c] = mfma_bf16(x[q], w[u][c], acc[c]);
+                    for (int q = 2; q >= 0; --q) acc[c] = mfma_bf16(x[q], b, acc[c]);
+                }
             }
         }
     };
@@ -138,6 +165,38 @@ __global__ __launch_bounds__(64 * kLowWaves) void adapter_low_kernel(const Adapt
             for (int i = 0; i < 4; ++i) part[wave - 1][c][i * 64 + lane] = acc[c][i];
     }
     __syncthreads();
+    if constexpr (CUT) {
+        // every thread adds up and cuts elements of the tile: lane l of
+        // chunk h holds token l%16 and columns 32 h + 8 (l/16) .. + 7
+        const float scale = a.scale[tile.e];
+        if (wave == 0) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = acc[c][i];
+#pragma unroll
+                    for (int w = 0; w < WAVES - 1; ++w) v += part[w][c][i * 64 + lane];
+                    part[0][c][i * 64 + lane] = c * 16 + m < a.r ? v * scale : 0.0f;
+                }
+        }
+        __syncthreads();
+        uint16_t *to = reinterpret_cast<uint16_t *>(a.low) + (size_t)blockIdx.x * chunks_of(a.r) * kCutChunk;
+        for (int h = wave; h < chunks_of(a.r); h += WAVES) {
+            float v[8];
+            v4u op[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // column 32 h + 8 g + j of token m: tile c, register i = m % 4 of lane group m / 4
+                const int column = 32 * h + 8 * g + j;
+                v[j] = column < 16 * CT ? part[0][min(column >> 4, CT - 1)][(m & 3) * 64 + 16 * (m >> 2) + (column & 15)] : 0.0f;
+            }
+            split8(v, op);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<v4u *>(to + (h * 3 + q) * 512 + lane * 8) = op[q];
+        }
+        return;
+    }
     if (wave > 0) return;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -146,139 +205,329 @@ __global__ __launch_bounds__(64 * kLowWaves) void adapter_low_kernel(const Adapt
         for (int i = 0; i < 4; ++i) {
             float v = acc[c][i];
 #pragma unroll
-            for (int w = 0; w < kLowWaves - 1; ++w) v += part[w][c][i * 64 + lane];
+            for (int w = 0; w < WAVES - 1; ++w) v += part[w][c][i * 64 + lane];
             const int p = p0 + 4 * g + i;
             if (p < tile.end && col < a.r) a.low[((size_t)blockIdx.y * a.T + p) * a.r + col] = v;
         }
     }
 }
 
-// out = y + scale B low. A wave takes 64 rows of B x TS tiles of 16 places of
-// one adapter. B is the MFMA's first operand, its rows dealt so that lane group
-// g ends up with 16 consecutive outputs (m0 + 16 g ..) of one token: tile c's
-// row 4 g + i is m0 + 16 g + 4 c + i. Bound by reading y and writing out.
-constexpr int kUpWaves = 4, kUpRows = 64;
-template <int TS, bool YB>
+// out = y + scale B low for few tokens: a work-group takes 16 places of one
+// adapter x 256 rows of B, 64 a wave. It adds up the parts of `low`, cuts scale
+// * low into three BF16 parts in LDS, and each wave multiplies them by its
+// rows. B is the MFMA's first operand, its rows dealt so that a lane ends up
+// with 16-byte runs of one token's outputs. A chain of round trips (offsets,
+// order, y and low) bounds it: all that a step needs is requested together.
+constexpr int kUpWaves = 4, kUpRows = 64, kUpBlock = kUpWaves * kUpRows;
+// BF16 elements of a token's row of one part: r padded to whole MFMAs, with 16
+// bytes more so that neighbouring rows start in different banks
+__host__ __device__ constexpr int up_pitch(int r) { return 32 * chunks_of(r) + 8; }
+
+// KC: 32-column chunks of B requested together.
+template <int KC, bool YB>
 __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const AdapterArgs a) {
+    constexpr int NY = YB ? 2 : 4;                           // 16-byte pieces of a lane's 16 outputs
+    extern __shared__ __attribute__((aligned(16))) uint16_t cut[];       // [3][16][pitch]
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const GroupTiles tiles = scan_tiles(a.offsets, a.n, 16 * TS, lane);
-    const int m0 = (blockIdx.y * kUpWaves + wave) * kUpRows;
+    const int mblocks = (a.M + kUpBlock - 1) / kUpBlock;
+    const int u = blockIdx.x / mblocks, m0 = (blockIdx.x - u * mblocks) * kUpBlock + wave * kUpRows;
+    const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
     int p0, p1, e = -1;
-    if ((int)blockIdx.x < tiles.total) {
-        const GroupTile tile = tile_at(tiles, a.offsets, 16 * TS, blockIdx.x);
+    if (u < tiles.total) {
+        const GroupTile tile = tile_at(tiles, a.offsets, kLowTile, u);
         e = tile.e;
-        p0 = tile.begin + tile.index * 16 * TS;
+        p0 = tile.begin + tile.index * kLowTile;
         p1 = tile.end;
     } else {
         // the tokens without an adapter keep y (already there when out is y)
-        p0 = a.offsets[a.n] + ((int)blockIdx.x - tiles.total) * 16 * TS;
+        p0 = a.offsets[a.n] + (u - tiles.total) * kLowTile;
         p1 = a.T;
         if (a.out == a.y || p0 >= p1) return;
     }
-    if (m0 >= a.M) return;
-    const int mg = m0 + 16 * g;                              // this lane's 16 outputs
-    v4f acc[TS][4];
+    const bool on = m0 < a.M;                                // (the others only help with `low`)
+    const size_t at = (size_t)a.order[min(p0 + n, p1 - 1)] * a.M;
+    // column of a lane's piece q, and the row of B that MFMA c has as its row i
+    auto col = [&](int q) { return m0 + (YB ? 32 * q + 8 * g : 16 * q + 4 * g); };
+    auto row = [&](int c, int i) { return m0 + (YB ? 32 * (c >> 1) + 8 * (i >> 2) + 4 * (c & 1) + (i & 3) : 16 * c + i); };
+    v4u yv[NY];
 #pragma unroll
-    for (int s = 0; s < TS; ++s)
+    for (int q = 0; q < NY; ++q)
+        yv[q] = *reinterpret_cast<const v4u *>(static_cast<const uint8_t *>(a.y) + (at + min(col(q), a.M - (YB ? 8 : 4))) * (YB ? 2 : 4));
+    v4f acc[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[s][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < 4; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (e >= 0) {
+        const int pitch = up_pitch(a.r), quads = (pitch - 8) / 4;
         const float scale = a.scale[e];
-        for (int k = 8 * g; k - 8 * g < a.r; k += 32) {
-            const bool in = k < a.r;
-            v4u b[4];
+        const size_t part = (size_t)a.T * a.r;
+        for (int i = tid; i < kLowTile * quads; i += 64 * kUpWaves) {
+            const int t = i / quads, c = (i - t * quads) * 4;
+            v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (c < a.r) {
+                const float *low = a.low + (size_t)min(p0 + t, p1 - 1) * a.r + c;
+                for (int q = 0; q < a.splits; q += 8) {
+                    v4f o[8];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int row = min(m0 + 16 * (n >> 2) + 4 * c + (n & 3), a.M - 1);
-                b[c] = in ? *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + row) * a.r + k) : v4u{0, 0, 0, 0};
-            }
+                    for (int j = 0; j < 8; ++j) o[j] = *reinterpret_cast<const v4f *>(low + (size_t)min(q + j, a.splits - 1) * part);
 #pragma unroll
-            for (int s = 0; s < TS; ++s) {
-                float v[8] = {};
-                const int p = min(p0 + 16 * s + n, p1 - 1);
-                if (in) {
-                    load8(a.low + (size_t)p * a.r + k, v);
-                    for (int q = 1; q < a.splits; ++q) {
-                        float o[8];
-                        load8(a.low + ((size_t)q * a.T + p) * a.r + k, o);
+                    for (int j = 0; j < 8; ++j)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] += o[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] *= scale;
+                        for (int x = 0; x < 4; ++x) v[x] = q + j < a.splits ? v[x] + o[j][x] : v[x];
                 }
-                v4u x[3];
-                split8(v, x);
+            }
+            uint32_t w[4][3];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+            for (int x = 0; x < 4; ++x) split3(v[x] * scale, w[x]);
 #pragma unroll
-                    for (int q = 2; q >= 0; --q) acc[s][c] = mfma_bf16(b[c], x[q], acc[s][c]);
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<v2u *>(cut + (q * kLowTile + t) * pitch + c) = v2u{w[0][q] >> 16 | w[1][q], w[2][q] >> 16 | w[3][q]};
+        }
+        __syncthreads();
+        if (!on) return;
+        for (int k0 = 0; k0 < a.r; k0 += 32 * KC) {
+            v4u b[KC][4];
+#pragma unroll
+            for (int h = 0; h < KC; ++h)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int k = k0 + 32 * h + 8 * g;
+                    const v4u w = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(row(c, n), a.M - 1)) * a.r + min(k, a.r - 8));
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) b[h][c][x] = k < a.r ? w[x] : 0u;
+                }
+#pragma unroll
+            for (int h = 0; h < KC; ++h) {
+                if (k0 + 32 * h >= a.r) break;
+#pragma unroll
+                for (int q = 2; q >= 0; --q) {
+                    const v4u x = *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * pitch + k0 + 32 * h + 8 * g);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[c] = mfma_bf16(b[h][c], x, acc[c]);
+                }
             }
         }
     }
-    if (mg >= a.M) return;
+    if (!on || p0 + n >= p1) return;
 #pragma unroll
-    for (int s = 0; s < TS; ++s) {
-        const int p = p0 + 16 * s + n;
-        if (p >= p1) continue;
-        const size_t at = (size_t)a.order[p] * a.M + mg;
-        if constexpr (YB) {
-            const v4u *y = reinterpret_cast<const v4u *>(static_cast<const uint16_t *>(a.y) + at);
-            v4u *out = reinterpret_cast<v4u *>(static_cast<uint16_t *>(a.out) + at);
+    for (int q = 0; q < NY; ++q) {
+        if (col(q) >= a.M) continue;
+        v4u o;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const v4u u = y[h];
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (YB) {
+                const v4f f = acc[2 * q + (i >> 1)];
+                o[i] = pack_bf16(__uint_as_float(yv[q][i] << 16) + f[2 * (i & 1)],
+                                 __uint_as_float(yv[q][i] & 0xFFFF0000u) + f[2 * (i & 1) + 1]);
+            } else {
+                o[i] = __float_as_uint(__uint_as_float(yv[q][i]) + acc[q][i]);
+            }
+        }
+        *reinterpret_cast<v4u *>(static_cast<uint8_t *>(a.out) + (at + col(q)) * (YB ? 2 : 4)) = o;
+    }
+}
+
+// The same for many tokens. A wave takes 128 rows of B, whose operands stay in
+// its registers, and walks up to a.run tiles of 16 places of one adapter. `low`
+// is the MFMA's first operand (rows are tokens), in the order the first launch
+// left it, so a load of it is one contiguous kilobyte; B's rows are dealt so
+// that a lane ends up with 16-byte runs of outputs and sixteen lanes with 256
+// consecutive bytes of one token (the other way round sixteen lanes touched
+// sixteen rows, 42 lookups of the L1 an access against 16). The next tile's y
+// and low are requested before this one's products. Bound by reading y and
+// writing out: 3,965 tokens, M = 17408, BF16, r = 32 60 us for 276 MB (4.6 TB/s).
+constexpr int kManyWaves = 4, kManyRows = 128, kManyBlock = kManyWaves * kManyRows;
+template <int KC, bool YB>
+__global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const AdapterArgs a) {
+    constexpr int NQ = YB ? 1 : 2, RUN = YB ? 8 : 4;         // 16-byte pieces of a lane and token, outputs of a piece
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int mblocks = (a.M + kManyBlock - 1) / kManyBlock;
+    const int u = blockIdx.x / mblocks, m0 = (blockIdx.x - u * mblocks) * kManyBlock + wave * kManyRows;
+    // a run: a.run tiles of one adapter; `first`: its first tile's number among all
+    const GroupTiles runs = scan_tiles(a.offsets, a.n, kLowTile * a.run, lane);
+    int p0, p1, e = -1;
+    size_t first = 0;
+    if (u < runs.total) {
+        const GroupTile run = tile_at(runs, a.offsets, kLowTile * a.run, u);
+        e = run.e;
+        p0 = run.begin + run.index * kLowTile * a.run;
+        p1 = min(run.end, p0 + kLowTile * a.run);
+        const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
+        // the adapter's first tile: the lane whose run of groups holds e, and
+        // the groups before it there
+        const int per = (a.n + 63) / 64, l = e / per;
+        int before = __builtin_amdgcn_readlane(tiles.tiles_before, l);
+        for (int i = l * per; i < e; ++i) before += (a.offsets[i + 1] - a.offsets[i] + kLowTile - 1) / kLowTile;
+        first = before + run.index * a.run;
+    } else {
+        // the tokens without an adapter keep y (already there when out is y)
+        p0 = a.offsets[a.n] + (u - runs.total) * kLowTile * a.run;
+        p1 = min(a.T, p0 + kLowTile * a.run);
+        if (a.out == a.y || p0 >= p1) return;
+    }
+    if (m0 >= a.M) return;
+    // column of output j of MFMA c = (piece, run element): a lane's own, and of
+    // the row of B that it supplies
+    auto col = [&](int q) { return m0 + 16 * RUN * q + RUN * n; };
+    v4u b[KC][8];
+    if (e >= 0) {
+#pragma unroll
+        for (int h = 0; h < KC; ++h)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const int k = 32 * h + 8 * g, row = min(col(c / RUN) + c % RUN, a.M - 1);
+                const v4u w = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + row) * a.r + min(k, a.r - 8));
+#pragma unroll
+                for (int x = 0; x < 4; ++x) b[h][c][x] = k < a.r ? w[x] : 0u;
+            }
+    }
+    auto tokens = [&](int p, size_t (&at)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = (size_t)a.order[min(p + 4 * g + i, p1 - 1)] * a.M;
+    };
+    auto load_y = [&](const size_t (&at)[4], v4u (&yv)[4][NQ]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+                yv[i][q] = *reinterpret_cast<const v4u *>(static_cast<const uint8_t *>(a.y) + (at[i] + min(col(q), a.M - RUN)) * (YB ? 2 : 4));
+    };
+    const uint16_t *cut = reinterpret_cast<const uint16_t *>(a.low) + first * chunks_of(a.r) * kCutChunk + lane * 8;
+    auto load_low = [&](int tile, v4u (&x)[KC][3]) {
+#pragma unroll
+        for (int h = 0; h < KC; ++h)
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                x[h][q] = *reinterpret_cast<const v4u *>(cut + ((size_t)tile * chunks_of(a.r) + min(h, chunks_of(a.r) - 1)) * kCutChunk + q * 512);
+    };
+    const int tiles = (p1 - p0 + kLowTile - 1) / kLowTile;
+    size_t at[4], atnext[4];
+    v4u yv[4][NQ], ynext[4][NQ], x[KC][3], xnext[KC][3];
+    tokens(p0, atnext);
+    load_y(atnext, ynext);
+    if (e >= 0) load_low(0, xnext);
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int p = p0 + kLowTile * tile;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at[i] = atnext[i];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) yv[i][q] = ynext[i][q];
+        }
+        v4f acc[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        const bool more = tile + 1 < tiles;
+        if (e >= 0) {
+#pragma unroll
+            for (int h = 0; h < KC; ++h)
+#pragma unroll
+                for (int q = 0; q < 3; ++q) x[h][q] = xnext[h][q];
+        }
+        if (more) {
+            tokens(p + kLowTile, atnext);
+            if (e >= 0) load_low(tile + 1, xnext);
+            load_y(atnext, ynext);
+        }
+        if (e >= 0) {
+#pragma unroll
+            for (int h = 0; h < KC; ++h)
+#pragma unroll
+                for (int q = 2; q >= 0; --q)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) acc[c] = mfma_bf16(x[h][q], b[h][c], acc[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (p + 4 * g + i >= p1) continue;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                if (col(q) >= a.M) continue;
                 v4u o;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = 2 * h + (i >> 1), r = 2 * (i & 1);
-                    o[i] = round_bf16(__uint_as_float(u[i] << 16) + acc[s][c][r]) |
-                           round_bf16(__uint_as_float(u[i] & 0xFFFF0000u) + acc[s][c][r + 1]) << 16;
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (YB)
+                        o[j] = pack_bf16(__uint_as_float(yv[i][q][j] << 16) + acc[2 * j][i],
+                                         __uint_as_float(yv[i][q][j] & 0xFFFF0000u) + acc[2 * j + 1][i]);
+                    else
+                        o[j] = __float_as_uint(__uint_as_float(yv[i][q][j]) + acc[4 * q + j][i]);
                 }
-                out[h] = o;
+                *reinterpret_cast<v4u *>(static_cast<uint8_t *>(a.out) + (at[i] + col(q)) * (YB ? 2 : 4)) = o;
             }
-        } else {
-            const v4f *y = reinterpret_cast<const v4f *>(static_cast<const float *>(a.y) + at);
-            v4f *out = reinterpret_cast<v4f *>(static_cast<float *>(a.out) + at);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) out[c] = y[c] + acc[s][c];
         }
     }
 }
 
-// Work-groups per 16-token tile of the first launch: enough to give each CU
-// one while a wave keeps at least four 32-K steps.
-int adapter_splits(int n, int T, int K) {
+// Many tokens, from about 1,500 and 64 an adapter on, while B's rows fit the
+// registers (us few / many: 3,965 tokens of 6 adapters, K = 5120, M = 17408, r =
+// 32 105 / 77, r = 128 226 / 152; 2,048 of 64, M = 5120, r = 16 27 / 29; 1,000 of
+// 4, M = 17408, float32 45.5 / 46.4; 500 of 8, r = 32 13.4 / 21.5).
+static bool many_tokens(int n, int T, int r) { return T >= 1536 && T >= 64ll * n && r <= 128; }
+
+// Work-groups per 16-token tile of the first launch for few tokens: enough to
+// give each CU four while a wave keeps at least four 32-K steps, and as many
+// as the second launch adds up in one round (us for 4 / 8 / 16: 8 tokens of 8,
+// K = 5120 8.3 / 7.7 / 8.2; 61 of 24, K = 17408, r = 64 30.0 / 21.7 / 22.3).
+static int adapter_splits(int n, int T, int K) {
     const long long tiles = std::max(1ll, tiles_at_most(T, n, kLowTile));
-    const long long most = std::max(1, K / (32 * kLowWaves * 4));
-    return (int)std::max(1ll, std::min({most, 256 / tiles, 32ll}));
+    const long long most = std::max(1, K / (32 * kFewWaves * 4));
+    return (int)std::max(1ll, std::min({most, 1024 / tiles, 8ll}));
 }
 
-template <int CT>
-static void launch_low(const AdapterArgs &a, bool x_bf16, dim3 grid, hipStream_t st) {
-    if (x_bf16) hipLaunchKernelGGL((adapter_low_kernel<CT, true>), grid, dim3(64 * kLowWaves), 0, st, a);
-    else hipLaunchKernelGGL((adapter_low_kernel<CT, false>), grid, dim3(64 * kLowWaves), 0, st, a);
+size_t adapter_scratch(int n, int T, int r, int K) {
+    if (many_tokens(n, T, r)) return (size_t)tiles_at_most(T, n, kLowTile) * chunks_of(r) * kCutChunk * 2;
+    return (size_t)adapter_splits(n, T, K) * T * r * sizeof(float);
 }
 
-template <int TS>
-static void launch_up(const AdapterArgs &a, bool y_bf16, hipStream_t st) {
-    const dim3 grid((unsigned)(tiles_at_most(a.T, a.n, 16 * TS) + 1), (a.M + kUpWaves * kUpRows - 1) / (kUpWaves * kUpRows));
-    if (y_bf16) hipLaunchKernelGGL((adapter_up_kernel<TS, true>), grid, dim3(64 * kUpWaves), 0, st, a);
-    else hipLaunchKernelGGL((adapter_up_kernel<TS, false>), grid, dim3(64 * kUpWaves), 0, st, a);
+template <int CT, int WAVES, bool CUT>
+static void launch_low(const AdapterArgs &a, bool x_bf16, hipStream_t st) {
+    const dim3 grid((unsigned)tiles_at_most(a.T, a.n, kLowTile), a.splits);
+    if (x_bf16) hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, true, CUT>), grid, dim3(64 * WAVES), 0, st, a);
+    else hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, false, CUT>), grid, dim3(64 * WAVES), 0, st, a);
+}
+
+template <int KC>
+static int launch_up(const AdapterArgs &a, bool y_bf16, hipStream_t st) {
+    const long long grid = (tiles_at_most(a.T, a.n, kLowTile) + 1) * ((a.M + kUpBlock - 1) / kUpBlock);
+    if (grid >= (1ll << 31)) return -2;
+    const size_t lds = (size_t)3 * kLowTile * up_pitch(a.r) * 2;          // (at most 25.3 KB: r = 256)
+    if (y_bf16) hipLaunchKernelGGL((adapter_up_kernel<KC, true>), dim3((unsigned)grid), dim3(64 * kUpWaves), lds, st, a);
+    else hipLaunchKernelGGL((adapter_up_kernel<KC, false>), dim3((unsigned)grid), dim3(64 * kUpWaves), lds, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -6;
+}
+
+// Tiles per run: up to twelve, so that B is read seldom, while six (three,
+// where its rows take most of the registers) work-groups a CU are left (r =
+// 32: runs of 4 / 6 / 12 78.5 / 77.9 / 82.1 us; r = 128 169 / 153 / 144).
+template <int KC>
+static int launch_many(AdapterArgs &a, bool y_bf16, hipStream_t st) {
+    const int mblocks = (a.M + kManyBlock - 1) / kManyBlock;
+    const long long work = tiles_at_most(a.T, a.n, kLowTile) * mblocks, groups = (KC <= 2 ? 6ll : 3ll) * device_cus();
+    a.run = (int)std::max(1ll, std::min(12ll, (work + groups / 2) / groups));
+    const long long grid = (tiles_at_most(a.T, a.n, kLowTile * a.run) + 1) * mblocks;
+    if (grid >= (1ll << 31)) return -2;
+    if (y_bf16) hipLaunchKernelGGL((adapter_many_kernel<KC, true>), dim3((unsigned)grid), dim3(64 * kManyWaves), 0, st, a);
+    else hipLaunchKernelGGL((adapter_many_kernel<KC, false>), dim3((unsigned)grid), dim3(64 * kManyWaves), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
+    if (many_tokens(a.n, a.T, a.r)) {
+        a.splits = 1;
+        if (a.r <= 16) launch_low<1, 16, true>(a, x_bf16, st);
+        else if (a.r <= 32) launch_low<2, 16, true>(a, x_bf16, st);
+        else if (a.r <= 64) launch_low<4, 8, true>(a, x_bf16, st);
+        else launch_low<8, 8, true>(a, x_bf16, st);
+        return a.r <= 32 ? launch_many<1>(a, y_bf16, st) : a.r <= 64 ? launch_many<2>(a, y_bf16, st) : launch_many<4>(a, y_bf16, st);
+    }
     a.splits = adapter_splits(a.n, a.T, a.K);
-    const dim3 grid((unsigned)tiles_at_most(a.T, a.n, kLowTile), a.splits);
-    if (a.r <= 16) launch_low<1>(a, x_bf16, grid, st);
-    else if (a.r <= 32) launch_low<2>(a, x_bf16, grid, st);
-    else if (a.r <= 64) launch_low<4>(a, x_bf16, grid, st);
-    else if (a.r <= 128) launch_low<8>(a, x_bf16, grid, st);
-    else launch_low<16>(a, x_bf16, grid, st);
-    if (a.T > 16 * a.n) launch_up<4>(a, y_bf16, st);
-    else launch_up<1>(a, y_bf16, st);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
+    if (a.r <= 16) launch_low<1, kFewWaves, false>(a, x_bf16, st);
+    else if (a.r <= 32) launch_low<2, kFewWaves, false>(a, x_bf16, st);
+    else if (a.r <= 64) launch_low<4, kFewWaves, false>(a, x_bf16, st);
+    else if (a.r <= 128) launch_low<8, kFewWaves, false>(a, x_bf16, st);
+    else launch_low<16, kFewWaves, false>(a, x_bf16, st);
+    return a.r <= 32 ? launch_up<1>(a, y_bf16, st) : launch_up<2>(a, y_bf16, st);
 }
 
 }  // namespace kxw4

@@ -84,11 +84,14 @@ __device__ __forceinline__ uint16_t float_to_bf16(float x) {
     return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
 }
 
-// The same in the low half of a word, for any value: a NaN stays a NaN (above,
-// one of low mantissa bits only is carried over to infinity or zero).
-__device__ __forceinline__ uint32_t round_bf16(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return x == x ? (b + 0x7fffu + ((b >> 16) & 1u)) >> 16 : (b >> 16) | 0x40u;
+// Two values as BF16 in one word, lo in its low half, by the hardware's
+// conversion (v_cvt_pk_bf16_f32: round to nearest even, a NaN stays a NaN; the
+// integer form above carries one of low mantissa bits over to infinity).
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const v2f v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2bf));
 }
 
 __device__ __forceinline__ float bf16_to_float(uint16_t b) {

@@ -221,12 +221,12 @@ struct AdapterArgs {
     void *out;
     const uint16_t *a, *b;
     const float *scale;
-    float *low;                       // scratch [splits][T][r]
+    float *low;                       // scratch
     const int *offsets, *order;
     int T, n, r, K, M;
-    int splits;                       // (set by the launcher)
+    int splits, run;                  // (set by the launcher)
 };
-int adapter_splits(int n, int T, int K);
+size_t adapter_scratch(int n, int T, int r, int K);       // bytes of `low`
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st);
 
 // Returns 1 (nothing launched) outside the per-token, one-split-per-token mode.

@@ -275,7 +275,7 @@ struct Piece {
     __device__ __forceinline__ void set(const float (&v)[V]) {       // one rounding each
 #pragma unroll
         for (int i = 0; i < WORDS; ++i) {
-            if constexpr (BF) w[i] = round_bf16(v[2 * i]) | round_bf16(v[2 * i + 1]) << 16;
+            if constexpr (BF) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
             else w[i] = __float_as_uint(v[i]);
         }
     }

@@ -65,7 +65,10 @@ def check(got, y, x, ad, ids):
 @pytest.mark.parametrize("T,n,r,K,M", [
     (1, 1, 8, 128, 16), (1, 5, 16, 1024, 64), (8, 8, 16, 5120, 5120), (13, 3, 24, 384, 80), (16, 1, 32, 256, 256),
     (17, 1, 32, 256, 272), (61, 24, 64, 2048, 512), (64, 64, 16, 640, 112), (65, 2, 8, 128, 1040), (100, 3, 128, 512, 144),
-    (129, 200, 40, 256, 48), (300, 4, 256, 384, 96), (1000, 6, 16, 256, 1008), (70, 1024, 8, 128, 32), (5, 2, 200, 17408, 64)])
+    (129, 200, 40, 256, 48), (300, 4, 256, 384, 96), (1000, 6, 16, 256, 1008), (70, 1024, 8, 128, 32), (5, 2, 200, 17408, 64),
+    # many tokens: B's rows in registers, r <= 128, and not
+    (1536, 24, 16, 128, 1040), (1537, 1, 8, 256, 16), (2100, 6, 40, 256, 528), (1601, 3, 128, 384, 80), (3000, 2, 72, 128, 144),
+    (1600, 3, 136, 128, 48), (1600, 30, 32, 128, 48)])
 @pytest.mark.parametrize("x_t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("y_t", [torch.float32, torch.bfloat16])
 def test_against_float64(T, n, r, K, M, x_t, y_t):
