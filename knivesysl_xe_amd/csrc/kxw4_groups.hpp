@@ -5,8 +5,8 @@
 // into tiles of TT places that never reach over two groups. The counts are
 // known on the device only, so the host launches enough work-groups for any
 // counts (tiles_at_most) and each finds its tile from the offsets: every lane
-// adds up the tiles of a run of groups, a scan over the lanes places them.
-// That is one memory round trip and about 300 cycles at up to 64 groups.
+// adds up the tiles of a run of groups, a scan over the lanes (on DPP moves, no
+// LDS) places them. At up to 64 groups that is one memory round trip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -28,7 +28,27 @@ __device__ __forceinline__ int tiles_of(int rows, int TT) {
 
 struct GroupTiles {
     int first, end, tiles_before, total;                     // this lane's run of groups, the tiles before it, all tiles
+    int begin, begin_end;                                    // the places of its first group
 };
+
+// v plus the lane of the DPP control's, 0 where there is none (row_mask: rows
+// of 16 lanes that take part).
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xF, false);
+}
+
+// Inclusive sum over the wave's lanes: row_shr 1, 2, 4, 8 within rows of 16,
+// then row_bcast:15 (a row's last lane to the next row) into rows 1 and 3 and
+// row_bcast:31 into rows 2 and 3.
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
 
 template <int WHICH = kTilesAll>
 __device__ __forceinline__ GroupTiles scan_tiles(const int *offsets, int groups, int TT, int lane) {
@@ -38,17 +58,15 @@ __device__ __forceinline__ GroupTiles scan_tiles(const int *offsets, int groups,
     s.end = min(s.first + run, groups);
     int sum = 0;
     int lo = offsets[s.first];
+    s.begin = lo;
+    s.begin_end = lo;
     for (int e = s.first; e < s.end; ++e) {
         const int hi = offsets[e + 1];
+        if (e == s.first) s.begin_end = hi;
         sum += tiles_of<WHICH>(hi - lo, TT);
         lo = hi;
     }
-    int inc = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += v;
-    }
+    const int inc = wave_scan(sum);
     s.tiles_before = inc - sum;
     s.total = __builtin_amdgcn_readlane(inc, 63);
     return s;
@@ -67,13 +85,15 @@ __device__ __forceinline__ GroupTile tile_at(const GroupTiles &s, const int *off
     GroupTile t;
     t.e = __builtin_amdgcn_readlane(s.first, l);
     t.before = __builtin_amdgcn_readlane(s.tiles_before, l);
+    t.begin = __builtin_amdgcn_readlane(s.begin, l);
+    t.end = __builtin_amdgcn_readlane(s.begin_end, l);
     for (;;) {
-        t.begin = offsets[t.e];
-        t.end = offsets[t.e + 1];
         t.count = tiles_of<WHICH>(t.end - t.begin, TT);
         if (u < t.before + t.count) break;
         t.before += t.count;
         ++t.e;
+        t.begin = t.end;
+        t.end = offsets[t.e + 1];
     }
     t.index = u - t.before;
     return t;

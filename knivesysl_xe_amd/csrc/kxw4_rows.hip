@@ -13,6 +13,7 @@
 // FP32 in a fixed order (choices in turn; the dot products over 256-thread
 // strides, then lanes, then waves) and is rounded once, to the output's type.
 #include "kxw4_device.hpp"
+#include "kxw4_groups.hpp"
 #include "kxw4_internal.hpp"
 
 #include <algorithm>
@@ -133,11 +134,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const RouteArgs a) {
         const int run = (G1 + 63) / 64, g0 = min(lane * run, G1), g1 = min(g0 + run, G1);
         int sum = 0;
         for (int g = g0; g < g1; ++g) sum += tot[g];
-        int inc = sum;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(inc, o, 64);
-            if (lane >= o) inc += v;
-        }
+        const int inc = wave_scan(sum);
         int at = inc - sum;
         for (int g = g0; g < g1; ++g) {
             const int c = tot[g];
@@ -197,8 +194,8 @@ int launch_route(RouteArgs &a, hipStream_t st) {
     const size_t lds = (size_t)(waves + 1) * G1 * sizeof(int);            // (at most 69.7 KB: 1,024 groups)
     static bool attr[64] = {};                               // (the attribute is per device)
     int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return -6;
-    if (!attr[dev]) {
+    if (lds > 64 * 1024 && (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64)) return -6;
+    if (lds > 64 * 1024 && !attr[dev]) {
         for (const void *k : {reinterpret_cast<const void *>(plan_hist_kernel), reinterpret_cast<const void *>(plan_kernel<1>),
                               reinterpret_cast<const void *>(plan_kernel<kPlanAhead>)})
             if (hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024) != hipSuccess) return -6;

@@ -277,13 +277,22 @@ __global__ __launch_bounds__(512) void strip_kernel(const StripArgs a) {
     // rows of 1,024-17,408 columns.)
     const int row = rg * 16 + n;
     float tsc[NT][4], rsd[NT][4];
+    // (grouped: the tokens' rows come from the plan now, not behind the first
+    // stage's loads, which a wait for them would wait for too)
+    uint32_t trow[NT][4];
+    if constexpr (GRP && !BLK) {
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) trow[b][r] = row_of(min(t0 + 16 * b + 4 * g4 + r, t1 - 1));
+    }
     auto load_epilogue = [&]() {
         if (sw != 0) return;
         if constexpr (!BLK) {
 #pragma unroll
             for (int b = 0; b < NT; ++b)
 #pragma unroll
-                for (int r = 0; r < NR; ++r) tsc[b][r] = a.ascale[row_of(min(t0 + 16 * b + 4 * g4 + r, t1 - 1))];
+                for (int r = 0; r < NR; ++r) tsc[b][r] = a.ascale[GRP ? trow[b][r] : (uint32_t)min(t0 + 16 * b + 4 * g4 + r, t1 - 1)];
         }
         if (GRP || !a.residual) return;
 #pragma unroll
