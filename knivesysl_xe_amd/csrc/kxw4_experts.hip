@@ -4,15 +4,17 @@
 // is dense. The arithmetic of a row is that of kxw4_gemm under the split count
 // of expert_splits (one on the large tiles).
 //
-// Grouped instances of the strip kernel and of the large-tile kernel do the
-// work; a work-group finds its expert and tile from the plan's offsets
+// Grouped instances of the strip kernel and of the two large-tile kernels do
+// the work; a work-group finds its expert and tile from the plan's offsets
 // (kxw4_groups.hpp), and the activations are read through the plan's order, so
 // no copy of them is made. What bounds them: with few rows an expert, reading
 // the weights (128 rows over 64 experts, 2 x 1,024 rows, K = 5120: 46.7 us for
 // 300 MB, 6.4 TB/s, a pure read's rate); with many, the large tiles' FP32 chain
 // beside the MFMAs, the power limit and the last round of work-groups (16,384
-// rows: 227 us, 1.51 POPS; strips 402 us).
+// rows: 227 us, 1.51 POPS; strips 402 us; with K32 blocks the chain, three VALU
+// operations per output and unit, x 1,024 rows 333 us, 0.52 POPS; strips 403).
 #include "kxw4_gemm3.hpp"
+#include "kxw4_gemmr.hpp"
 #include "kxw4_route.hpp"
 #include "kxw4_strip.hpp"
 
@@ -86,10 +88,8 @@ static int ex_shape(const ExpertArgs &x, int TT, hipStream_t st) {
     }
 }
 
-// Tiles of 32 TA places x 32 TB WNW rows of the large-tile kernel.
-template <int TA, int TB, int WNW, int UNIT, int NST, int OCC>
-static int ex_tiles(const ExpertArgs &x, hipStream_t st) {
-    using S = G3Shape<TA, TB, 1, WNW, UNIT, 0>;
+// The arguments of a large-tile launch whose tiles have `rgs` row-groups.
+static GemmArgs ex_args(const ExpertArgs &x, int rgs) {
     GemmArgs a{};
     int nt = 0;
     for (int i = 0; i < x.count; ++i) {
@@ -98,7 +98,7 @@ static int ex_tiles(const ExpertArgs &x, hipStream_t st) {
         a.w[i].y = x.w[i].y;
         a.w[i].M = x.w[i].M;
         a.w[i].nt_begin = nt;
-        nt += (x.w[i].M / 16 + S::BNG - 1) / S::BNG;
+        nt += (x.w[i].M / 16 + rgs - 1) / rgs;
     }
     a.count = x.count;
     a.q = x.q;
@@ -113,12 +113,37 @@ static int ex_tiles(const ExpertArgs &x, hipStream_t st) {
     a.groups = x.groups;
     a.k = x.k;
     a.rows = x.rows;
-    const long long grid = tiles_at_most(x.N, x.groups, S::BM) * nt;
+    return a;
+}
+
+// Tiles of 32 TA places x 32 TB WNW rows of the large-tile kernel.
+template <int TA, int TB, int WNW, int UNIT, int NST, int OCC>
+static int ex_tiles(const ExpertArgs &x, hipStream_t st) {
+    using S = G3Shape<TA, TB, 1, WNW, UNIT, 0>;
+    const GemmArgs a = ex_args(x, S::BNG);
+    const long long grid = tiles_at_most(x.N, x.groups, S::BM) * a.n_tiles;
     if (grid >= (1ll << 31)) return -2;
     auto k = gemm3_group_kernel<TA, TB, WNW, UNIT, NST, OCC>;
     // (the shorter tiles' output staging may take more than their stages)
     const size_t lds = std::max({S::template lds_bytes<NST>(), G3Shape<(TA > 1 ? TA / 2 : 1), TB, 1, WNW, UNIT, 0>::template lds_bytes<NST>(),
                                  G3Shape<1, TB, 1, WNW, UNIT, 0>::template lds_bytes<NST>()});
+    static bool done[64] = {};
+    const int rc = ex_lds(reinterpret_cast<const void *>(k), lds, done);
+    if (rc) return rc;
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(S::NTH), lds, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -6;
+}
+
+// Tiles of 64 places x 128 rows of the reference-mode kernel.
+template <int GROUP>
+static int ex_blocks(const ExpertArgs &x, hipStream_t st) {
+    constexpr int NST = 2;
+    using S = GrShape<2, 4, 1, GROUP>;
+    const GemmArgs a = ex_args(x, S::RGS);
+    const long long grid = tiles_at_most(x.N, x.groups, S::BM) * a.n_tiles;
+    if (grid >= (1ll << 31)) return -2;
+    auto k = gemmr_group_kernel<GROUP, NST, 4>;
+    const size_t lds = std::max(S::template lds_bytes<NST>(), GrShape<1, 4, 1, GROUP>::template lds_bytes<NST>());
     static bool done[64] = {};
     const int rc = ex_lds(reinterpret_cast<const void *>(k), lds, done);
     if (rc) return rc;
@@ -134,6 +159,7 @@ int launch_experts(const ExpertArgs &x, hipStream_t st) {
     }
     const int route = expert_route(s);
     if (s.w8) return ex_shape<32, true, kStW8>(x, route, st);
+    if (route == kExpertBlock64) return x.group == 32 ? ex_blocks<32>(x, st) : ex_blocks<64>(x, st);
     if (s.blocks) return ex_shape<32, true, kStW4>(x, route, st);
     if (x.group == 128) {
         switch (route) {

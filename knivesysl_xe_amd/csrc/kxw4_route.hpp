@@ -199,13 +199,14 @@ inline bool packed_general(const PackedShape &s) {
     return others > general;
 }
 
-// The experts' projections: strips of 16 weight rows x `tokens` places, or (per
-// token) tiles of the large-tile kernel.
+// The experts' projections: strips of 16 weight rows x some places, or tiles of
+// the large-tile kernels.
 enum ExpertRoute {
     kExpertStrip2 = 2, kExpertStrip8 = 8, kExpertStrip16 = 16, kExpertStrip32 = 32,
     kExpertTile32 = 132,              // 32 places x 128 rows
     kExpertTile64 = 164,              // 64 x 256
-    kExpertTile128 = 228              // 128 x 256, group 128
+    kExpertTile128 = 228,             // 128 x 256, group 128
+    kExpertBlock64 = 264              // 64 x 128 of the reference-mode kernel
 };
 
 struct ExpertShape {
@@ -244,6 +245,12 @@ inline int expert_route(const ExpertShape &s) {
         if (each < 30 || !fits || tiles(64, s.rows256) < s.cus) return kExpertTile32;
         return s.group == 128 && each >= 128 && tiles(128, s.rows256) >= 3 * s.cus ? kExpertTile128 : kExpertTile64;
     }
+    // K32 blocks, zero points: tiles of 64 places x 128 rows while there are
+    // three for each CU (strips of 32 / tiles: 64 experts of 256, 1,024 rows, K =
+    // 5120, group 64 399 / 311, group 32 403 / 333; 64 of 64, 2 x 1,024 244 /
+    // 217; 64 of 187, 512 rows, 768 tiles: 75 / 71; 32 of 125, 1,024 rows, 512
+    // tiles: 119 / 117; 40 of 45, 1,408 rows, 440 tiles: 44 / 51).
+    if (s.blocks && !s.w8 && each >= 48 && tiles(64, s.rows128) >= 3 * s.cus) return kExpertBlock64;
     // Strips: 8 places below four rows each (16 experts of 4, K32 blocks, 2 x
     // 1,472 10.0 / 8.9 on 16; 64 of 2 per token, 2 x 1,024 46.7 / 50.4), 16
     // places below 28 (32 of 24, K32 blocks, 2 x 512 14.6 / 15.1 on 32; of 33, 2

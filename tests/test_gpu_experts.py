@@ -136,11 +136,12 @@ def test_a_row_has_the_bits_of_its_experts_own_projection(mode, T, groups, K, M)
     assert any(same)
 
 
-@pytest.mark.parametrize("mode", ["token128", "token64"])
-@pytest.mark.parametrize("T,groups,K,Ms", [
-    (700, 40, 384, [144, 272]),                              # tiles of 32 places x 128 rows
-    (2100, 8, 256, [512, 496]),                              # 64 x 256
-    (4150, 16, 128, [1040, 1040]),                           # group 128: 128 x 256
+@pytest.mark.parametrize("mode,T,groups,K,Ms", [
+    ("token128", 700, 40, 384, [144, 272]), ("token64", 700, 40, 384, [144, 272]),       # tiles of 32 places x 128 rows
+    ("token128", 2100, 8, 256, [512, 496]), ("token64", 2100, 8, 256, [512, 496]),       # 64 x 256
+    ("token128", 4150, 16, 128, [1040, 1040]), ("token64", 4150, 16, 128, [1040, 1040]),  # group 128: 128 x 256
+    ("block32", 1600, 24, 256, [704, 688]), ("block64", 1600, 24, 256, [704, 688]),      # K32 blocks: 64 x 128
+    ("block32", 3100, 100, 128, [512]),
 ])
 def test_large_tiles(mode, T, groups, K, Ms):
     # uneven experts: some with no rows, one row, and most of them; the bits of

@@ -229,6 +229,11 @@ def test_w4a4_tiles(rules, M, T, small):
     ("w8", 32, 840, 64, [256, 256], 16),                 # 9.8, of 32 11.4
     ("w8", 32, 2168, 128, [768, 768], 32),               # 93, of 16 99
     ("token", 128, 1, 1, [16], 8),
+    ("block", 64, 16384, 64, [1024], 264),               # 311, strips 399
+    ("block", 32, 12000, 64, [512], 264),                # 71, strips 75
+    ("block", 32, 4000, 32, [1024], 32),                 # 512 tiles: 119, tiles 117
+    ("block", 32, 1800, 40, [1408], 32),                 # 44, tiles 51
+    ("w8", 32, 16384, 64, [1024], 32),
 ])
 def test_expert_tiles(rules, mode, group, N, experts, rows, want):
     r128, r256 = (sum((m + w - 1) // w for m in rows) for w in (128, 256))
