@@ -330,7 +330,8 @@ int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count,
  * Products are exact and summed in FP32, A x is held in FP32, out is rounded
  * once. K % 128 == 0, M % 16 == 0 (as the projection's weight), r a multiple
  * of 8 up to 256 (pad smaller ranks with zeros); 16-byte aligned pointers.
- * workspace: kxw4_adapter_workspace bytes, this call's own while it runs. */
+ * workspace: kxw4_adapter_workspace bytes (then it may be NULL when that is 0),
+ * this call's own while it runs. */
 typedef struct kxw4_adapters {
     int32_t n, r, K, M;
     const uint16_t *a, *b;

@@ -616,8 +616,8 @@ int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count,
 }
 
 size_t kxw4_adapter_workspace(const kxw4_adapters_t *ad, int T) {
-    if (!ad || T <= 0 || ad->n <= 0 || ad->r <= 0 || ad->K <= 0) return 0;
-    return adapter_scratch(ad->n, T, ad->r, ad->K);
+    if (!ad || T <= 0 || ad->n <= 0 || ad->r <= 0 || ad->K <= 0 || ad->M <= 0) return 0;
+    return adapter_scratch(ad->n, T, ad->r, ad->K, ad->M);
 }
 
 int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, const kxw4_adapters_t *ad,
@@ -630,7 +630,8 @@ int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, con
         return KXW4_ESHAPE;
     if (!valid_dtype(y_dtype) || !valid_dtype(x_dtype)) return KXW4_ESHAPE;
     if (route->T == 0) return KXW4_OK;
-    if (!y || !x || !out || !workspace || !ad->a || !ad->b || !ad->scale) return KXW4_EARG;
+    if (!y || !x || !out || !ad->a || !ad->b || !ad->scale) return KXW4_EARG;
+    if (!workspace && kxw4_adapter_workspace(ad, route->T)) return KXW4_EARG;
     if (!aligned(y, 16) || !aligned(x, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(ad->a, 16) ||
         !aligned(ad->b, 16) || !aligned(ad->scale, 4))
         return KXW4_EARG;

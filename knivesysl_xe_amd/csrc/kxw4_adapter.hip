@@ -3,14 +3,16 @@
 // t, out[t] = y[t] for a token without one. No counterpart in the reference.
 //
 // The tokens come sorted by adapter (RouteArgs' plan with one choice per
-// token), in tiles that belong to one adapter. Two launches: `low` = A x into
-// FP32 scratch, K split over waves and work-groups, then the update.
+// token), in tiles that belong to one adapter. `low` = A x comes first, K split
+// over waves and work-groups, then the update: in one launch where both are
+// short, else in two with `low` in scratch between them, and for many tokens in
+// two that keep B in registers.
 //
 // Arithmetic. A and B are BF16, so a BF16 x makes exact products on the BF16
 // MFMA, summed in FP32. An FP32 value is cut into three BF16 parts of eight
 // mantissa bits each, which hold all 24 (split3), and each part takes an MFMA
-// of its own: the products are exact again. `low` stays FP32 between the
-// launches and is cut the same way. The sums run in a fixed order: within a
+// of its own: the products are exact again. `low` is held in FP32 and cut the
+// same way. The sums run in a fixed order: within a
 // wave's steps, then the waves of a work-group, then the work-groups' parts.
 //
 // v_mfma_f32_16x16x32_bf16: lane l supplies row (A) / column (B) l%16 and the
@@ -84,32 +86,17 @@ constexpr int kLowTile = 16, kFewWaves = 4;
 __host__ __device__ constexpr int chunks_of(int r) { return (r + 31) / 32; }
 constexpr int kCutChunk = 3 * 64 * 8;
 
-// low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
-// work-group takes 16 places of one adapter and part s, its WAVES waves
-// consecutive runs of 32-K steps, all r columns (CT tiles of 16). Operands come
-// straight from memory: a step's x piece is used by every column tile, an A
-// piece once. CUT: one part; scale * low is cut into its three BF16 parts here,
-// in the order the second launch's operand takes them.
-template <int CT, int WAVES, bool XB, bool CUT>
-__global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
-    __shared__ float part[WAVES - 1][CT][256];
-    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
-    if ((int)blockIdx.x >= tiles.total) return;
-    const GroupTile tile = tile_at(tiles, a.offsets, kLowTile, blockIdx.x);
-    const int p0 = tile.begin + tile.index * kLowTile;
-    const int steps = a.K / 32, ways = a.splits * WAVES, way = blockIdx.y * WAVES + wave;
-    const int k0 = (int)((long long)steps * way / ways), k1 = (int)((long long)steps * (way + 1) / ways);
-
+// acc[c] = the 32-K steps [k0, k1) of A_e's columns 16 c .. + 15 times x. Each
+// lane loads 16-byte pieces of the row of `token` (place lane / 4 of the tile) and
+// of A's rows; a step's x piece is used by every column tile, an A piece once.
+template <int CT, bool XB>
+__device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, int token, int k0, int k1, int lane, v4f (&acc)[CT]) {
     const int lr = lane >> 2, lk = 8 * (lane & 3);           // row and columns that this lane loads
-    const int token = a.order[min(p0 + lr, tile.end - 1)];
     const size_t xrow = (size_t)token * a.K + lk;
     const uint16_t *arow[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
-        arow[c] = a.a + ((size_t)tile.e * a.r + min(c * 16 + lr, a.r - 1)) * a.K + lk;
-    v4f acc[CT];
+        arow[c] = a.a + ((size_t)e * a.r + min(c * 16 + lr, a.r - 1)) * a.K + lk;
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     // U steps' loads are requested before the first of them is used
@@ -157,7 +144,33 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterAr
     constexpr int kSteps = CT <= 2 ? 4 : CT <= 4 ? 2 : 1;
     int k = k0;
     for (; k + kSteps <= k1; k += kSteps) run(k, std::integral_constant<int, kSteps>{});
+    if constexpr (kSteps > 2) {
+        if (k + 2 <= k1) {
+            run(k, std::integral_constant<int, 2>{});
+            k += 2;
+        }
+    }
     for (; k < k1; ++k) run(k, std::integral_constant<int, 1>{});
+}
+
+// low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
+// work-group takes 16 places of one adapter and part s, its WAVES waves
+// consecutive runs of 32-K steps, all r columns (CT tiles of 16). CUT: one part; scale * low is cut into its three BF16 parts here,
+// in the order the second launch's operand takes them.
+template <int CT, int WAVES, bool XB, bool CUT>
+__global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
+    __shared__ float part[WAVES - 1][CT][256];
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
+    if ((int)blockIdx.x >= tiles.total) return;
+    const GroupTile tile = tile_at(tiles, a.offsets, kLowTile, blockIdx.x);
+    const int p0 = tile.begin + tile.index * kLowTile;
+    const int steps = a.K / 32, ways = a.splits * WAVES, way = blockIdx.y * WAVES + wave;
+    const int k0 = (int)((long long)steps * way / ways), k1 = (int)((long long)steps * (way + 1) / ways);
+
+    v4f acc[CT];
+    low_steps<CT, XB>(a, tile.e, a.order[min(p0 + (lane >> 2), tile.end - 1)], k0, k1, lane, acc);
     if (wave > 0) {
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -222,6 +235,28 @@ constexpr int kUpWaves = 4, kUpRows = 64, kUpBlock = kUpWaves * kUpRows;
 // BF16 elements of a token's row of one part: r padded to whole MFMAs, with 16
 // bytes more so that neighbouring rows start in different banks
 __host__ __device__ constexpr int up_pitch(int r) { return 32 * chunks_of(r) + 8; }
+
+// out = y + acc for a lane's pieces of one token, rounded once; piece q's
+// outputs are acc[2 q], acc[2 q + 1] (BF16) or acc[q].
+template <int NY, bool YB, class Col>
+__device__ __forceinline__ void store_up(const AdapterArgs &a, size_t at, Col col, const v4u (&yv)[NY], const v4f (&acc)[4]) {
+#pragma unroll
+    for (int q = 0; q < NY; ++q) {
+        if (col(q) >= a.M) continue;
+        v4u o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (YB) {
+                const v4f f = acc[2 * q + (i >> 1)];
+                o[i] = pack_bf16(__uint_as_float(yv[q][i] << 16) + f[2 * (i & 1)],
+                                 __uint_as_float(yv[q][i] & 0xFFFF0000u) + f[2 * (i & 1) + 1]);
+            } else {
+                o[i] = __float_as_uint(__uint_as_float(yv[q][i]) + acc[q][i]);
+            }
+        }
+        *reinterpret_cast<v4u *>(static_cast<uint8_t *>(a.out) + (at + col(q)) * (YB ? 2 : 4)) = o;
+    }
+}
 
 // KC: 32-column chunks of B requested together.
 template <int KC, bool YB>
@@ -309,22 +344,91 @@ __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const Adapter
         }
     }
     if (!on || p0 + n >= p1) return;
-#pragma unroll
-    for (int q = 0; q < NY; ++q) {
-        if (col(q) >= a.M) continue;
-        v4u o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (YB) {
-                const v4f f = acc[2 * q + (i >> 1)];
-                o[i] = pack_bf16(__uint_as_float(yv[q][i] << 16) + f[2 * (i & 1)],
-                                 __uint_as_float(yv[q][i] & 0xFFFF0000u) + f[2 * (i & 1) + 1]);
-            } else {
-                o[i] = __float_as_uint(__uint_as_float(yv[q][i]) + acc[q][i]);
-            }
-        }
-        *reinterpret_cast<v4u *>(static_cast<uint8_t *>(a.out) + (at + col(q)) * (YB ? 2 : 4)) = o;
+    store_up<NY, YB>(a, at, [&](int q) { return col(q); }, yv, acc);
+}
+
+// Both in one launch, for few tokens and small adapters: a work-group takes 16
+// places of one adapter x 1,024 rows of B, 64 a wave, and works out the whole
+// `low` of its places first, its sixteen waves K split between them. The A rows
+// are read again by every work-group of a tile, from the L2 (one_launch says what
+// that costs and saves).
+constexpr int kOneWaves = 16, kOneBlock = kOneWaves * kUpRows;
+template <int CT, bool XB, bool YB>
+__global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(const AdapterArgs a) {
+    constexpr int NY = YB ? 2 : 4, PITCH = up_pitch(16 * CT);
+    __shared__ float part[kOneWaves][CT][256];
+    __shared__ __attribute__((aligned(16))) uint16_t cut[3 * kLowTile * PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int mblocks = (a.M + kOneBlock - 1) / kOneBlock;
+    const int u = blockIdx.x / mblocks, m0 = (blockIdx.x - u * mblocks) * kOneBlock + wave * kUpRows;
+    const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
+    int p0, p1, e = -1;
+    if (u < tiles.total) {
+        const GroupTile tile = tile_at(tiles, a.offsets, kLowTile, u);
+        e = tile.e;
+        p0 = tile.begin + tile.index * kLowTile;
+        p1 = tile.end;
+    } else {
+        // the tokens without an adapter keep y (already there when out is y)
+        p0 = a.offsets[a.n] + (u - tiles.total) * kLowTile;
+        p1 = a.T;
+        if (a.out == a.y || p0 >= p1) return;
     }
+    const bool on = m0 < a.M;                                // (the others only help with `low`)
+    const int row = a.order[min(p0 + (lane >> 2), p1 - 1)];
+    const size_t at = (size_t)a.order[min(p0 + n, p1 - 1)] * a.M;
+    // (columns and rows as in adapter_up_kernel)
+    auto col = [&](int q) { return m0 + (YB ? 32 * q + 8 * g : 16 * q + 4 * g); };
+    auto brow = [&](int c) { return m0 + (YB ? 32 * (c >> 1) + 8 * (n >> 2) + 4 * (c & 1) + (n & 3) : 16 * c + n); };
+    v4u yv[NY], b[4];
+#pragma unroll
+    for (int q = 0; q < NY; ++q)
+        yv[q] = *reinterpret_cast<const v4u *>(static_cast<const uint8_t *>(a.y) + (at + min(col(q), a.M - (YB ? 8 : 4))) * (YB ? 2 : 4));
+    v4f acc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (e >= 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            b[c] = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(brow(c), a.M - 1)) * a.r + min(8 * g, a.r - 8));
+        const int steps = a.K / 32;
+        v4f low[CT];
+        low_steps<CT, XB>(a, e, row, steps * wave / kOneWaves, steps * (wave + 1) / kOneWaves, lane, low);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[wave][c][i * 64 + lane] = low[c][i];
+        __syncthreads();
+        // element i of tile c: token 4 (i%64 / 16) + i / 64, column 16 c + i % 16
+        if (tid < 512) {
+            const int c = tid >> 8, i = tid & 255, t = 4 * ((i & 63) >> 4) + (i >> 6), column = 16 * c + (i & 15);
+            float v = 0.0f;
+            if (c < CT && column < a.r) {
+#pragma unroll
+                for (int w = 0; w < kOneWaves; ++w) v += part[w][min(c, CT - 1)][i];
+                v *= a.scale[e];
+            }
+            uint32_t w[3];
+            split3(v, w);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) cut[(q * kLowTile + t) * PITCH + column] = (uint16_t)(w[q] >> 16);
+        }
+        __syncthreads();
+        if (!on) return;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) b[c][x] = 8 * g < a.r ? b[c][x] : 0u;
+#pragma unroll
+        for (int q = 2; q >= 0; --q) {
+            const v4u x = *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * PITCH + 8 * g);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = mfma_bf16(b[c], x, acc[c]);
+        }
+    }
+    if (!on || p0 + n >= p1) return;
+    store_up<NY, YB>(a, at, [&](int q) { return col(q); }, yv, acc);
 }
 
 // The same for many tokens. A wave takes 128 rows of B, whose operands stay in
@@ -475,9 +579,31 @@ static int adapter_splits(int n, int T, int K) {
     return (int)std::max(1ll, std::min({most, 1024 / tiles, 8ll}));
 }
 
-size_t adapter_scratch(int n, int T, int r, int K) {
+// One launch, while a work-group's waves have at most ten 32-K steps of one
+// column tile each and every CU at most one work-group: the host's second
+// launch costs more than what the GPU loses (us two launches / one, called in
+// turn; replayed from a graph: 1 to 8 tokens of as many adapters, K = M = 5120, r
+// = 16 14.2 / 10.1; 7.1 / 7.8; 64 of 64, 4,096 14.3 / 9.9; 8.4 / 8.1; 4 of 4, K =
+// 1024, M = 4096, float32 14.3 / 10.0; 8.0 / 6.1; 16 of 16, K = 17408 14.2 / 16.7;
+// 8.4 / 17.4; 200 of 100, r = 32 21.4 / 39.1).
+static bool one_launch(int n, int T, int r, int K, int M) {
+    const long long groups = (tiles_at_most(T, n, kLowTile) + 1) * ((M + kOneBlock - 1) / kOneBlock);
+    return (long long)(r + 15) / 16 * K <= 5120 && r <= 32 && groups <= device_cus();
+}
+
+size_t adapter_scratch(int n, int T, int r, int K, int M) {
     if (many_tokens(n, T, r)) return (size_t)tiles_at_most(T, n, kLowTile) * chunks_of(r) * kCutChunk * 2;
-    return (size_t)adapter_splits(n, T, K) * T * r * sizeof(float);
+    return one_launch(n, T, r, K, M) ? 0 : (size_t)adapter_splits(n, T, K) * T * r * sizeof(float);
+}
+
+template <int CT>
+static int launch_one(const AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
+    const long long grid = (tiles_at_most(a.T, a.n, kLowTile) + 1) * ((a.M + kOneBlock - 1) / kOneBlock);
+    if (grid >= (1ll << 31)) return -2;
+    auto k = x_bf16 ? (y_bf16 ? adapter_one_kernel<CT, true, true> : adapter_one_kernel<CT, true, false>)
+                    : (y_bf16 ? adapter_one_kernel<CT, false, true> : adapter_one_kernel<CT, false, false>);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * kOneWaves), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 template <int CT, int WAVES, bool CUT>
@@ -521,6 +647,7 @@ int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
         else launch_low<8, 8, true>(a, x_bf16, st);
         return a.r <= 32 ? launch_many<1>(a, y_bf16, st) : a.r <= 64 ? launch_many<2>(a, y_bf16, st) : launch_many<4>(a, y_bf16, st);
     }
+    if (one_launch(a.n, a.T, a.r, a.K, a.M)) return a.r <= 16 ? launch_one<1>(a, x_bf16, y_bf16, st) : launch_one<2>(a, x_bf16, y_bf16, st);
     a.splits = adapter_splits(a.n, a.T, a.K);
     if (a.r <= 16) launch_low<1, kFewWaves, false>(a, x_bf16, st);
     else if (a.r <= 32) launch_low<2, kFewWaves, false>(a, x_bf16, st);

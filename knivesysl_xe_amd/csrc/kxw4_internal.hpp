@@ -226,7 +226,7 @@ struct AdapterArgs {
     int T, n, r, K, M;
     int splits, run;                  // (set by the launcher)
 };
-size_t adapter_scratch(int n, int T, int r, int K);       // bytes of `low`
+size_t adapter_scratch(int n, int T, int r, int K, int M);      // bytes of `low`
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st);
 
 // Returns 1 (nothing launched) outside the per-token, one-split-per-token mode.

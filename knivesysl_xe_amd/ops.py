@@ -495,22 +495,31 @@ def gemm_w4a4(w: W4Weight, a: QuantActS4, dtype=torch.float32, residual=None,
 
 def _gpu(t, name: str) -> torch.device:
     """The GPU of a call's first tensor, which the others have to share."""
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        return t.device
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be on the GPU")
-    return t.device
+    raise ValueError(f"{name} must be on the GPU")
+
+
+_FUNCTIONS = {}
 
 
 def _launch(name: str, device: torch.device, *args) -> None:
     """Call `name` on the current stream of `device`, which need not be the
-    current device."""
+    current device. (A small launch is bound by the host, so its path here is
+    kept short.)"""
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(lib(), name)
     i = device.index
-    if i == torch.cuda.current_device():
-        check(name, getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i)))
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(i):
-            check(name, getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(i)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        check(name, rc)
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -711,9 +720,10 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     _need(adapters.scale, "adapters.scale", torch.float32, (n,), dev)
     o = _need(out, "out", y.dtype, (T, M), dev) if out is not None else torch.empty_like(y)
     ad, rc = adapters.c(), route.c()
-    ws = torch.empty(lib().kxw4_adapter_workspace(C.byref(ad), T), dtype=torch.uint8, device=dev)
+    nbytes = lib().kxw4_adapter_workspace(C.byref(ad), T)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("kxw4_adapter_add", dev, y.data_ptr(), _dtype_code(y.dtype), x.data_ptr(), _dtype_code(x.dtype),
-            C.byref(ad), C.byref(rc), o.data_ptr(), ws.data_ptr())
+            C.byref(ad), C.byref(rc), o.data_ptr(), _ptr(ws))
     return o
 
 

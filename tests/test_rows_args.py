@@ -115,14 +115,16 @@ def test_adapter_add_refuses_bad_arguments():
     assert call(yt=2) == call(xt=2) == _lib.ESHAPE
     odd = C.c_void_p(72)
     for name in ("y", "x", "out", "ws"):
-        assert call(**{name: None}) == call(**{name: odd}) == _lib.EARG
+        assert call(ad=D(r=64), **{name: None}) == call(ad=D(r=64), **{name: odd}) == _lib.EARG
     for name in ("a", "b", "scale"):
         assert call(ad=D(**{name: None})) == _lib.EARG
     assert call(ad=D(a=72)) == call(ad=D(b=72)) == call(ad=D(scale=66)) == _lib.EARG
     assert call(r=R(T=0, k=1, offsets=None, order=None, position=None), y=None, x=None, out=None, ws=None) == 0
     size = L.kxw4_adapter_workspace
     assert size(None, 8) == 0 and size(C.byref(D()), 0) == 0
-    assert size(C.byref(D()), 8) % (8 * 16 * 4) == 0 and size(C.byref(D()), 8) >= 8 * 16 * 4
+    # two launches keep the low rows of every part between them, one nothing
+    assert size(C.byref(D(r=64)), 8) % (8 * 64 * 4) == 0 and size(C.byref(D(r=64)), 8) >= 8 * 64 * 4
+    assert size(C.byref(D()), 8) == 0 and size(C.byref(D(K=17408)), 8) > 0
 
 
 def test_front_end_refuses_host_tensors():
