@@ -281,7 +281,7 @@ int kxw4_gemm_w4a4(const kxw4_weight_t *w, const uint8_t *q4, const float *scale
  * (kxw4_route_rows still clears the offsets). Limits: groups 1..1024, T*k up
  * to 2^30 slots. Row buffers of N rows are written up to offsets[groups];
  * what lies behind stays as it was. Outputs must not overlap inputs unless
- * said. Results do not depend on the order in which work-groups run. */
+ * said (the same pointer for both is refused with -1). Results do not depend on the order in which work-groups run. */
 typedef struct kxw4_route {
     int32_t T, k, groups;
     int32_t *offsets, *order, *position;

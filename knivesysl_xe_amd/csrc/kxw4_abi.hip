@@ -515,7 +515,7 @@ int kxw4_dispatch_rows(const void *x, int dtype, int H, const kxw4_route_t *rout
     if (rc) return rc;
     if (!valid_dtype(dtype)) return KXW4_ESHAPE;
     if (route->T == 0) return KXW4_OK;
-    if (!x || !rows || !aligned(x, elem_bytes(dtype)) || !aligned(rows, elem_bytes(dtype))) return KXW4_EARG;
+    if (!x || !rows || x == rows || !aligned(x, elem_bytes(dtype)) || !aligned(rows, elem_bytes(dtype))) return KXW4_EARG;
     RowArgs a{};
     a.x = x;
     a.rows = rows;
@@ -532,7 +532,7 @@ int kxw4_combine_rows(const void *rows, int rows_dtype, int H, const float *weig
     if (rc) return rc;
     if (!valid_dtype(rows_dtype) || !valid_dtype(y_dtype)) return KXW4_ESHAPE;
     if (route->T == 0) return KXW4_OK;
-    if (!rows || !y || !aligned(rows, elem_bytes(rows_dtype)) || !aligned(y, elem_bytes(y_dtype)) || !aligned(weights, 4))
+    if (!rows || !y || rows == y || !aligned(rows, elem_bytes(rows_dtype)) || !aligned(y, elem_bytes(y_dtype)) || !aligned(weights, 4))
         return KXW4_EARG;
     RowArgs a{};
     a.rows = const_cast<void *>(rows);
@@ -552,7 +552,7 @@ int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, i
     if (rc) return rc;
     if (!valid_dtype(dy_dtype) || !valid_dtype(rows_dtype)) return KXW4_ESHAPE;
     if (route->T == 0) return KXW4_OK;
-    if (!dy || !rows || !weights || !drows || !dweights) return KXW4_EARG;
+    if (!dy || !rows || !weights || !drows || !dweights || drows == rows || drows == dy) return KXW4_EARG;
     if (!aligned(dy, elem_bytes(dy_dtype)) || !aligned(rows, elem_bytes(rows_dtype)) ||
         !aligned(drows, elem_bytes(rows_dtype)) || !aligned(weights, 4) || !aligned(dweights, 4))
         return KXW4_EARG;
@@ -630,7 +630,7 @@ int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, con
         return KXW4_ESHAPE;
     if (!valid_dtype(y_dtype) || !valid_dtype(x_dtype)) return KXW4_ESHAPE;
     if (route->T == 0) return KXW4_OK;
-    if (!y || !x || !out || !ad->a || !ad->b || !ad->scale) return KXW4_EARG;
+    if (!y || !x || !out || out == x || !ad->a || !ad->b || !ad->scale) return KXW4_EARG;
     if (!workspace && kxw4_adapter_workspace(ad, route->T)) return KXW4_EARG;
     if (!aligned(y, 16) || !aligned(x, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(ad->a, 16) ||
         !aligned(ad->b, 16) || !aligned(ad->scale, 4))

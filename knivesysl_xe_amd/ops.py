@@ -553,6 +553,8 @@ class RowRoute:
 def _check_route(r: RowRoute, device) -> RowRoute:
     if not isinstance(r, RowRoute):
         raise ValueError("route must be a RowRoute")
+    if r.T < 0 or r.k < 1 or r.groups < 1:
+        raise ValueError(f"route has T {r.T}, k {r.k}, groups {r.groups}")
     _need(r.offsets, "route offsets", torch.int32, (r.groups + 1,), device)
     _need(r.order, "route order", torch.int32, (r.T * r.k,), device)
     _need(r.position, "route position", torch.int32, (r.T, r.k), device)
@@ -656,12 +658,15 @@ def expert_gemm_fanout(ws: Sequence[W4Weight], a: QuantAct, route: RowRoute, dty
     rows: W4Weight.from_codes of [groups * rows][K] codes. `a` holds the T
     tokens, or with sorted_rows the T*k rows in the plan's order (the hidden
     rows of a down projection)."""
+    if not 1 <= len(ws) <= 4:
+        raise ValueError(f"one to four weights, got {len(ws)}")
     dev = ws[0].codes.device
     for w in ws:
         _check_weight(w, dev)
+    _check_route(route, dev)
+    for w in ws:
         if w.M % route.groups:
             raise ValueError(f"weight rows {w.M} are not a multiple of {route.groups} groups")
-    _check_route(route, dev)
     _check_act(a, dev)
     N = route.T * route.k
     if a.T != (N if sorted_rows else route.T):

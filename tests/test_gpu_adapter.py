@@ -186,3 +186,55 @@ def test_front_end_refuses_mismatched_buffers():
     with pytest.raises(_lib.KxError):
         ops.adapter_add(torch.zeros(4, 40, device=DEV), x, make(rng, 3, 16, 256, 40), r)
     assert ops.adapter_add(y[:0], x[:0], ad, ops.route_rows(torch.zeros(0, dtype=torch.int32, device=DEV), 3)).shape == (0, 64)
+
+
+@pytest.mark.parametrize("T,n,r,K,M", [(8, 8, 16, 1024, 512), (61, 24, 64, 2048, 512), (2000, 3, 32, 512, 528)])
+def test_the_same_bits_every_time_two_streams_and_two_graphs(T, n, r, K, M):
+    rng = np.random.default_rng(T)
+    ad = make(rng, n, r, K, M)
+    route = ops.route_rows(torch.from_numpy(pick(rng, T, n)).to(DEV), n)
+    x = [normal(rng, T, K).to(DEV) for _ in range(2)]
+    y = normal(rng, T, M).to(DEV)
+    want = [ops.adapter_add(y, x[i], ad, route) for i in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, ops.adapter_add(y, x[i], ad, route)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in got)
+    # two captured steps replayed side by side: each has scratch of its own
+    graphs, outs = [], []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(ops.adapter_add(y, x[i], ad, route))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_adapters_past_two_to_the_31_elements():
+    n, r, K, M, T = 600, 256, 17408, 17408, 40               # 2.7e9 elements of a and of b
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(2)
+    a = torch.randn(n, r, K, generator=gen, device=DEV, dtype=torch.bfloat16) / K ** 0.5
+    b = torch.randn(n, M, r, generator=gen, device=DEV, dtype=torch.bfloat16) / r ** 0.5
+    ad = ops.Adapters(a, b, torch.rand(n, generator=gen, device=DEV) + 0.5)
+    ids = torch.tensor([599, 0, 598, 300, -1] * 8, dtype=torch.int32, device=DEV)
+    x = torch.randn(T, K, generator=gen, device=DEV)
+    y = torch.randn(T, M, generator=gen, device=DEV)
+    got = ops.adapter_add(y, x, ad, ops.route_rows(ids, n))
+    part = ops.Adapters(a[[0, 300, 598, 599]], b[[0, 300, 598, 599]], ad.scale[[0, 300, 598, 599]])
+    local = np.array([{599: 3, 0: 0, 598: 2, 300: 1, -1: -1}[i] for i in ids.tolist()])
+    check(got, y, x, part, local)

@@ -258,3 +258,45 @@ def test_another_stream():
         got = ops.expert_gemm(w, a, ops.route_rows(torch.from_numpy(ids).to(DEV), 4), out=out)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("mode", ["token128", "block32"])
+def test_weights_past_two_to_the_31_codes(mode):
+    # the last experts' codes and scales lie past 32-bit offsets
+    group, block, enc = MODES[mode]
+    groups, M, K, T = 70, 2048, 17408, 9                     # 2.5e9 codes
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(3)
+    codes = torch.randint(0, 256, (groups * M * K // 2,), generator=gen, device=DEV, dtype=torch.uint8)
+    scales = (torch.rand(groups * M * (K // group), generator=gen, device=DEV) * 0.02).half().view(torch.int16)
+    w = ops.W4Weight(groups * M, K, group, enc, codes, scales)
+    ids = torch.tensor([0, 69, 68, 61, 69, 35, 60, 69, 1], dtype=torch.int32, device=DEV)
+    r = ops.route_rows(ids, groups)
+    a = ops.quantize_act(torch.randn(T, K, generator=gen, device=DEV), block)
+    y = ops.expert_gemm(w, a, r)
+    for e in (0, 60, 61, 68, 69):
+        p0, p1 = int(r.offsets[e]), int(r.offsets[e + 1])
+        tokens = r.order[p0:p1].long()
+        own = [ops.gemm(slice_of(w, e, groups), rows_of(a, tokens), forced_splits=s) for s in (1, 2, 4, 8)]
+        assert any(torch.equal(o, y[p0:p1]) for o in own), e
+
+
+@pytest.mark.parametrize("mode,T,groups,K,M", [("token128", 40, 8, 1024, 64), ("w8", 300, 5, 512, 80),
+                                               ("token64", 1500, 6, 256, 1040), ("block64", 1700, 24, 128, 1408)])
+def test_the_same_bits_every_time_and_two_streams_at_once(mode, T, groups, K, M):
+    rng = np.random.default_rng(T)
+    group, block, _ = MODES[mode]
+    w, _ = weight(rng, mode, groups * M, K)
+    ids = torch.from_numpy(make_ids(rng, T, 2, groups)).to(DEV)
+    a = ops.quantize_act(torch.from_numpy(rng.standard_normal((T, K)).astype(np.float32)).to(DEV), block)
+    r = ops.route_rows(ids, groups)
+    want = ops.expert_gemm(w, a, r, out=torch.zeros(2 * T, M, device=DEV))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.expert_gemm(w, a, r, out=torch.zeros(2 * T, M, device=DEV)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)

@@ -254,3 +254,52 @@ def test_another_stream_and_a_captured_step():
         for got, want in zip(held, step()):
             assert torch.equal(got, want)
         torch.cuda.synchronize()
+
+
+def test_rows_past_two_to_the_31_elements():
+    T, k, groups, H = 66000, 8, 37, 4160                     # 2.2e9 elements of rows
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(1)
+    ids = torch.randint(-1, groups, (T, k), generator=gen, device=DEV, dtype=torch.int32)
+    r = ops.route_rows(ids, groups)
+    check_plan(r, ids.cpu().numpy(), groups)
+    x = torch.randn(T, H, generator=gen, device=DEV, dtype=torch.bfloat16)
+    w = torch.rand(T, k, generator=gen, device=DEV)
+    rows = ops.dispatch_rows(x, r)
+    live = int(r.offsets[-1])
+    at = torch.cat([torch.arange(100), torch.randint(0, live, (300,)), torch.arange(live - 100, live)]).to(DEV)
+    assert torch.equal(rows[at], x[r.order[at].long() // k])
+    y = ops.combine_rows(rows, r, w, dtype=torch.float32)
+    tokens = torch.cat([torch.arange(50), torch.arange(T - 50, T)]).to(DEV)
+    # every row of a token is its own x: y = x times the sum of its weights
+    want = x[tokens].double() * torch.where(r.position[tokens] >= 0, w[tokens], 0.0).double().sum(1, keepdim=True)
+    assert ((y[tokens].double() - want).abs() <= (k + 1) * 2.0 ** -24 * k * x[tokens].double().abs()).all()
+    drows, dw = ops.combine_rows_backward(x, rows, r, w)
+    slot = r.order[at].long()
+    assert torch.equal(drows[at], (w.reshape(-1)[slot][:, None] * x[slot // k].float()).bfloat16())
+    norm = (x[tokens].double() ** 2).sum(1, keepdim=True)
+    off = (dw[tokens].double() - torch.where(r.position[tokens] >= 0, norm, 0.0)).abs()
+    assert (off <= H * 2.0 ** -24 * norm).all()
+
+
+def test_calls_at_once_on_two_streams():
+    # the same inputs and plans, each call with scratch of its own
+    rng = np.random.default_rng(7)
+    T, k, groups, H = 20000, 2, 100, 320
+    ids = [torch.from_numpy(make_ids(rng, T, k, groups)).to(DEV) for _ in range(2)]
+    x = torch.from_numpy(rng.standard_normal((T, H)).astype(np.float32)).to(DEV)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                r = ops.route_rows(ids[i], groups)
+                rows = ops.dispatch_rows(x, r, out=torch.zeros(T * k, H, device=DEV))
+                got[i].append((r, rows, ops.combine_rows(rows, r)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        check_plan(got[i][0][0], ids[i].cpu().numpy(), groups)
+        for r, rows, y in got[i]:
+            assert torch.equal(r.order, got[i][0][0].order) and torch.equal(rows, got[i][0][1])
+            assert torch.equal(y, got[i][0][2])

@@ -8,6 +8,7 @@ import torch
 from knivesysl_xe_amd import _lib, ops
 
 P = C.c_void_p(64)
+OTHER = C.c_void_p(128)                                     # an output beside the inputs at P
 
 
 def R(T=8, k=2, groups=4, offsets=64, order=64, position=64):
@@ -49,13 +50,13 @@ def test_route_workspace_sizes():
 def test_row_calls_refuse_bad_arguments():
     L = _lib.lib()
 
-    def dispatch(x=P, dtype=0, H=64, r=R(), rows=P):
+    def dispatch(x=P, dtype=0, H=64, r=R(), rows=OTHER):
         return L.kxw4_dispatch_rows(x, dtype, H, None if r is None else C.byref(r), rows, None)
 
-    def combine(rows=P, rt=0, H=64, w=P, r=R(), y=P, yt=0):
+    def combine(rows=P, rt=0, H=64, w=P, r=R(), y=OTHER, yt=0):
         return L.kxw4_combine_rows(rows, rt, H, w, None if r is None else C.byref(r), y, yt, None)
 
-    def backward(dy=P, dt=0, rows=P, rt=0, H=64, w=P, r=R(), drows=P, dw=P):
+    def backward(dy=P, dt=0, rows=P, rt=0, H=64, w=P, r=R(), drows=OTHER, dw=P):
         return L.kxw4_combine_rows_backward(dy, dt, rows, rt, H, w, None if r is None else C.byref(r), drows, dw, None)
 
     for call in (dispatch, combine, backward):
@@ -71,6 +72,9 @@ def test_row_calls_refuse_bad_arguments():
     assert combine(rows=None) == combine(y=None) == combine(rows=odd) == combine(y=odd) == combine(w=odd) == _lib.EARG
     for name in ("dy", "rows", "w", "drows", "dw"):
         assert backward(**{name: None}) == backward(**{name: odd}) == _lib.EARG
+    # an output in the place of an input
+    assert dispatch(rows=P) == combine(y=P) == backward(drows=P) == _lib.EARG
+    assert backward(rows=C.c_void_p(256), drows=C.c_void_p(256)) == _lib.EARG
 
 
 def test_expert_gemm_refuses_bad_arguments():
@@ -104,7 +108,7 @@ def test_expert_gemm_refuses_bad_arguments():
 def test_adapter_add_refuses_bad_arguments():
     L = _lib.lib()
 
-    def call(y=P, yt=1, x=P, xt=1, ad=D(), r=R(k=1), out=P, ws=P):
+    def call(y=P, yt=1, x=OTHER, xt=1, ad=D(), r=R(k=1), out=P, ws=P):
         return L.kxw4_adapter_add(y, yt, x, xt, None if ad is None else C.byref(ad), None if r is None else C.byref(r),
                                   out, ws, None)
 
@@ -118,6 +122,7 @@ def test_adapter_add_refuses_bad_arguments():
         assert call(ad=D(r=64), **{name: None}) == call(ad=D(r=64), **{name: odd}) == _lib.EARG
     for name in ("a", "b", "scale"):
         assert call(ad=D(**{name: None})) == _lib.EARG
+    assert call(out=OTHER) == _lib.EARG                                  # out in the place of x
     assert call(ad=D(a=72)) == call(ad=D(b=72)) == call(ad=D(scale=66)) == _lib.EARG
     assert call(r=R(T=0, k=1, offsets=None, order=None, position=None), y=None, x=None, out=None, ws=None) == 0
     size = L.kxw4_adapter_workspace
@@ -143,6 +148,10 @@ def test_front_end_refuses_host_tensors():
     with pytest.raises(ValueError, match="must be a torch.Tensor"):
         ops.route_rows([[1, 2]], 8)
     w = ops.W4Weight(64, 128, 128, 0, torch.zeros(64 * 64, dtype=torch.uint8), torch.zeros(64, dtype=torch.int16))
+    with pytest.raises(ValueError, match="one to four weights, got 0"):
+        ops.expert_gemm_fanout([], ops.QuantAct.empty(4, 128, 0, "cpu"), r)
+    with pytest.raises(ValueError, match="one to four weights, got 5"):
+        ops.expert_gemm_fanout([w] * 5, ops.QuantAct.empty(4, 128, 0, "cpu"), r)
     with pytest.raises(ValueError, match="weights must be on the GPU"):
         ops.expert_gemm(w, ops.QuantAct.empty(4, 128, 0, "cpu"), r)
 
@@ -152,6 +161,8 @@ def test_route_buffers_are_checked():
     assert ops._check_route(r, torch.device("cpu")) is r
     with pytest.raises(ValueError, match="must be a RowRoute"):
         ops._check_route(None, torch.device("cpu"))
+    with pytest.raises(ValueError, match="groups 0"):
+        ops._check_route(ops.RowRoute(4, 2, 0, r.offsets, r.order, r.position), torch.device("cpu"))
     short = ops.RowRoute(4, 2, 9, r.offsets, r.order, r.position)
     with pytest.raises(ValueError, match="route offsets must have shape"):
         ops._check_route(short, torch.device("cpu"))
