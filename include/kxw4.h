@@ -280,8 +280,9 @@ int kxw4_gemm_w4a4(const kxw4_weight_t *w, const uint8_t *q4, const float *scale
  * calls read the plan and trust it. T may be 0: nothing is read or written
  * (kxw4_route_rows still clears the offsets). Limits: groups 1..1024, T*k up
  * to 2^30 slots. Row buffers of N rows are written up to offsets[groups];
- * what lies behind stays as it was. Outputs must not overlap inputs unless
- * said (the same pointer for both is refused with -1). Results do not depend on the order in which work-groups run. */
+ * what lies behind stays as it was. Outputs must not overlap inputs or each
+ * other unless said (equal pointers are refused with -1). Results do not
+ * depend on the order in which work-groups run. */
 typedef struct kxw4_route {
     int32_t T, k, groups;
     int32_t *offsets, *order, *position;
@@ -319,7 +320,8 @@ int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, i
  * (block 0) with KXW4_SCALE_FP16 weights of group 64 or 128; block 32 with
  * KXW4_SCALE_FP16_ZP4 of group 32 or 64, or with KXW4_SCALE_W8; else
  * KXW4_ETIER. The arithmetic of a row is kxw4_gemm's under a split count that
- * follows from the sizes alone (T, k, groups, rows, K). a's rows * K < 2^31. */
+ * follows from the sizes alone (T, k, groups, rows, K). a's rows * K < 2^31;
+ * 16-byte aligned pointers (4 for per-token scales). */
 int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count, const kxw4_act_t *a,
                      const kxw4_route_t *route, int sorted_rows, int y_dtype, void *stream);
 

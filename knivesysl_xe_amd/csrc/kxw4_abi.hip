@@ -552,7 +552,7 @@ int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, i
     if (rc) return rc;
     if (!valid_dtype(dy_dtype) || !valid_dtype(rows_dtype)) return KXW4_ESHAPE;
     if (route->T == 0) return KXW4_OK;
-    if (!dy || !rows || !weights || !drows || !dweights || drows == rows || drows == dy) return KXW4_EARG;
+    if (!dy || !rows || !weights || !drows || !dweights || drows == rows || drows == dy || dweights == weights) return KXW4_EARG;
     if (!aligned(dy, elem_bytes(dy_dtype)) || !aligned(rows, elem_bytes(rows_dtype)) ||
         !aligned(drows, elem_bytes(rows_dtype)) || !aligned(weights, 4) || !aligned(dweights, 4))
         return KXW4_EARG;
@@ -596,8 +596,14 @@ int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count,
     if (!strip_takes(ws[0]->group, a->block, ws[0]->scale_enc, rows, ws[0]->K)) return KXW4_ESHAPE;
     if (rows == 0) return KXW4_OK;
     if (!a->q || !a->scale) return KXW4_EPREP;
-    for (int i = 0; i < count; ++i)
-        if (!ys[i]) return KXW4_EARG;
+    // (16-byte pieces, of the block scales too)
+    if (!aligned(a->q, 16) || !aligned(a->scale, a->block ? 16 : 4)) return KXW4_EARG;
+    for (int i = 0; i < count; ++i) {
+        if (!aligned(ws[i]->codes, 16) || !aligned(ws[i]->scales, 16)) return KXW4_EARG;
+        if (!ys[i] || !aligned(ys[i], 16)) return KXW4_EARG;
+        for (int j = 0; j < i; ++j)
+            if (ys[i] == ys[j]) return KXW4_EARG;
+    }
     x.count = count;
     x.q = a->q;
     x.ascale = a->scale;

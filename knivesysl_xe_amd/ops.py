@@ -34,6 +34,7 @@ GPU; nothing here falls back to the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -359,9 +360,12 @@ def gemv(w: W4Weight, a: QuantAct, dtype=torch.float32, residual=None, splits: i
     return y
 
 
+_WEIGHT_PTR = C.POINTER(_lib.Weight)
+
+
 def _weight_array(ws: Sequence[W4Weight]):
     cs = [w.c() for w in ws]
-    arr = (C.POINTER(_lib.Weight) * len(ws))(*[C.pointer(c) for c in cs])
+    arr = (_WEIGHT_PTR * len(ws))(*[C.pointer(c) for c in cs])
     return cs, arr
 
 
@@ -545,12 +549,22 @@ class RowRoute:
 
     @classmethod
     def empty(cls, T: int, k: int, groups: int, device="cuda") -> "RowRoute":
-        def ints(*shape):
-            return torch.empty(*shape, dtype=torch.int32, device=device)
-        return cls(T, k, groups, ints(groups + 1), ints(T * k), ints(T, k))
+        i32 = torch.int32
+        return cls(T, k, groups, torch.empty(groups + 1, dtype=i32, device=device),
+                   torch.empty(T * k, dtype=i32, device=device), torch.empty(T, k, dtype=i32, device=device))
 
 
 def _check_route(r: RowRoute, device) -> RowRoute:
+    # (a plan as it should be passes this test; the checks below only name what is wrong)
+    if r.__class__ is RowRoute:
+        o, q, p, T, k = r.offsets, r.order, r.position, r.T, r.k
+        i32 = torch.int32
+        if (o.__class__ is q.__class__ is p.__class__ is torch.Tensor and T >= 0 and k > 0 and r.groups > 0
+                and o.dtype is i32 and q.dtype is i32 and p.dtype is i32
+                and o.shape == (r.groups + 1,) and q.shape == (T * k,) and p.shape == (T, k)
+                and o.device == device and q.device == device and p.device == device
+                and o.is_contiguous() and q.is_contiguous() and p.is_contiguous()):
+            return r
     if not isinstance(r, RowRoute):
         raise ValueError("route must be a RowRoute")
     if r.T < 0 or r.k < 1 or r.groups < 1:
@@ -561,15 +575,21 @@ def _check_route(r: RowRoute, device) -> RowRoute:
     return r
 
 
+@functools.lru_cache(maxsize=4096)
+def _route_bytes(T: int, k: int, groups: int) -> int:
+    return lib().kxw4_route_workspace(T, k, groups)
+
+
 def route_rows(ids: torch.Tensor, groups: int, out: Optional[RowRoute] = None) -> RowRoute:
     """Sort the slots of ids ([T][k] or [T], int32 or int64) by group, stably.
     An id outside [0, groups) names no group. `out` (same T, k, groups) is
     reused when given."""
     dev = _gpu(ids, "ids")
-    if ids.dim() not in (1, 2) or (ids.dim() == 2 and ids.shape[1] < 1):
-        raise ValueError(f"ids must have shape (T,) or (T, k), got {tuple(ids.shape)}")
-    _need(ids, "ids", _IDS, ids.shape, dev)
-    T, k = ids.shape if ids.dim() == 2 else (ids.shape[0], 1)
+    shape = ids.shape
+    if len(shape) not in (1, 2) or (len(shape) == 2 and shape[1] < 1):
+        raise ValueError(f"ids must have shape (T,) or (T, k), got {tuple(shape)}")
+    _need(ids, "ids", _IDS, shape, dev)
+    T, k = shape if len(shape) == 2 else (shape[0], 1)
     if not 1 <= groups <= 1024:
         raise ValueError(f"groups must be 1 to 1024, got {groups}")
     if out is not None:
@@ -578,10 +598,11 @@ def route_rows(ids: torch.Tensor, groups: int, out: Optional[RowRoute] = None) -
         r = _check_route(out, dev)
     else:
         r = RowRoute.empty(T, k, groups, dev)
-    nbytes = lib().kxw4_route_workspace(T, k, groups)
+    nbytes = _route_bytes(T, k, groups)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     rc = r.c()
-    _launch("kxw4_route_rows", dev, ids.data_ptr(), ids.dtype is torch.int64, C.byref(rc), _ptr(ws))
+    _launch("kxw4_route_rows", dev, ids.data_ptr(), ids.dtype is torch.int64, C.byref(rc),
+            ws.data_ptr() if nbytes else None)
     return r
 
 
@@ -619,8 +640,8 @@ def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Te
     y = _out(route.T, H, dtype or (out.dtype if out is not None else rows.dtype), dev, out)
     if route.T:
         rc = route.c()
-        _launch("kxw4_combine_rows", dev, rows.data_ptr(), _dtype_code(rows.dtype), H, _ptr(weights), C.byref(rc),
-                y.data_ptr(), _dtype_code(y.dtype))
+        _launch("kxw4_combine_rows", dev, rows.data_ptr(), _dtype_code(rows.dtype), H,
+                None if weights is None else weights.data_ptr(), C.byref(rc), y.data_ptr(), _dtype_code(y.dtype))
     return y
 
 
@@ -728,7 +749,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     nbytes = lib().kxw4_adapter_workspace(C.byref(ad), T)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("kxw4_adapter_add", dev, y.data_ptr(), _dtype_code(y.dtype), x.data_ptr(), _dtype_code(x.dtype),
-            C.byref(ad), C.byref(rc), o.data_ptr(), _ptr(ws))
+            C.byref(ad), C.byref(rc), o.data_ptr(), ws.data_ptr() if nbytes else None)
     return o
 
 

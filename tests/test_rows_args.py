@@ -75,6 +75,7 @@ def test_row_calls_refuse_bad_arguments():
     # an output in the place of an input
     assert dispatch(rows=P) == combine(y=P) == backward(drows=P) == _lib.EARG
     assert backward(rows=C.c_void_p(256), drows=C.c_void_p(256)) == _lib.EARG
+    assert backward(drows=C.c_void_p(256), dw=P, w=P) == _lib.EARG
 
 
 def test_expert_gemm_refuses_bad_arguments():
@@ -102,6 +103,10 @@ def test_expert_gemm_refuses_bad_arguments():
     assert call(ws=(W(group=32),)) == call(ws=(W(enc=1),)) == call(a=A(block=32)) == _lib.ETIER
     assert call(ws=(W(group=128, enc=1),), a=A(block=32)) == call(ws=(W(group=16, enc=1),), a=A(block=32)) == _lib.ETIER
     assert call(ws=(W(group=32, enc=2),)) == _lib.ETIER                  # W8 has K32 activation blocks
+    # one output for two weights, buffers off their alignment
+    assert call(ws=(W(), W())) == call(y=72) == _lib.EARG
+    assert call(a=A(q=72)) == call(a=A(scale=66)) == call(ws=(W(codes=72),)) == call(ws=(W(scales=72),)) == _lib.EARG
+    assert call(ws=(W(group=32, enc=1),), a=A(block=32, scale=68)) == _lib.EARG
     assert call(r=R(T=0, offsets=None, order=None, position=None), a=A(T=0, q=None, scale=None), y=None) == 0
 
 
