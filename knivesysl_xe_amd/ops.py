@@ -530,12 +530,13 @@ _FLOATS = (torch.float32, torch.bfloat16)
 _IDS = (torch.int32, torch.int64)
 
 
-@dataclass
+@dataclass(frozen=True)
 class RowRoute:
     """The plan that sorts a batch's slots (token t, choice j, slot t*k + j) by
     the group each names: an expert, or an adapter (k = 1). Made by route_rows
     and shared by every call of a step, its backward pass among them; the calls
-    trust its contents."""
+    trust its contents. The first call checks its buffers, which stay its own
+    (route_rows writes them again when the plan is passed as `out`)."""
     T: int
     k: int
     groups: int
@@ -543,9 +544,14 @@ class RowRoute:
     order: torch.Tensor      # int32 [T*k]: the slot at each place, those without a group last
     position: torch.Tensor   # int32 [T][k]: the place of each slot, -1 without a group
 
+    _made = None             # (device, reference to the C struct) once checked
+
     def c(self) -> _lib.Route:
         return _lib.Route(self.T, self.k, self.groups, self.offsets.data_ptr(), self.order.data_ptr(),
                           self.position.data_ptr())
+
+    def __reduce__(self):    # (a copy is checked anew)
+        return RowRoute, (self.T, self.k, self.groups, self.offsets, self.order, self.position)
 
     @classmethod
     def empty(cls, T: int, k: int, groups: int, device="cuda") -> "RowRoute":
@@ -554,17 +560,22 @@ class RowRoute:
                    torch.empty(T * k, dtype=i32, device=device), torch.empty(T, k, dtype=i32, device=device))
 
 
-def _check_route(r: RowRoute, device) -> RowRoute:
-    # (a plan as it should be passes this test; the checks below only name what is wrong)
+def _plan(r: RowRoute, device):
+    """The C struct of a plan on `device`, by reference."""
     if r.__class__ is RowRoute:
-        o, q, p, T, k = r.offsets, r.order, r.position, r.T, r.k
-        i32 = torch.int32
-        if (o.__class__ is q.__class__ is p.__class__ is torch.Tensor and T >= 0 and k > 0 and r.groups > 0
-                and o.dtype is i32 and q.dtype is i32 and p.dtype is i32
-                and o.shape == (r.groups + 1,) and q.shape == (T * k,) and p.shape == (T, k)
-                and o.device == device and q.device == device and p.device == device
-                and o.is_contiguous() and q.is_contiguous() and p.is_contiguous()):
-            return r
+        made = r._made
+        if made is not None and made[0] == device:
+            return made[1]
+    return _make_plan(_check_route(r, device), device)
+
+
+def _make_plan(r: RowRoute, device):
+    ref = C.byref(r.c())
+    r.__dict__["_made"] = (device, ref)
+    return ref
+
+
+def _check_route(r: RowRoute, device) -> RowRoute:
     if not isinstance(r, RowRoute):
         raise ValueError("route must be a RowRoute")
     if r.T < 0 or r.k < 1 or r.groups < 1:
@@ -588,20 +599,21 @@ def route_rows(ids: torch.Tensor, groups: int, out: Optional[RowRoute] = None) -
     shape = ids.shape
     if len(shape) not in (1, 2) or (len(shape) == 2 and shape[1] < 1):
         raise ValueError(f"ids must have shape (T,) or (T, k), got {tuple(shape)}")
-    _need(ids, "ids", _IDS, shape, dev)
+    if ids.dtype not in _IDS or not ids.is_contiguous():
+        _need(ids, "ids", _IDS, shape, dev)
     T, k = shape if len(shape) == 2 else (shape[0], 1)
     if not 1 <= groups <= 1024:
         raise ValueError(f"groups must be 1 to 1024, got {groups}")
     if out is not None:
         if (out.T, out.k, out.groups) != (T, k, groups):
             raise ValueError("out does not match the ids' shape / groups")
-        r = _check_route(out, dev)
+        r, ref = out, _plan(out, dev)
     else:
         r = RowRoute.empty(T, k, groups, dev)
+        ref = _make_plan(r, dev)
     nbytes = _route_bytes(T, k, groups)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    rc = r.c()
-    _launch("kxw4_route_rows", dev, ids.data_ptr(), ids.dtype is torch.int64, C.byref(rc),
+    _launch("kxw4_route_rows", dev, ids.data_ptr(), ids.dtype is torch.int64, ref,
             ws.data_ptr() if nbytes else None)
     return r
 
@@ -611,7 +623,7 @@ def dispatch_rows(x: torch.Tensor, route: RowRoute, out=None) -> torch.Tensor:
     which the first offsets[groups] are written. For expert_gemm no such copy
     is needed: it reads the tokens' rows where they are."""
     dev = _gpu(x, "x")
-    _check_route(route, dev)
+    plan = _plan(route, dev)
     if x.dim() != 2:
         raise ValueError("x must have shape (T, H)")
     T, H = x.shape
@@ -619,8 +631,7 @@ def dispatch_rows(x: torch.Tensor, route: RowRoute, out=None) -> torch.Tensor:
     N = route.T * route.k
     rows = _need(out, "out", x.dtype, (N, H), dev) if out is not None else torch.empty(N, H, dtype=x.dtype, device=dev)
     if N:
-        rc = route.c()
-        _launch("kxw4_dispatch_rows", dev, x.data_ptr(), _dtype_code(x.dtype), H, C.byref(rc), rows.data_ptr())
+        _launch("kxw4_dispatch_rows", dev, x.data_ptr(), _dtype_code(x.dtype), H, plan, rows.data_ptr())
     return rows
 
 
@@ -630,7 +641,7 @@ def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Te
     / bf16), summed in FP32; weights [T][k] f32, all 1 when None. y [T][H] is
     of `dtype` (the rows' by default)."""
     dev = _gpu(rows, "rows")
-    _check_route(route, dev)
+    plan = _plan(route, dev)
     if rows.dim() != 2:
         raise ValueError("rows must have shape (T*k, H)")
     H = rows.shape[1]
@@ -639,9 +650,8 @@ def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Te
         _need(weights, "weights", torch.float32, (route.T, route.k), dev)
     y = _out(route.T, H, dtype or (out.dtype if out is not None else rows.dtype), dev, out)
     if route.T:
-        rc = route.c()
         _launch("kxw4_combine_rows", dev, rows.data_ptr(), _dtype_code(rows.dtype), H,
-                None if weights is None else weights.data_ptr(), C.byref(rc), y.data_ptr(), _dtype_code(y.dtype))
+                None if weights is None else weights.data_ptr(), plan, y.data_ptr(), _dtype_code(y.dtype))
     return y
 
 
@@ -650,7 +660,7 @@ def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, route: RowRoute,
     to offsets[groups], written to `out` when given; of weights [T][k], f32, 0
     for a slot without a group)."""
     dev = _gpu(rows, "rows")
-    _check_route(route, dev)
+    plan = _plan(route, dev)
     if rows.dim() != 2:
         raise ValueError("rows must have shape (T*k, H)")
     N, H = route.T * route.k, rows.shape[1]
@@ -660,9 +670,8 @@ def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, route: RowRoute,
     drows = _need(out, "out", rows.dtype, (N, H), dev) if out is not None else torch.empty_like(rows)
     dweights = torch.empty(route.T, route.k, dtype=torch.float32, device=dev)
     if N:
-        rc = route.c()
         _launch("kxw4_combine_rows_backward", dev, dy.data_ptr(), _dtype_code(dy.dtype), rows.data_ptr(),
-                _dtype_code(rows.dtype), H, weights.data_ptr(), C.byref(rc), drows.data_ptr(), dweights.data_ptr())
+                _dtype_code(rows.dtype), H, weights.data_ptr(), plan, drows.data_ptr(), dweights.data_ptr())
     return drows, dweights
 
 
@@ -684,7 +693,7 @@ def expert_gemm_fanout(ws: Sequence[W4Weight], a: QuantAct, route: RowRoute, dty
     dev = ws[0].codes.device
     for w in ws:
         _check_weight(w, dev)
-    _check_route(route, dev)
+    plan = _plan(route, dev)
     for w in ws:
         if w.M % route.groups:
             raise ValueError(f"weight rows {w.M} are not a multiple of {route.groups} groups")
@@ -698,9 +707,8 @@ def expert_gemm_fanout(ws: Sequence[W4Weight], a: QuantAct, route: RowRoute, dty
           for i, w in enumerate(ws)]
     keep, warr = _weight_array(ws)
     yarr = (C.c_void_p * len(ws))(*[y.data_ptr() for y in ys])
-    ac, rc = a.c(), route.c()
-    _launch("kxw4_expert_gemm", dev, warr, yarr, len(ws), C.byref(ac), C.byref(rc), bool(sorted_rows),
-            _dtype_code(dtype))
+    ac = a.c()
+    _launch("kxw4_expert_gemm", dev, warr, yarr, len(ws), C.byref(ac), plan, bool(sorted_rows), _dtype_code(dtype))
     return ys
 
 
@@ -731,25 +739,27 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     input (f32 / bf16 each), route of one adapter id per token. `out` may be y
     itself; else it must not overlap it."""
     dev = _gpu(y, "y")
-    if adapters.a.dim() != 3 or adapters.b.dim() != 3:
+    plan = _plan(route, dev)
+    a, b, scale = adapters.a, adapters.b, adapters.scale
+    sa, sb = a.shape, b.shape
+    if len(sa) != 3 or len(sb) != 3:
         raise ValueError("adapters must have shapes (n, r, K) and (n, M, r)")
-    n, r, K = adapters.a.shape
-    M = adapters.b.shape[1]
-    _check_route(route, dev)
+    n, r, K = sa
+    M = sb[1]
     if route.groups != n or route.k != 1:
         raise ValueError(f"the plan has {route.groups} groups and k {route.k} for {n} adapters")
     T = route.T
     _need(y, "y", _FLOATS, (T, M), dev)
     _need(x, "x", _FLOATS, (T, K), dev)
-    _need(adapters.a, "adapters.a", torch.bfloat16, (n, r, K), dev)
-    _need(adapters.b, "adapters.b", torch.bfloat16, (n, M, r), dev)
-    _need(adapters.scale, "adapters.scale", torch.float32, (n,), dev)
+    _need(a, "adapters.a", torch.bfloat16, sa, dev)
+    _need(b, "adapters.b", torch.bfloat16, (n, M, r), dev)
+    _need(scale, "adapters.scale", torch.float32, (n,), dev)
     o = _need(out, "out", y.dtype, (T, M), dev) if out is not None else torch.empty_like(y)
-    ad, rc = adapters.c(), route.c()
-    nbytes = lib().kxw4_adapter_workspace(C.byref(ad), T)
+    ref = C.byref(adapters.c())
+    nbytes = lib().kxw4_adapter_workspace(ref, T)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("kxw4_adapter_add", dev, y.data_ptr(), _dtype_code(y.dtype), x.data_ptr(), _dtype_code(x.dtype),
-            C.byref(ad), C.byref(rc), o.data_ptr(), ws.data_ptr() if nbytes else None)
+            ref, plan, o.data_ptr(), ws.data_ptr() if nbytes else None)
     return o
 
 

@@ -177,3 +177,24 @@ def test_route_buffers_are_checked():
     flat = ops.RowRoute(4, 2, 8, r.offsets, r.order, r.position.view(-1))
     with pytest.raises(ValueError, match="route position must have shape"):
         ops._check_route(flat, torch.device("cpu"))
+
+
+def test_a_plan_is_checked_once_and_copied_whole():
+    import copy
+    import dataclasses
+    import pickle
+    cpu = torch.device("cpu")
+    r = ops.RowRoute.empty(4, 2, 8, "cpu")
+    ref = ops._plan(r, cpu)
+    assert ops._plan(r, cpu) is ref
+    with pytest.raises(ValueError, match="must be on"):
+        ops._plan(r, torch.device("meta"))
+    for name in ("T", "offsets"):
+        with pytest.raises(dataclasses.FrozenInstanceError):
+            setattr(r, name, getattr(r, name))
+    for other in (copy.deepcopy(r), pickle.loads(pickle.dumps(r)), dataclasses.replace(r, order=r.order.clone())):
+        assert ops._plan(other, cpu) is not ref
+        c = ops._plan(other, cpu)._obj
+        assert (c.T, c.k, c.groups, c.order) == (4, 2, 8, other.order.data_ptr()) and c.order != ref._obj.order
+    with pytest.raises(ValueError, match="route order must have shape"):
+        ops._plan(dataclasses.replace(r, order=r.order[:3]), cpu)
