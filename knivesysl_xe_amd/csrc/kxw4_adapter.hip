@@ -258,10 +258,14 @@ __device__ __forceinline__ void store_up(const AdapterArgs &a, size_t at, Col co
     }
 }
 
-// KC: 32-column chunks of B requested together.
+// KC: 32-column chunks of B requested together; from two on a row of B is long
+// enough for the loads of to_operand (1,500 tokens of 8, K = 5120, M = 8192, r =
+// 128 56.5 / 49.5 us, r = 64 35.9 / 32.3; r = 32 stays at 24, 250 tokens 9.2 /
+// 9.5).
 template <int KC, bool YB>
 __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const AdapterArgs a) {
     constexpr int NY = YB ? 2 : 4;                           // 16-byte pieces of a lane's 16 outputs
+    constexpr bool SPREAD = KC > 1;
     extern __shared__ __attribute__((aligned(16))) uint16_t cut[];       // [3][16][pitch]
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -326,14 +330,17 @@ __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const Adapter
             for (int h = 0; h < KC; ++h)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int k = k0 + 32 * h + 8 * g;
-                    const v4u w = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(row(c, n), a.M - 1)) * a.r + min(k, a.r - 8));
+                    const int k = k0 + 32 * h + 8 * (SPREAD ? lane & 3 : g);
+                    const v4u w = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(row(c, SPREAD ? lane >> 2 : n), a.M - 1)) * a.r + min(k, a.r - 8));
 #pragma unroll
                     for (int x = 0; x < 4; ++x) b[h][c][x] = k < a.r ? w[x] : 0u;
                 }
 #pragma unroll
             for (int h = 0; h < KC; ++h) {
                 if (k0 + 32 * h >= a.r) break;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if constexpr (SPREAD) b[h][c] = to_operand(b[h][c], lane);
 #pragma unroll
                 for (int q = 2; q >= 0; --q) {
                     const v4u x = *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * pitch + k0 + 32 * h + 8 * g);
