@@ -303,3 +303,18 @@ def test_calls_at_once_on_two_streams():
         for r, rows, y in got[i]:
             assert torch.equal(r.order, got[i][0][0].order) and torch.equal(rows, got[i][0][1])
             assert torch.equal(y, got[i][0][2])
+
+
+def test_every_float32_pattern_rounds_to_the_nearest_bfloat16():
+    # random bit patterns (subnormals, ties, infinities and NaNs among them);
+    # one choice without weights: y = 1 * x + 0
+    rng = np.random.default_rng(12)
+    bits = rng.integers(0, 1 << 32, (4096, 512), dtype=np.uint64).astype(np.uint32)
+    bits[0] = np.arange(512, dtype=np.uint32) << 7           # subnormals
+    bits[1] |= 0x7F000000                                    # large ones, infinities, NaNs
+    bits[2] = (bits[2] & 0xFFFF0000) | 0x8000                # ties
+    x = torch.from_numpy(bits.view(np.float32)).to(DEV)
+    r = ops.route_rows(torch.arange(4096, device=DEV) % 7, 7)
+    y = ops.combine_rows(ops.dispatch_rows(x, r), r, dtype=torch.bfloat16)
+    want = x.bfloat16()
+    assert ((y == want) | (torch.isnan(y) & torch.isnan(want))).all()
