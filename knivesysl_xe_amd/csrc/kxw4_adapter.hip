@@ -86,62 +86,79 @@ constexpr int kLowTile = 16, kFewWaves = 4;
 __host__ __device__ constexpr int chunks_of(int r) { return (r + 31) / 32; }
 constexpr int kCutChunk = 3 * 64 * 8;
 
-// acc[c] = the 32-K steps [k0, k1) of A_e's columns 16 c .. + 15 times x. Each
-// lane loads 16-byte pieces of the row of `token` (place lane / 4 of the tile) and
-// of A's rows; a step's x piece is used by every column tile, an A piece once.
-template <int CT, bool XB>
-__device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, int token, int k0, int k1, int lane, v4f (&acc)[CT]) {
+// acc[t][c] = the 32-K steps [k0, k1) of A_e's columns 16 c .. + 15 times the x
+// of token tile t. Each lane loads 16-byte pieces of the row of `token[t]` (place
+// lane / 4 of the tile) and of A's rows; an x piece is used by every column tile,
+// an A piece by every token tile.
+template <int CT, bool XB, int TT>
+__device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int (&token)[TT], int k0, int k1, int lane, v4f (&acc)[TT][CT]) {
     const int lr = lane >> 2, lk = 8 * (lane & 3);           // row and columns that this lane loads
-    const size_t xrow = (size_t)token * a.K + lk;
+    size_t xrow[TT];
     const uint16_t *arow[CT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) xrow[t] = (size_t)token[t] * a.K + lk;
 #pragma unroll
     for (int c = 0; c < CT; ++c)
         arow[c] = a.a + ((size_t)e * a.r + min(c * 16 + lr, a.r - 1)) * a.K + lk;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[t][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     // U steps' loads are requested before the first of them is used
     auto run = [&](int k, auto uc) {
         constexpr int U = decltype(uc)::value;
         v4u w[U][CT];
         if constexpr (XB) {
-            v4u x[U];
+            v4u x[U][TT];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                x[u] = *reinterpret_cast<const v4u *>(static_cast<const uint16_t *>(a.x) + xrow + 32 * (k + u));
 #pragma unroll
-                for (int c = 0; c < CT; ++c) w[u][c] = *reinterpret_cast<const v4u *>(arow[c] + 32 * (k + u));
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    if (c == 0) x[u] = to_operand(x[u], lane);
-                    acc[c] = mfma_bf16(x[u], to_operand(w[u][c], lane), acc[c]);
-                }
-        } else {
-            float v[U][8];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                load8(static_cast<const float *>(a.x) + xrow + 32 * (k + u), v[u]);
+                for (int t = 0; t < TT; ++t)
+                    x[u][t] = *reinterpret_cast<const v4u *>(static_cast<const uint16_t *>(a.x) + xrow[t] + 32 * (k + u));
 #pragma unroll
                 for (int c = 0; c < CT; ++c) w[u][c] = *reinterpret_cast<const v4u *>(arow[c] + 32 * (k + u));
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                v4u x[3];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] = __uint_as_float(to_operand(__float_as_uint(v[u][i]), lane));
-                split8(v[u], x);
+                for (int t = 0; t < TT; ++t) x[u][t] = to_operand(x[u][t], lane);
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     const v4u b = to_operand(w[u][c], lane);
 #pragma unroll
-                    for (int q = 2; q >= 0; --q) acc[c] = mfma_bf16(x[q], b, acc[c]);
+                    for (int t = 0; t < TT; ++t) acc[t][c] = mfma_bf16(x[u][t], b, acc[t][c]);
+                }
+            }
+        } else {
+            float v[U][TT][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) load8(static_cast<const float *>(a.x) + xrow[t] + 32 * (k + u), v[u][t]);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) w[u][c] = *reinterpret_cast<const v4u *>(arow[c] + 32 * (k + u));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                v4u x[TT][3];
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[u][t][i] = __uint_as_float(to_operand(__float_as_uint(v[u][t][i]), lane));
+                    split8(v[u][t], x[t]);
+                }
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const v4u b = to_operand(w[u][c], lane);
+#pragma unroll
+                    for (int t = 0; t < TT; ++t)
+#pragma unroll
+                        for (int q = 2; q >= 0; --q) acc[t][c] = mfma_bf16(x[t][q], b, acc[t][c]);
                 }
             }
         }
     };
-    constexpr int kSteps = CT <= 2 ? 4 : CT <= 4 ? 2 : 1;
+    constexpr int kSteps = CT * TT <= 2 ? 4 : CT <= 4 ? 2 : 1;
     int k = k0;
     for (; k + kSteps <= k1; k += kSteps) run(k, std::integral_constant<int, kSteps>{});
     if constexpr (kSteps > 2) {
@@ -155,72 +172,83 @@ __device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, int token
 
 // low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
 // work-group takes 16 places of one adapter and part s, its WAVES waves
-// consecutive runs of 32-K steps, all r columns (CT tiles of 16). CUT: one part; scale * low is cut into its three BF16 parts here,
-// in the order the second launch's operand takes them.
-template <int CT, int WAVES, bool XB, bool CUT>
+// consecutive runs of 32-K steps, all r columns (CT tiles of 16). CUT: one part
+// of 16 TT places; scale * low is cut into its three BF16 parts here, in the
+// order the second launch's operand takes them. The places [p, p + 16) of adapter
+// e are cut tile p / 16 + e, a number of its own for each tile.
+template <int CT, int WAVES, bool XB, bool CUT, int TT>
 __global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
+    static_assert(CUT || TT == 1, "parts of one tile");
     __shared__ float part[WAVES - 1][CT][256];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
+    const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile * TT, lane);
     if ((int)blockIdx.x >= tiles.total) return;
-    const GroupTile tile = tile_at(tiles, a.offsets, kLowTile, blockIdx.x);
-    const int p0 = tile.begin + tile.index * kLowTile;
+    const GroupTile tile = tile_at(tiles, a.offsets, kLowTile * TT, blockIdx.x);
+    const int p0 = tile.begin + tile.index * kLowTile * TT;
     const int steps = a.K / 32, ways = a.splits * WAVES, way = blockIdx.y * WAVES + wave;
     const int k0 = (int)((long long)steps * way / ways), k1 = (int)((long long)steps * (way + 1) / ways);
 
-    v4f acc[CT];
-    low_steps<CT, XB>(a, tile.e, a.order[min(p0 + (lane >> 2), tile.end - 1)], k0, k1, lane, acc);
-    if (wave > 0) {
+    v4f acc[TT][CT];
+    int token[TT];
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+    for (int t = 0; t < TT; ++t) token[t] = a.order[min(p0 + kLowTile * t + (lane >> 2), tile.end - 1)];
+    low_steps<CT, XB, TT>(a, tile.e, token, k0, k1, lane, acc);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave - 1][c][i * 64 + lane] = acc[c][i];
-    }
-    __syncthreads();
-    if constexpr (CUT) {
-        // every thread adds up and cuts elements of the tile: lane l of
-        // chunk h holds token l%16 and columns 32 h + 8 (l/16) .. + 7
-        const float scale = a.scale[tile.e];
-        if (wave == 0) {
+    for (int t = 0; t < TT; ++t) {
+        const int pt = p0 + kLowTile * t;
+        if (pt >= tile.end) return;
+        if (t > 0) __syncthreads();
+        if (wave > 0) {
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = acc[c][i];
-#pragma unroll
-                    for (int w = 0; w < WAVES - 1; ++w) v += part[w][c][i * 64 + lane];
-                    part[0][c][i * 64 + lane] = c * 16 + m < a.r ? v * scale : 0.0f;
-                }
+                for (int i = 0; i < 4; ++i) part[wave - 1][c][i * 64 + lane] = acc[t][c][i];
         }
         __syncthreads();
-        uint16_t *to = reinterpret_cast<uint16_t *>(a.low) + (size_t)blockIdx.x * chunks_of(a.r) * kCutChunk;
-        for (int h = wave; h < chunks_of(a.r); h += WAVES) {
-            float v[8];
-            v4u op[3];
+        if constexpr (CUT) {
+            // every thread adds up and cuts elements of the tile: lane l of
+            // chunk h holds token l%16 and columns 32 h + 8 (l/16) .. + 7
+            const float scale = a.scale[tile.e];
+            if (wave == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // column 32 h + 8 g + j of token m: tile c, register i = m % 4 of lane group m / 4
-                const int column = 32 * h + 8 * g + j;
-                v[j] = column < 16 * CT ? part[0][min(column >> 4, CT - 1)][(m & 3) * 64 + 16 * (m >> 2) + (column & 15)] : 0.0f;
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v = acc[t][c][i];
+#pragma unroll
+                        for (int w = 0; w < WAVES - 1; ++w) v += part[w][c][i * 64 + lane];
+                        part[0][c][i * 64 + lane] = c * 16 + m < a.r ? v * scale : 0.0f;
+                    }
             }
-            split8(v, op);
+            __syncthreads();
+            uint16_t *to = reinterpret_cast<uint16_t *>(a.low) + (size_t)(pt / kLowTile + tile.e) * chunks_of(a.r) * kCutChunk;
+            for (int h = wave; h < chunks_of(a.r); h += WAVES) {
+                float v[8];
+                v4u op[3];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<v4u *>(to + (h * 3 + q) * 512 + lane * 8) = op[q];
-        }
-        return;
-    }
-    if (wave > 0) return;
+                for (int j = 0; j < 8; ++j) {
+                    // column 32 h + 8 g + j of token m: tile c, register i = m % 4 of lane group m / 4
+                    const int column = 32 * h + 8 * g + j;
+                    v[j] = column < 16 * CT ? part[0][min(column >> 4, CT - 1)][(m & 3) * 64 + 16 * (m >> 2) + (column & 15)] : 0.0f;
+                }
+                split8(v, op);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        const int col = c * 16 + m;
+                for (int q = 0; q < 3; ++q) *reinterpret_cast<v4u *>(to + (h * 3 + q) * 512 + lane * 8) = op[q];
+            }
+        } else if (wave == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v = acc[c][i];
+            for (int c = 0; c < CT; ++c) {
+                const int col = c * 16 + m;
 #pragma unroll
-            for (int w = 0; w < WAVES - 1; ++w) v += part[w][c][i * 64 + lane];
-            const int p = p0 + 4 * g + i;
-            if (p < tile.end && col < a.r) a.low[((size_t)blockIdx.y * a.T + p) * a.r + col] = v;
+                for (int i = 0; i < 4; ++i) {
+                    float v = acc[t][c][i];
+#pragma unroll
+                    for (int w = 0; w < WAVES - 1; ++w) v += part[w][c][i * 64 + lane];
+                    const int p = pt + 4 * g + i;
+                    if (p < tile.end && col < a.r) a.low[((size_t)blockIdx.y * a.T + p) * a.r + col] = v;
+                }
+            }
         }
     }
 }
@@ -383,7 +411,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(const Adapt
         if (a.out == a.y || p0 >= p1) return;
     }
     const bool on = m0 < a.M;                                // (the others only help with `low`)
-    const int row = a.order[min(p0 + (lane >> 2), p1 - 1)];
+    const int row[1] = {a.order[min(p0 + (lane >> 2), p1 - 1)]};
     const size_t at = (size_t)a.order[min(p0 + n, p1 - 1)] * a.M;
     // (columns and rows as in adapter_up_kernel)
     auto col = [&](int q) { return m0 + (YB ? 32 * q + 8 * g : 16 * q + 4 * g); };
@@ -400,12 +428,12 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(const Adapt
         for (int c = 0; c < 4; ++c)
             b[c] = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(brow(c), a.M - 1)) * a.r + min(8 * g, a.r - 8));
         const int steps = a.K / 32;
-        v4f low[CT];
-        low_steps<CT, XB>(a, e, row, steps * wave / kOneWaves, steps * (wave + 1) / kOneWaves, lane, low);
+        v4f low[1][CT];
+        low_steps<CT, XB, 1>(a, e, row, steps * wave / kOneWaves, steps * (wave + 1) / kOneWaves, lane, low);
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave][c][i * 64 + lane] = low[c][i];
+            for (int i = 0; i < 4; ++i) part[wave][c][i * 64 + lane] = low[0][c][i];
         __syncthreads();
         // element i of tile c: token 4 (i%64 / 16) + i / 64, column 16 c + i % 16
         if (tid < 512) {
@@ -455,7 +483,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const Ada
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int mblocks = (a.M + kManyBlock - 1) / kManyBlock;
     const int u = blockIdx.x / mblocks, m0 = (blockIdx.x - u * mblocks) * kManyBlock + wave * kManyRows;
-    // a run: a.run tiles of one adapter; `first`: its first tile's number among all
+    // a run: a.run tiles of one adapter; `first`: the cut tile of its first
     const GroupTiles runs = scan_tiles(a.offsets, a.n, kLowTile * a.run, lane);
     int p0, p1, e = -1;
     size_t first = 0;
@@ -464,13 +492,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const Ada
         e = run.e;
         p0 = run.begin + run.index * kLowTile * a.run;
         p1 = min(run.end, p0 + kLowTile * a.run);
-        const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
-        // the adapter's first tile: the lane whose run of groups holds e, and
-        // the groups before it there
-        const int per = (a.n + 63) / 64, l = e / per;
-        int before = __builtin_amdgcn_readlane(tiles.tiles_before, l);
-        for (int i = l * per; i < e; ++i) before += (a.offsets[i + 1] - a.offsets[i] + kLowTile - 1) / kLowTile;
-        first = before + run.index * a.run;
+        first = p0 / kLowTile + e;
     } else {
         // the tokens without an adapter keep y (already there when out is y)
         p0 = a.offsets[a.n] + (u - runs.total) * kLowTile * a.run;
@@ -613,11 +635,25 @@ static int launch_one(const AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-template <int CT, int WAVES, bool CUT>
+template <int CT, int WAVES, bool CUT, int TT>
 static void launch_low(const AdapterArgs &a, bool x_bf16, hipStream_t st) {
-    const dim3 grid((unsigned)tiles_at_most(a.T, a.n, kLowTile), a.splits);
-    if (x_bf16) hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, true, CUT>), grid, dim3(64 * WAVES), 0, st, a);
-    else hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, false, CUT>), grid, dim3(64 * WAVES), 0, st, a);
+    const dim3 grid((unsigned)tiles_at_most(a.T, a.n, kLowTile * TT), a.splits);
+    if (x_bf16) hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, true, CUT, TT>), grid, dim3(64 * WAVES), 0, st, a);
+    else hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, false, CUT, TT>), grid, dim3(64 * WAVES), 0, st, a);
+}
+
+// The first launch for many tokens. One work-group of either takes about as long
+// as it has bytes to fetch through its CU's L1 (24 a clock): x of its tokens and
+// all of A, so two tiles, which share A, pay once there are more tiles than CUs
+// (us in all for one / two: 8,000 tokens of 12, K = 5120, M = 4096, r = 32 53.5 /
+// 48.8, r = 128 117 / 99, K = 12288, M = 1024, r = 64 71 / 58; 3,965 of 6, K =
+// 5120, r = 32 32 / 36).
+template <int TT>
+static void launch_cut(const AdapterArgs &a, bool x_bf16, hipStream_t st) {
+    if (a.r <= 16) launch_low<1, 16, true, TT>(a, x_bf16, st);
+    else if (a.r <= 32) launch_low<2, 16, true, TT>(a, x_bf16, st);
+    else if (a.r <= 64) launch_low<4, 8, true, TT>(a, x_bf16, st);
+    else launch_low<8, 8, true, TT>(a, x_bf16, st);
 }
 
 template <int KC>
@@ -648,19 +684,17 @@ static int launch_many(AdapterArgs &a, bool y_bf16, hipStream_t st) {
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
     if (many_tokens(a.n, a.T, a.r)) {
         a.splits = 1;
-        if (a.r <= 16) launch_low<1, 16, true>(a, x_bf16, st);
-        else if (a.r <= 32) launch_low<2, 16, true>(a, x_bf16, st);
-        else if (a.r <= 64) launch_low<4, 8, true>(a, x_bf16, st);
-        else launch_low<8, 8, true>(a, x_bf16, st);
+        if (tiles_at_most(a.T, a.n, kLowTile) <= device_cus()) launch_cut<1>(a, x_bf16, st);
+        else launch_cut<2>(a, x_bf16, st);
         return a.r <= 32 ? launch_many<1>(a, y_bf16, st) : a.r <= 64 ? launch_many<2>(a, y_bf16, st) : launch_many<4>(a, y_bf16, st);
     }
     if (one_launch(a.n, a.T, a.r, a.K, a.M)) return a.r <= 16 ? launch_one<1>(a, x_bf16, y_bf16, st) : launch_one<2>(a, x_bf16, y_bf16, st);
     a.splits = adapter_splits(a.n, a.T, a.K);
-    if (a.r <= 16) launch_low<1, kFewWaves, false>(a, x_bf16, st);
-    else if (a.r <= 32) launch_low<2, kFewWaves, false>(a, x_bf16, st);
-    else if (a.r <= 64) launch_low<4, kFewWaves, false>(a, x_bf16, st);
-    else if (a.r <= 128) launch_low<8, kFewWaves, false>(a, x_bf16, st);
-    else launch_low<16, kFewWaves, false>(a, x_bf16, st);
+    if (a.r <= 16) launch_low<1, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 32) launch_low<2, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 64) launch_low<4, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 128) launch_low<8, kFewWaves, false, 1>(a, x_bf16, st);
+    else launch_low<16, kFewWaves, false, 1>(a, x_bf16, st);
     return a.r <= 32 ? launch_up<1>(a, y_bf16, st) : launch_up<2>(a, y_bf16, st);
 }
 

@@ -86,6 +86,18 @@ def test_against_float64(T, n, r, K, M, x_t, y_t):
     assert torch.equal(y, got)
 
 
+# more 16-token tiles than CUs
+@pytest.mark.parametrize("T,n,r,K,M", [(4200, 3, 16, 128, 64), (4300, 60, 24, 384, 48), (5003, 40, 64, 256, 80), (4500, 1, 128, 640, 16)])
+@pytest.mark.parametrize("x_t", [torch.float32, torch.bfloat16])
+def test_many_tiles(T, n, r, K, M, x_t):
+    rng = np.random.default_rng(T)
+    ad = make(rng, n, r, K, M)
+    for ids in (pick(rng, T, n), np.sort(pick(rng, T, n))[::-1], np.full(T, n - 1)):
+        ids = np.ascontiguousarray(ids).astype(np.int32)
+        x, y = normal(rng, T, K, dtype=x_t).to(DEV), normal(rng, T, M).to(DEV)
+        check(ops.adapter_add(y, x, ad, ops.route_rows(torch.from_numpy(ids).to(DEV), n)), y, x, ad, ids)
+
+
 @pytest.mark.parametrize("T", [3, 90, 700])
 def test_one_adapter_for_all_none_for_all_and_packed_prompts(T):
     rng = np.random.default_rng(T)
