@@ -592,11 +592,14 @@ __global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const Ada
     }
 }
 
-// Many tokens, from about 1,500 and 64 an adapter on, while B's rows fit the
-// registers (us few / many: 3,965 tokens of 6 adapters, K = 5120, M = 17408, r =
-// 32 105 / 77, r = 128 226 / 152; 2,048 of 64, M = 5120, r = 16 27 / 29; 1,000 of
-// 4, M = 17408, float32 45.5 / 46.4; 500 of 8, r = 32 13.4 / 21.5).
-static bool many_tokens(int n, int T, int r) { return T >= 1536 && T >= 64ll * n && r <= 128; }
+// Many tokens, while B's rows fit the registers: from 20 million outputs on, where
+// what the first launch loses (no split of K) is less than what the second gains.
+// Swept over 144 shapes of 1,100-6,000 tokens, 2-24 adapters, r 16-128, K 512-
+// 12,288, M 1,024-17,408: 0.5 % behind the better of the two on average (us few /
+// many: 3,965 tokens of 6, K = 5120, M = 17408, r = 32 101 / 74, r = 128 196 / 144;
+// M = 4096, r = 32 32.3 / 32.2; 1,536 of 8, K = 512, M = 16384, r = 64 40.0 / 36.5;
+// K = 12288, M = 1024 26.3 / 35.0; 2,048 of 8, K = 5120, M = 4096 29.6 / 34.7).
+static bool many_tokens(int n, int T, int r, int M) { return (long long)T * M >= 20000000 && T >= 1024 && T >= 64ll * n && r <= 128; }
 
 // Work-groups per 16-token tile of the first launch for few tokens: enough to
 // give each CU four while a wave keeps at least four 32-K steps, and as many
@@ -621,7 +624,7 @@ static bool one_launch(int n, int T, int r, int K, int M) {
 }
 
 size_t adapter_scratch(int n, int T, int r, int K, int M) {
-    if (many_tokens(n, T, r)) return (size_t)tiles_at_most(T, n, kLowTile) * chunks_of(r) * kCutChunk * 2;
+    if (many_tokens(n, T, r, M)) return (size_t)tiles_at_most(T, n, kLowTile) * chunks_of(r) * kCutChunk * 2;
     return one_launch(n, T, r, K, M) ? 0 : (size_t)adapter_splits(n, T, K) * T * r * sizeof(float);
 }
 
@@ -682,7 +685,7 @@ static int launch_many(AdapterArgs &a, bool y_bf16, hipStream_t st) {
 }
 
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
-    if (many_tokens(a.n, a.T, a.r)) {
+    if (many_tokens(a.n, a.T, a.r, a.M)) {
         a.splits = 1;
         if (tiles_at_most(a.T, a.n, kLowTile) <= device_cus()) launch_cut<1>(a, x_bf16, st);
         else launch_cut<2>(a, x_bf16, st);

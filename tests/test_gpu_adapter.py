@@ -66,7 +66,7 @@ def check(got, y, x, ad, ids):
     (1, 1, 8, 128, 16), (1, 5, 16, 1024, 64), (8, 8, 16, 5120, 5120), (13, 3, 24, 384, 80), (16, 1, 32, 256, 256),
     (17, 1, 32, 256, 272), (61, 24, 64, 2048, 512), (64, 64, 16, 640, 112), (65, 2, 8, 128, 1040), (100, 3, 128, 512, 144),
     (129, 200, 40, 256, 48), (300, 4, 256, 384, 96), (1000, 6, 16, 256, 1008), (70, 1024, 8, 128, 32), (5, 2, 200, 17408, 64),
-    # many tokens: B's rows in registers, r <= 128, and not
+    # many tokens, of few outputs
     (1536, 24, 16, 128, 1040), (1537, 1, 8, 256, 16), (2100, 6, 40, 256, 528), (1601, 3, 128, 384, 80), (3000, 2, 72, 128, 144),
     (1600, 3, 136, 128, 48), (1600, 30, 32, 128, 48)])
 @pytest.mark.parametrize("x_t", [torch.float32, torch.bfloat16])
@@ -86,16 +86,31 @@ def test_against_float64(T, n, r, K, M, x_t, y_t):
     assert torch.equal(y, got)
 
 
-# more 16-token tiles than CUs
-@pytest.mark.parametrize("T,n,r,K,M", [(4200, 3, 16, 128, 64), (4300, 60, 24, 384, 48), (5003, 40, 64, 256, 80), (4500, 1, 128, 640, 16)])
-@pytest.mark.parametrize("x_t", [torch.float32, torch.bfloat16])
-def test_many_tiles(T, n, r, K, M, x_t):
+# 20 million outputs: B's rows in registers, one token tile for each CU and more
+@pytest.mark.parametrize("T,n,r,K,M", [
+    (1024, 16, 16, 128, 19536), (1025, 1, 8, 256, 19520), (1600, 24, 24, 128, 12512), (2100, 6, 40, 256, 9536),
+    (1601, 3, 128, 384, 12512), (3000, 2, 72, 128, 6672), (4200, 3, 16, 128, 4768), (4300, 60, 24, 384, 4656),
+    (5003, 40, 64, 256, 4000), (4500, 1, 128, 640, 4448)])
+@pytest.mark.parametrize("x_t,y_t", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                     (torch.bfloat16, torch.bfloat16)])
+def test_many_outputs(T, n, r, K, M, x_t, y_t):
+    # (the first, the last and every 29th column against float64)
     rng = np.random.default_rng(T)
-    ad = make(rng, n, r, K, M)
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(T)
+    a = torch.randn(n, r, K, generator=gen, device=DEV) / K ** 0.5
+    b = torch.randn(n, M, r, generator=gen, device=DEV) / r ** 0.5
+    ad = ops.Adapters(a.bfloat16(), b.bfloat16(), torch.rand(n, generator=gen, device=DEV) * 2)
+    cols = torch.cat([torch.arange(130), torch.arange(130, M - 130, 29), torch.arange(M - 130, M)]).to(DEV)
+    part = ops.Adapters(ad.a, ad.b[:, cols].contiguous(), ad.scale)
     for ids in (pick(rng, T, n), np.sort(pick(rng, T, n))[::-1], np.full(T, n - 1)):
         ids = np.ascontiguousarray(ids).astype(np.int32)
-        x, y = normal(rng, T, K, dtype=x_t).to(DEV), normal(rng, T, M).to(DEV)
-        check(ops.adapter_add(y, x, ad, ops.route_rows(torch.from_numpy(ids).to(DEV), n)), y, x, ad, ids)
+        x = torch.randn(T, K, generator=gen, device=DEV).to(x_t)
+        y = torch.randn(T, M, generator=gen, device=DEV).to(y_t)
+        route = ops.route_rows(torch.from_numpy(ids).to(DEV), n)
+        got = ops.adapter_add(y, x, ad, route)
+        check(got[:, cols], y[:, cols], x, part, ids)
+        assert torch.equal(ops.adapter_add(y, x, ad, route, out=y), got)
 
 
 @pytest.mark.parametrize("T", [3, 90, 700])
@@ -200,7 +215,8 @@ def test_front_end_refuses_mismatched_buffers():
     assert ops.adapter_add(y[:0], x[:0], ad, ops.route_rows(torch.zeros(0, dtype=torch.int32, device=DEV), 3)).shape == (0, 64)
 
 
-@pytest.mark.parametrize("T,n,r,K,M", [(8, 8, 16, 1024, 512), (61, 24, 64, 2048, 512), (2000, 3, 32, 512, 528)])
+@pytest.mark.parametrize("T,n,r,K,M", [(8, 8, 16, 1024, 512), (61, 24, 64, 2048, 512), (2000, 3, 32, 512, 528),
+                                       (2000, 3, 32, 512, 10000)])
 def test_the_same_bits_every_time_two_streams_and_two_graphs(T, n, r, K, M):
     rng = np.random.default_rng(T)
     ad = make(rng, n, r, K, M)
