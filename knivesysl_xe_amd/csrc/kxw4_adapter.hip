@@ -171,14 +171,13 @@ __device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int
 }
 
 // low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
-// work-group takes 16 places of one adapter and part s, its WAVES waves
-// consecutive runs of 32-K steps, all r columns (CT tiles of 16). CUT: one part
-// of 16 TT places; scale * low is cut into its three BF16 parts here, in the
-// order the second launch's operand takes them. The places [p, p + 16) of adapter
-// e are cut tile p / 16 + e, a number of its own for each tile.
+// work-group takes 16 TT places of one adapter and part s, its WAVES waves
+// consecutive runs of 32-K steps, all r columns (CT tiles of 16). CUT: one part;
+// scale * low is cut into its three BF16 parts here, in the order the second
+// launch's operand takes them. The places [p, p + 16) of adapter e are cut tile p
+// / 16 + e, a number of its own for each tile.
 template <int CT, int WAVES, bool XB, bool CUT, int TT>
 __global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
-    static_assert(CUT || TT == 1, "parts of one tile");
     __shared__ float part[WAVES - 1][CT][256];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -693,10 +692,15 @@ int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
     }
     if (one_launch(a.n, a.T, a.r, a.K, a.M)) return a.r <= 16 ? launch_one<1>(a, x_bf16, y_bf16, st) : launch_one<2>(a, x_bf16, y_bf16, st);
     a.splits = adapter_splits(a.n, a.T, a.K);
+    // Two token tiles share A where many tiles read a long one (us in all for
+    // one / two: 2,520 tokens of 24, M = 1024, K = 12288, r = 128 70.4 / 49.6, r =
+    // 64 37.8 / 31.0; 1,536 of 8 48.3 / 40.0, M = 4096, K = 5120 40.1 / 38.6; K =
+    // 2048 25.2 / 26.9; 1,100 of 2, K = 5120 33.2 / 34.5; r = 16 alike).
+    const bool two = a.T >= 1536 && a.K >= 4096;
     if (a.r <= 16) launch_low<1, kFewWaves, false, 1>(a, x_bf16, st);
-    else if (a.r <= 32) launch_low<2, kFewWaves, false, 1>(a, x_bf16, st);
-    else if (a.r <= 64) launch_low<4, kFewWaves, false, 1>(a, x_bf16, st);
-    else if (a.r <= 128) launch_low<8, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 32) two ? launch_low<2, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<2, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 64) two ? launch_low<4, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<4, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 128) two ? launch_low<8, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<8, kFewWaves, false, 1>(a, x_bf16, st);
     else launch_low<16, kFewWaves, false, 1>(a, x_bf16, st);
     return a.r <= 32 ? launch_up<1>(a, y_bf16, st) : launch_up<2>(a, y_bf16, st);
 }

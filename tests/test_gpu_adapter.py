@@ -68,7 +68,9 @@ def check(got, y, x, ad, ids):
     (129, 200, 40, 256, 48), (300, 4, 256, 384, 96), (1000, 6, 16, 256, 1008), (70, 1024, 8, 128, 32), (5, 2, 200, 17408, 64),
     # many tokens, of few outputs
     (1536, 24, 16, 128, 1040), (1537, 1, 8, 256, 16), (2100, 6, 40, 256, 528), (1601, 3, 128, 384, 80), (3000, 2, 72, 128, 144),
-    (1600, 3, 136, 128, 48), (1600, 30, 32, 128, 48)])
+    (1600, 3, 136, 128, 48), (1600, 30, 32, 128, 48),
+    # with long rows of A
+    (1537, 3, 24, 4096, 48), (1600, 40, 56, 4224, 32), (2003, 1, 128, 5120, 16)])
 @pytest.mark.parametrize("x_t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("y_t", [torch.float32, torch.bfloat16])
 def test_against_float64(T, n, r, K, M, x_t, y_t):
