@@ -1,7 +1,6 @@
-// kxw4_gemm3.hpp — the large-tile kernel: prefill projections in the per-token mode (the BASELINE
-// configurations) on the 32x32x32 int8 MFMA: x_gemm_w4a8 / gemm_rc16
-// arithmetic (kernels_dpas.cpp:1255-1332, 1334-1490) with one split per
-// token.
+// kxw4_gemm3.hpp — the large-tile kernel: prefill projections in the per-token
+// mode on the 32x32x32 int8 MFMA: x_gemm_w4a8 / gemm_rc16 arithmetic
+// (kernels_dpas.cpp:1255-1332, 1334-1490) with one split per token.
 //
 // Cost model (measured on the MI355X): the FP32 chain needs one int->float
 // conversion and one FMA per output and weight group. A 32x32 block's four

@@ -1,6 +1,6 @@
-// kxw4_strip.hpp — the strip kernel: projections of one to a few hundred tokens under any split
-// plan: the GEMV (kernels_dpas.cpp:586-675, K16 683-760, W8 771-844), the
-// fan-out GEMV (945-1102) and the GEMM (1334-1490, W8 1578-1629).
+// kxw4_strip.hpp — the strip kernel: projections of one to a few hundred tokens
+// under any split plan: the GEMV (kernels_dpas.cpp:586-675, K16 683-760, W8
+// 771-844), the fan-out GEMV (945-1102) and the GEMM (1334-1490, W8 1578-1629).
 //
 // A wave owns a strip of 16 weight rows x one tile of TT tokens and one split
 // of K at a time, and runs its outputs' reference chains in registers: the
