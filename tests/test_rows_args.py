@@ -198,3 +198,27 @@ def test_a_plan_is_checked_once_and_copied_whole():
         assert (c.T, c.k, c.groups, c.order) == (4, 2, 8, other.order.data_ptr()) and c.order != ref._obj.order
     with pytest.raises(ValueError, match="route order must have shape"):
         ops._plan(dataclasses.replace(r, order=r.order[:3]), cpu)
+
+
+def test_a_call_runs_on_its_tensors_device(monkeypatch):
+    # the current device is 0; a call for device 1 makes that current around
+    # the launch and takes its stream, and a failure names the function
+    import contextlib
+    seen, current = [], [0]
+
+    @contextlib.contextmanager
+    def device(i):
+        before, current[0] = current[0], i
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setitem(ops._FUNCTIONS, "call", lambda *args: seen.append((current[0], args)) or 0)
+    monkeypatch.setitem(ops._FUNCTIONS, "fails", lambda *args: -2)
+    ops._launch("call", torch.device("cuda:0"), 5)
+    ops._launch("call", torch.device("cuda:1"), 6)
+    assert seen == [(0, (5, 100)), (1, (6, 101))] and current == [0]
+    with pytest.raises(_lib.KxError, match="fails"):
+        ops._launch("fails", torch.device("cuda:1"))
