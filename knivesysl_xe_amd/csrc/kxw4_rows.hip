@@ -177,7 +177,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const RouteArgs a) {
 // Slots per block: one block up to kPlanOne, past which the scattered writes
 // of `order` by one CU cost more than a second launch; else blocks of 2,048 up
 // to 256 of them, then larger ones. A small plan's block has a wave for each
-// 64 slots.
+// 64 slots, and for each 64 groups (64 slots of 1,024 groups: one wave 13.3 us,
+// sixteen 6.4; of 256 6.0 / 4.3).
 static int plan_round(long long v, int to) { return (int)((v + to - 1) / to * to); }
 int route_blocks_of(int N, int *per_block) {
     if (N <= kPlanOne) {
@@ -190,7 +191,8 @@ int route_blocks_of(int N, int *per_block) {
 
 int launch_route(RouteArgs &a, hipStream_t st) {
     const int nb = route_blocks_of(a.N, &a.per_block), G1 = a.groups + 1;
-    const int waves = std::min(a.per_block / 64, kPlanWaves);
+    const int waves = std::min(std::max(a.per_block, plan_round(G1, 64)) / 64, kPlanWaves);
+    if (a.per_block < 64 * waves) a.per_block = 64 * waves;  // (one block: the later waves' runs are empty)
     const size_t lds = (size_t)(waves + 1) * G1 * sizeof(int);            // (at most 69.7 KB: 1,024 groups)
     static bool attr[64] = {};                               // (the attribute is per device)
     int dev = 0;
