@@ -154,21 +154,26 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const RouteArgs a) {
             if (s0 + 64 * i >= w1) break;
             const int s = s0 + 64 * i + lane, kk = key[i];
             const bool on = kk >= 0;
-            unsigned long long same = __ballot(on);
+            // (lanes with this lane's key: for each bit those that agree with
+            // it, the bit spread over a word)
+            const unsigned long long all = __ballot(on);
+            uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
             for (int b = 0; b < bits; ++b) {
-                const unsigned long long one = __ballot(kk >> b & 1);
-                same &= (kk >> b & 1) ? one : ~one;
+                const uint32_t bit = (uint32_t)((int32_t)((uint32_t)kk << (31 - b)) >> 31);
+                const unsigned long long one = __ballot(bit);
+                lo &= ~((uint32_t)one ^ bit);
+                hi &= ~((uint32_t)(one >> 32) ^ bit);
             }
-            const unsigned long long below = same & ((1ull << lane) - 1);
+            const int below = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
             if (on) {
-                const int place = tot[kk] + mine[kk] + __popcll(below);
+                const int place = tot[kk] + mine[kk] + below;
                 a.order[place] = s;
                 a.position[s] = kk < G ? place : -1;
             }
             // (the wave's reads above come before this write: LDS accesses of
             // one wave complete in order)
             __builtin_amdgcn_wave_barrier();
-            if (on && below == 0) mine[kk] = mine[kk] + __popcll(same);
+            if (on && below == 0) mine[kk] = mine[kk] + __popc(lo) + __popc(hi);
             __builtin_amdgcn_wave_barrier();
         }
     }
