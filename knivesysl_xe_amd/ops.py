@@ -605,9 +605,9 @@ def route_rows(ids: torch.Tensor, groups: int, out: Optional[RowRoute] = None) -
     if not 1 <= groups <= 1024:
         raise ValueError(f"groups must be 1 to 1024, got {groups}")
     if out is not None:
-        if (out.T, out.k, out.groups) != (T, k, groups):
-            raise ValueError("out does not match the ids' shape / groups")
         r, ref = out, _plan(out, dev)
+        if (r.T, r.k, r.groups) != (T, k, groups):
+            raise ValueError("out does not match the ids' shape / groups")
     else:
         r = RowRoute.empty(T, k, groups, dev)
         ref = _make_plan(r, dev)

@@ -300,3 +300,13 @@ def test_the_same_bits_every_time_and_two_streams_at_once(mode, T, groups, K, M)
                 got.append(ops.expert_gemm(w, a, r, out=torch.zeros(2 * T, M, device=DEV)))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("mode", ["token128", "block32", "w8"])
+def test_no_tokens(mode):
+    rng = np.random.default_rng(4)
+    w, _ = weight(rng, mode, 4 * 32, 256)
+    r = ops.route_rows(torch.zeros(0, 3, dtype=torch.int64, device=DEV), 4)
+    assert r.offsets.tolist() == [0] * 5
+    a = ops.QuantAct.empty(0, 256, MODES[mode][1], DEV)
+    assert ops.expert_gemm(w, a, r).shape == ops.expert_gemm(w, a, r, sorted_rows=True).shape == (0, 32)

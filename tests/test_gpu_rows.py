@@ -318,3 +318,17 @@ def test_every_float32_pattern_rounds_to_the_nearest_bfloat16():
     y = ops.combine_rows(ops.dispatch_rows(x, r), r, dtype=torch.bfloat16)
     want = x.bfloat16()
     assert ((y == want) | (torch.isnan(y) & torch.isnan(want))).all()
+
+
+def test_plans_passed_as_out_are_checked():
+    import dataclasses
+    ids = torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="must be a RowRoute"):
+        ops.route_rows(ids, 8, out=(4, 2, 8))
+    with pytest.raises(ValueError, match="does not match"):
+        ops.route_rows(ids, 8, out=ops.RowRoute.empty(4, 2, 9))
+    r = ops.RowRoute.empty(4, 2, 8)
+    with pytest.raises(ValueError, match="route position must be torch.int32"):
+        ops.route_rows(ids, 8, out=dataclasses.replace(r, position=r.position.float()))
+    with pytest.raises(ValueError, match="must be on the GPU|must be on cuda"):
+        ops.route_rows(ids, 8, out=ops.RowRoute.empty(4, 2, 8, "cpu"))
