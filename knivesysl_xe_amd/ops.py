@@ -360,12 +360,9 @@ def gemv(w: W4Weight, a: QuantAct, dtype=torch.float32, residual=None, splits: i
     return y
 
 
-_WEIGHT_PTR = C.POINTER(_lib.Weight)
-
-
 def _weight_array(ws: Sequence[W4Weight]):
     cs = [w.c() for w in ws]
-    arr = (_WEIGHT_PTR * len(ws))(*[C.pointer(c) for c in cs])
+    arr = (C.POINTER(_lib.Weight) * len(ws))(*[C.pointer(c) for c in cs])
     return cs, arr
 
 
@@ -680,6 +677,11 @@ def dispatch_rows_backward(drows: torch.Tensor, route: RowRoute, dtype=None, out
     return combine_rows(drows, route, None, dtype, out)
 
 
+_OUTS = tuple(f"outs[{i}]" for i in range(4))
+_WEIGHT_ARRAYS = tuple(C.POINTER(_lib.Weight) * n for n in range(5))
+_POINTER_ARRAYS = tuple(C.c_void_p * n for n in range(5))
+
+
 def expert_gemm_fanout(ws: Sequence[W4Weight], a: QuantAct, route: RowRoute, dtype=torch.float32,
                        sorted_rows: bool = False, outs=None):
     """Up to 4 weights (an expert's gate and up) over one activation, each row
@@ -703,10 +705,11 @@ def expert_gemm_fanout(ws: Sequence[W4Weight], a: QuantAct, route: RowRoute, dty
         raise ValueError(f"the activation has {a.T} rows for {N if sorted_rows else route.T} of the plan")
     if outs is not None and len(outs) != len(ws):
         raise ValueError(f"outs has {len(outs)} tensors for {len(ws)} weights")
-    ys = [_out(N, w.M // route.groups, dtype, dev, None if outs is None else outs[i], f"outs[{i}]")
+    ys = [_out(N, w.M // route.groups, dtype, dev, None if outs is None else outs[i], _OUTS[i])
           for i, w in enumerate(ws)]
-    keep, warr = _weight_array(ws)
-    yarr = (C.c_void_p * len(ws))(*[y.data_ptr() for y in ys])
+    keep = [w.c() for w in ws]
+    warr = _WEIGHT_ARRAYS[len(ws)](*[C.pointer(c) for c in keep])
+    yarr = _POINTER_ARRAYS[len(ws)](*[y.data_ptr() for y in ys])
     ac = a.c()
     _launch("kxw4_expert_gemm", dev, warr, yarr, len(ws), C.byref(ac), plan, bool(sorted_rows), _dtype_code(dtype))
     return ys
