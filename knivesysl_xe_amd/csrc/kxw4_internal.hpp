@@ -200,6 +200,10 @@ struct RouteArgs {
 int route_blocks_of(int N, int *per_block);
 int launch_route(RouteArgs &a, hipStream_t st);
 
+// Work-groups of `threads` that one launch takes: the runtime cuts a grid's
+// threads to 32 bits, without an error, so it has to hold fewer than 2^32.
+inline long long grid_limit(int threads) { return ((1ll << 32) - 1) / threads; }
+
 // Rows of H elements: x by token, rows by sorted place.
 struct RowArgs {
     const void *x;                    // dispatch: source; combine backward: dy
@@ -209,7 +213,7 @@ struct RowArgs {
     float *dweights;
     const int *position;
     int T, k, H;
-    int pieces, lanes, per, chunks, past;       // (set by the launcher)
+    int pieces, lanes, per, chunks, past, t0;   // (set by the launcher; t0: a launch's first token)
 };
 int launch_dispatch(RowArgs &a, bool bf16, hipStream_t st);
 int launch_combine(RowArgs &a, bool rows_bf16, bool y_bf16, hipStream_t st);

@@ -299,10 +299,10 @@ __device__ __forceinline__ RowAt row_at(const RowArgs &a) {
     const int block = blockIdx.x;
     if constexpr (WIDE) {
         const int t = block / a.chunks;
-        return {t, (block - t * a.chunks) * a.lanes + (int)threadIdx.x};
+        return {a.t0 + t, (block - t * a.chunks) * a.lanes + (int)threadIdx.x};
     } else {
         const int sub = threadIdx.x / a.lanes;
-        return {block * a.per + sub, (int)threadIdx.x - sub * a.lanes};
+        return {a.t0 + block * a.per + sub, (int)threadIdx.x - sub * a.lanes};
     }
 }
 template <int V, bool SHORT>
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Row
     constexpr int V = RB ? 8 : 4;
     __shared__ float part[kRowThreads / 64][kDots];
     const int runs = (a.k + kDots - 1) / kDots;
-    const int t = blockIdx.x / runs, j0 = (blockIdx.x - t * runs) * kDots;
+    const int run = blockIdx.x / runs, t = a.t0 + run, j0 = (blockIdx.x - run * runs) * kDots;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int p[kDots];
     float w[kDots], dot[kDots] = {};
@@ -420,29 +420,37 @@ __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(const Row
     }
 }
 
+// One launch for as many tokens as its grid holds (grid_limit); a block takes
+// `tokens` of them, or a token `blocks` blocks. (16.8 million tokens at 256
+// threads each.)
+typedef void (*RowKernel)(const RowArgs);
+static int launch_tokens(RowKernel k, RowArgs &a, int tokens, int blocks, int threads, hipStream_t st) {
+    const long long most = grid_limit(threads) / blocks * tokens;
+    if (most == 0) return -2;
+    for (long long t0 = 0; t0 < a.T; t0 += most) {
+        a.t0 = (int)t0;
+        const long long grid = (std::min(most, a.T - t0) + tokens - 1) / tokens * blocks;
+        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(threads), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return -6;
+    }
+    return 0;
+}
+
 // Threads and blocks of a row kernel: rows of up to 32 pieces share a
 // 256-thread block, longer ones take a block each, or several of up to 512
 // threads.
-typedef void (*RowKernel)(const RowArgs);
 static int launch_rows(RowKernel wide, RowKernel narrow, RowArgs &a, hipStream_t st) {
-    long long blocks;
-    int threads;
     if (a.pieces <= 32) {
         a.lanes = 1;
         while (a.lanes < a.pieces) a.lanes *= 2;
         a.per = kRowThreads / a.lanes;
         a.chunks = 1;
-        threads = kRowThreads;
-        blocks = ((long long)a.T + a.per - 1) / a.per;
-    } else {
-        a.per = 1;
-        a.chunks = (a.pieces + 511) / 512;
-        a.lanes = threads = ((a.pieces + a.chunks - 1) / a.chunks + 63) / 64 * 64;
-        blocks = (long long)a.T * a.chunks;
+        return launch_tokens(narrow, a, a.per, 1, kRowThreads, st);
     }
-    if (blocks >= (1ll << 31)) return -2;
-    hipLaunchKernelGGL(a.pieces <= 32 ? narrow : wide, dim3((unsigned)blocks), dim3(threads), 0, st, a);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
+    a.per = 1;
+    a.chunks = (a.pieces + 511) / 512;
+    a.lanes = ((a.pieces + a.chunks - 1) / a.chunks + 63) / 64 * 64;
+    return launch_tokens(wide, a, 1, a.chunks, a.lanes, st);
 }
 
 // Every row is read once, so the loads are marked as not to be kept. The
@@ -486,11 +494,8 @@ static RowKernel backward_of(bool dy_bf16, bool rows_bf16) {
 int launch_combine_backward(RowArgs &a, bool dy_bf16, bool rows_bf16, hipStream_t st) {
     a.pieces = pieces_of(a.H, rows_bf16);
     a.past = past_cache((long long)a.T * a.k * a.H * (rows_bf16 ? 2 : 4));
-    const long long blocks = (long long)a.T * ((a.k + kDots - 1) / kDots);
-    if (blocks >= (1ll << 31)) return -2;
     const RowKernel k = a.pieces == 1 ? backward_of<true>(dy_bf16, rows_bf16) : backward_of<false>(dy_bf16, rows_bf16);
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kRowThreads), 0, st, a);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
+    return launch_tokens(k, a, 1, (a.k + kDots - 1) / kDots, kRowThreads, st);
 }
 
 }  // namespace kxw4
