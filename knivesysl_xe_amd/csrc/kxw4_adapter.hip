@@ -182,8 +182,9 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterAr
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile * TT, lane);
-    if ((int)blockIdx.x >= tiles.total) return;
-    const GroupTile tile = tile_at(tiles, a.offsets, kLowTile * TT, blockIdx.x);
+    const int u = a.tile0 + blockIdx.x;
+    if (u >= tiles.total) return;
+    const GroupTile tile = tile_at(tiles, a.offsets, kLowTile * TT, u);
     const int p0 = tile.begin + tile.index * kLowTile * TT;
     const int steps = a.K / 32, ways = a.splits * WAVES, way = blockIdx.y * WAVES + wave;
     const int k0 = (int)((long long)steps * way / ways), k1 = (int)((long long)steps * (way + 1) / ways);
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const Adapter
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int mblocks = (a.M + kUpBlock - 1) / kUpBlock;
-    const int u = blockIdx.x / mblocks, m0 = (blockIdx.x - u * mblocks) * kUpBlock + wave * kUpRows;
+    const int v = blockIdx.x / mblocks, u = a.tile0 + v, m0 = (blockIdx.x - v * mblocks) * kUpBlock + wave * kUpRows;
     const GroupTiles tiles = scan_tiles(a.offsets, a.n, kLowTile, lane);
     int p0, p1, e = -1;
     if (u < tiles.total) {
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const Ada
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int mblocks = (a.M + kManyBlock - 1) / kManyBlock;
-    const int u = blockIdx.x / mblocks, m0 = (blockIdx.x - u * mblocks) * kManyBlock + wave * kManyRows;
+    const int v = blockIdx.x / mblocks, u = a.tile0 + v, m0 = (blockIdx.x - v * mblocks) * kManyBlock + wave * kManyRows;
     // a run: a.run tiles of one adapter; `first`: the cut tile of its first
     const GroupTiles runs = scan_tiles(a.offsets, a.n, kLowTile * a.run, lane);
     int p0, p1, e = -1;
@@ -627,10 +628,22 @@ size_t adapter_scratch(int n, int T, int r, int K, int M) {
     return one_launch(n, T, r, K, M) ? 0 : (size_t)adapter_splits(n, T, K) * T * r * sizeof(float);
 }
 
+// One launch for as many tiles as its grid holds (grid_limit), each of `blocks`
+// work-groups. (134 million tokens of one adapter at 1,024 threads a tile of 32.)
+typedef void (*AdapterKernel)(const AdapterArgs);
+static int launch_tiles(AdapterKernel k, AdapterArgs &a, long long tiles, int blocks, int parts, int threads, size_t lds, hipStream_t st) {
+    const long long most = grid_limit(threads) / blocks;
+    for (long long t0 = 0; t0 < tiles; t0 += most) {
+        a.tile0 = (int)t0;
+        hipLaunchKernelGGL(k, dim3((unsigned)(std::min(most, tiles - t0) * blocks), parts), dim3(threads), lds, st, a);
+        if (hipGetLastError() != hipSuccess) return -6;
+    }
+    return 0;
+}
+
 template <int CT>
 static int launch_one(const AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
-    const long long grid = (tiles_at_most(a.T, a.n, kLowTile) + 1) * ((a.M + kOneBlock - 1) / kOneBlock);
-    if (grid >= (1ll << 31)) return -2;
+    const long long grid = (tiles_at_most(a.T, a.n, kLowTile) + 1) * ((a.M + kOneBlock - 1) / kOneBlock);      // (at most the CUs: one_launch)
     auto k = x_bf16 ? (y_bf16 ? adapter_one_kernel<CT, true, true> : adapter_one_kernel<CT, true, false>)
                     : (y_bf16 ? adapter_one_kernel<CT, false, true> : adapter_one_kernel<CT, false, false>);
     hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * kOneWaves), 0, st, a);
@@ -638,10 +651,9 @@ static int launch_one(const AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_
 }
 
 template <int CT, int WAVES, bool CUT, int TT>
-static void launch_low(const AdapterArgs &a, bool x_bf16, hipStream_t st) {
-    const dim3 grid((unsigned)tiles_at_most(a.T, a.n, kLowTile * TT), a.splits);
-    if (x_bf16) hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, true, CUT, TT>), grid, dim3(64 * WAVES), 0, st, a);
-    else hipLaunchKernelGGL((adapter_low_kernel<CT, WAVES, false, CUT, TT>), grid, dim3(64 * WAVES), 0, st, a);
+static int launch_low(AdapterArgs &a, bool x_bf16, hipStream_t st) {
+    return launch_tiles(x_bf16 ? adapter_low_kernel<CT, WAVES, true, CUT, TT> : adapter_low_kernel<CT, WAVES, false, CUT, TT>, a,
+                        tiles_at_most(a.T, a.n, kLowTile * TT), 1, a.splits, 64 * WAVES, 0, st);
 }
 
 // The first launch for many tokens. One work-group of either takes about as long
@@ -651,21 +663,18 @@ static void launch_low(const AdapterArgs &a, bool x_bf16, hipStream_t st) {
 // 48.8, r = 128 117 / 99, K = 12288, M = 1024, r = 64 71 / 58; 3,965 of 6, K =
 // 5120, r = 32 32 / 36).
 template <int TT>
-static void launch_cut(const AdapterArgs &a, bool x_bf16, hipStream_t st) {
-    if (a.r <= 16) launch_low<1, 16, true, TT>(a, x_bf16, st);
-    else if (a.r <= 32) launch_low<2, 16, true, TT>(a, x_bf16, st);
-    else if (a.r <= 64) launch_low<4, 8, true, TT>(a, x_bf16, st);
-    else launch_low<8, 8, true, TT>(a, x_bf16, st);
+static int launch_cut(AdapterArgs &a, bool x_bf16, hipStream_t st) {
+    if (a.r <= 16) return launch_low<1, 16, true, TT>(a, x_bf16, st);
+    if (a.r <= 32) return launch_low<2, 16, true, TT>(a, x_bf16, st);
+    if (a.r <= 64) return launch_low<4, 8, true, TT>(a, x_bf16, st);
+    return launch_low<8, 8, true, TT>(a, x_bf16, st);
 }
 
 template <int KC>
-static int launch_up(const AdapterArgs &a, bool y_bf16, hipStream_t st) {
-    const long long grid = (tiles_at_most(a.T, a.n, kLowTile) + 1) * ((a.M + kUpBlock - 1) / kUpBlock);
-    if (grid >= (1ll << 31)) return -2;
+static int launch_up(AdapterArgs &a, bool y_bf16, hipStream_t st) {
     const size_t lds = (size_t)3 * kLowTile * up_pitch(a.r) * 2;          // (at most 25.3 KB: r = 256)
-    if (y_bf16) hipLaunchKernelGGL((adapter_up_kernel<KC, true>), dim3((unsigned)grid), dim3(64 * kUpWaves), lds, st, a);
-    else hipLaunchKernelGGL((adapter_up_kernel<KC, false>), dim3((unsigned)grid), dim3(64 * kUpWaves), lds, st, a);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
+    return launch_tiles(y_bf16 ? adapter_up_kernel<KC, true> : adapter_up_kernel<KC, false>, a,
+                        tiles_at_most(a.T, a.n, kLowTile) + 1, (a.M + kUpBlock - 1) / kUpBlock, 1, 64 * kUpWaves, lds, st);
 }
 
 // Tiles per run: up to twelve, so that B is read seldom, while six (three,
@@ -676,18 +685,15 @@ static int launch_many(AdapterArgs &a, bool y_bf16, hipStream_t st) {
     const int mblocks = (a.M + kManyBlock - 1) / kManyBlock;
     const long long work = tiles_at_most(a.T, a.n, kLowTile) * mblocks, groups = (KC <= 2 ? 6ll : 3ll) * device_cus();
     a.run = (int)std::max(1ll, std::min(12ll, (work + groups / 2) / groups));
-    const long long grid = (tiles_at_most(a.T, a.n, kLowTile * a.run) + 1) * mblocks;
-    if (grid >= (1ll << 31)) return -2;
-    if (y_bf16) hipLaunchKernelGGL((adapter_many_kernel<KC, true>), dim3((unsigned)grid), dim3(64 * kManyWaves), 0, st, a);
-    else hipLaunchKernelGGL((adapter_many_kernel<KC, false>), dim3((unsigned)grid), dim3(64 * kManyWaves), 0, st, a);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
+    return launch_tiles(y_bf16 ? adapter_many_kernel<KC, true> : adapter_many_kernel<KC, false>, a,
+                        tiles_at_most(a.T, a.n, kLowTile * a.run) + 1, mblocks, 1, 64 * kManyWaves, 0, st);
 }
 
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
     if (many_tokens(a.n, a.T, a.r, a.M)) {
         a.splits = 1;
-        if (tiles_at_most(a.T, a.n, kLowTile) <= device_cus()) launch_cut<1>(a, x_bf16, st);
-        else launch_cut<2>(a, x_bf16, st);
+        const int rc = tiles_at_most(a.T, a.n, kLowTile) <= device_cus() ? launch_cut<1>(a, x_bf16, st) : launch_cut<2>(a, x_bf16, st);
+        if (rc) return rc;
         return a.r <= 32 ? launch_many<1>(a, y_bf16, st) : a.r <= 64 ? launch_many<2>(a, y_bf16, st) : launch_many<4>(a, y_bf16, st);
     }
     if (one_launch(a.n, a.T, a.r, a.K, a.M)) return a.r <= 16 ? launch_one<1>(a, x_bf16, y_bf16, st) : launch_one<2>(a, x_bf16, y_bf16, st);
@@ -697,11 +703,13 @@ int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
     // 64 37.8 / 31.0; 1,536 of 8 48.3 / 40.0, M = 4096, K = 5120 40.1 / 38.6; K =
     // 2048 25.2 / 26.9; 1,100 of 2, K = 5120 33.2 / 34.5; r = 16 alike).
     const bool two = a.T >= 1536 && a.K >= 4096;
-    if (a.r <= 16) launch_low<1, kFewWaves, false, 1>(a, x_bf16, st);
-    else if (a.r <= 32) two ? launch_low<2, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<2, kFewWaves, false, 1>(a, x_bf16, st);
-    else if (a.r <= 64) two ? launch_low<4, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<4, kFewWaves, false, 1>(a, x_bf16, st);
-    else if (a.r <= 128) two ? launch_low<8, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<8, kFewWaves, false, 1>(a, x_bf16, st);
-    else launch_low<16, kFewWaves, false, 1>(a, x_bf16, st);
+    int rc;
+    if (a.r <= 16) rc = launch_low<1, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 32) rc = two ? launch_low<2, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<2, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 64) rc = two ? launch_low<4, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<4, kFewWaves, false, 1>(a, x_bf16, st);
+    else if (a.r <= 128) rc = two ? launch_low<8, kFewWaves, false, 2>(a, x_bf16, st) : launch_low<8, kFewWaves, false, 1>(a, x_bf16, st);
+    else rc = launch_low<16, kFewWaves, false, 1>(a, x_bf16, st);
+    if (rc) return rc;
     return a.r <= 32 ? launch_up<1>(a, y_bf16, st) : launch_up<2>(a, y_bf16, st);
 }
 

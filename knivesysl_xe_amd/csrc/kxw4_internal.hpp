@@ -228,7 +228,7 @@ struct AdapterArgs {
     float *low;                       // scratch
     const int *offsets, *order;
     int T, n, r, K, M;
-    int splits, run;                  // (set by the launcher)
+    int splits, run, tile0;           // (set by the launcher; tile0: a launch's first tile)
 };
 size_t adapter_scratch(int n, int T, int r, int K, int M);      // bytes of `low`
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st);

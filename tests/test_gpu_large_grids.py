@@ -61,3 +61,24 @@ def test_dispatch_and_combine_of_many_tokens():
     for t in range(0, T, step):
         assert torch.equal(rows[r.position[t:t + step, 0].long()], x[t:t + step]), t
         assert torch.equal(y[t:t + step], x[t:t + step]), t
+
+
+def test_adapters_of_many_tokens():
+    # 32 tokens a work-group of 1,024 threads in the first of the two launches
+    T, K, M, r, n, step = (1 << 27) + 777, 128, 16, 8, 3, 1 << 20
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(2)
+    ids = torch.randint(-1, n, (T,), generator=gen, device=DEV, dtype=torch.int32)
+    x = torch.empty(T, K, dtype=torch.bfloat16, device=DEV)              # 34 GB of 1 and -1
+    x.view(torch.int16).random_(0, 2, generator=gen).mul_(-0x8000).add_(0x3F80)
+    a, b, y = whole(gen, n, r, K), whole(gen, n, M, r), whole(gen, T, M, dtype=torch.float32)
+    scale = torch.tensor([0.5, 2.0, -1.0], device=DEV)
+    got = ops.adapter_add(y, x, ops.Adapters(a, b, scale), ops.route_rows(ids, n))
+    # (|update| <= 2 * 8 * 8 * 8 * 128 = 2^17 in halves: exact)
+    both = (b.double() @ a.double()) * scale.double()[:, None, None]
+    for t in range(0, T, step):
+        want = y[t:t + step].double()
+        for e in range(n):
+            at = ids[t:t + step] == e
+            want[at] += x[t:t + step][at].double() @ both[e].t()
+        assert torch.equal(got[t:t + step].double(), want), t
