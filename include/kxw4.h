@@ -321,7 +321,9 @@ int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, i
  * KXW4_SCALE_FP16_ZP4 of group 32 or 64, or with KXW4_SCALE_W8; else
  * KXW4_ETIER. The arithmetic of a row is kxw4_gemm's under a split count that
  * follows from the sizes alone (T, k, groups, rows, K). a's rows * K < 2^31;
- * 16-byte aligned pointers (4 for per-token scales). */
+ * -2 too where the launch would take 2^32 threads (with tens of rows an expert
+ * not before N times the weights' rows per expert comes to 2^35); 16-byte
+ * aligned pointers (4 for per-token scales). */
 int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count, const kxw4_act_t *a,
                      const kxw4_route_t *route, int sorted_rows, int y_dtype, void *stream);
 

@@ -62,7 +62,7 @@ static int ex_strips(const ExpertArgs &x, int S, hipStream_t st) {
     a.groups = x.groups;
     a.k = x.k;
     const long long grid = tiles_at_most(x.N, x.groups, TT) * blk;
-    if (grid >= (1ll << 31)) return -2;
+    if (grid > grid_limit(64 * a.waves)) return -2;
     const size_t lds = std::max((size_t)2 * S * SH::STAGE, (size_t)std::max(2 * a.waves, RW) * SH::NT * 1024);
     if (lds > 160 * 1024 || a.waves > 8) return -2;          // (expert_splits never asks for it)
     auto k = strip_kernel<TT, RW, U, UNIT, BLK, kVarGemm, WF, true>;
@@ -122,7 +122,7 @@ static int ex_tiles(const ExpertArgs &x, hipStream_t st) {
     using S = G3Shape<TA, TB, 1, WNW, UNIT, 0>;
     const GemmArgs a = ex_args(x, S::BNG);
     const long long grid = tiles_at_most(x.N, x.groups, S::BM) * a.n_tiles;
-    if (grid >= (1ll << 31)) return -2;
+    if (grid > grid_limit(S::NTH)) return -2;
     auto k = gemm3_group_kernel<TA, TB, WNW, UNIT, NST, OCC>;
     // (the shorter tiles' output staging may take more than their stages)
     const size_t lds = std::max({S::template lds_bytes<NST>(), G3Shape<(TA > 1 ? TA / 2 : 1), TB, 1, WNW, UNIT, 0>::template lds_bytes<NST>(),
@@ -141,7 +141,7 @@ static int ex_blocks(const ExpertArgs &x, hipStream_t st) {
     using S = GrShape<2, 4, 1, GROUP>;
     const GemmArgs a = ex_args(x, S::RGS);
     const long long grid = tiles_at_most(x.N, x.groups, S::BM) * a.n_tiles;
-    if (grid >= (1ll << 31)) return -2;
+    if (grid > grid_limit(S::NTH)) return -2;
     auto k = gemmr_group_kernel<GROUP, NST, 4>;
     const size_t lds = std::max(S::template lds_bytes<NST>(), GrShape<1, 4, 1, GROUP>::template lds_bytes<NST>());
     static bool done[64] = {};

@@ -110,6 +110,17 @@ def test_expert_gemm_refuses_bad_arguments():
     assert call(r=R(T=0, offsets=None, order=None, position=None), a=A(T=0, q=None, scale=None), y=None) == 0
 
 
+def test_expert_gemm_refuses_grids_past_two_to_the_32_threads():
+    # W8 strips of 32 places x 64 rows: 2^25 slots x 2,048 rows come to 2^25
+    # work-groups of 256 threads, of which a launch would leave none
+    f = _lib.lib().kxw4_expert_gemm
+    for rows in (2048, 1 << 14):
+        w = W(M=8 * rows, K=1024, group=32, enc=2)
+        arr, ys = (C.POINTER(_lib.Weight) * 1)(C.pointer(w)), (C.c_void_p * 1)(64)
+        a, r = A(T=1 << 20, block=32), R(T=1 << 20, k=32, groups=8)
+        assert f(arr, ys, 1, C.byref(a), C.byref(r), 0, 0, None) == _lib.ESHAPE
+
+
 def test_adapter_add_refuses_bad_arguments():
     L = _lib.lib()
 
