@@ -532,8 +532,9 @@ class RowRoute:
     """The plan that sorts a batch's slots (token t, choice j, slot t*k + j) by
     the group each names: an expert, or an adapter (k = 1). Made by route_rows
     and shared by every call of a step, its backward pass among them; the calls
-    trust its contents. The first call checks its buffers, which stay its own
-    (route_rows writes them again when the plan is passed as `out`)."""
+    trust its contents. The first call checks its buffers, and so does one that
+    finds them at another address (route_rows writes them again when the plan is
+    passed as `out`)."""
     T: int
     k: int
     groups: int
@@ -541,11 +542,13 @@ class RowRoute:
     order: torch.Tensor      # int32 [T*k]: the slot at each place, those without a group last
     position: torch.Tensor   # int32 [T][k]: the place of each slot, -1 without a group
 
-    _made = None             # (device, reference to the C struct) once checked
+    _made = None             # (device, addresses, reference to the C struct) once checked
+
+    def at(self) -> tuple:
+        return self.offsets.data_ptr(), self.order.data_ptr(), self.position.data_ptr()
 
     def c(self) -> _lib.Route:
-        return _lib.Route(self.T, self.k, self.groups, self.offsets.data_ptr(), self.order.data_ptr(),
-                          self.position.data_ptr())
+        return _lib.Route(self.T, self.k, self.groups, *self.at())
 
     def __reduce__(self):    # (a copy is checked anew)
         return RowRoute, (self.T, self.k, self.groups, self.offsets, self.order, self.position)
@@ -558,17 +561,19 @@ class RowRoute:
 
 
 def _plan(r: RowRoute, device):
-    """The C struct of a plan on `device`, by reference."""
+    """The C struct of a plan on `device`, by reference: the one made before
+    while its tensors lie where they did. (set_, .data and resize_ past their
+    memory move them; a tensor shortened in place keeps its memory.)"""
     if r.__class__ is RowRoute:
         made = r._made
-        if made is not None and made[0] == device:
-            return made[1]
+        if made is not None and made[0] == device and made[1] == r.at():
+            return made[2]
     return _make_plan(_check_route(r, device), device)
 
 
 def _make_plan(r: RowRoute, device):
     ref = C.byref(r.c())
-    r.__dict__["_made"] = (device, ref)
+    r.__dict__["_made"] = (device, r.at(), ref)
     return ref
 
 

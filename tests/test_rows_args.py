@@ -211,6 +211,36 @@ def test_a_plan_is_checked_once_and_copied_whole():
         ops._plan(dataclasses.replace(r, order=r.order[:3]), cpu)
 
 
+def test_a_checked_plan_follows_its_tensors():
+    # a plan whose tensors were given other memory is checked anew
+    cpu = torch.device("cpu")
+
+    def checked():
+        r = ops.RowRoute.empty(4, 2, 8, "cpu")
+        ops._plan(r, cpu)
+        return r
+
+    for name in ("offsets", "order", "position"):
+        size = getattr(checked(), name).shape
+        for move in (lambda t: t.set_(torch.empty(size, dtype=torch.int32)),
+                     lambda t: setattr(t, "data", torch.empty(size, dtype=torch.int32))):
+            r = checked()
+            move(getattr(r, name))
+            assert getattr(ops._plan(r, cpu)._obj, name) == getattr(r, name).data_ptr()
+        r = checked()
+        getattr(r, name).resize_(4096)
+        with pytest.raises(ValueError, match=f"route {name} must have shape"):
+            ops._plan(r, cpu)
+        r = checked()
+        getattr(r, name).data = torch.empty(size, dtype=torch.int64)
+        with pytest.raises(ValueError, match=f"route {name} must be torch.int32"):
+            ops._plan(r, cpu)
+        # memory that was given back: no address is left, which the C calls refuse
+        r = checked()
+        getattr(r, name).untyped_storage().resize_(0)
+        assert not getattr(ops._plan(r, cpu)._obj, name)
+
+
 def test_a_call_runs_on_its_tensors_device(monkeypatch):
     # the current device is 0; a call for device 1 makes that current around
     # the launch and takes its stream, and a failure names the function
