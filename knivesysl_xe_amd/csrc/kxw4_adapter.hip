@@ -14,6 +14,10 @@
 // of its own: the products are exact again. `low` is held in FP32 and cut the
 // same way. The sums run in a fixed order: within a
 // wave's steps, then the waves of a work-group, then the work-groups' parts.
+// A part that is zero makes a NaN of an infinity in A or B that the whole value
+// does not, so a wave whose sums are not finite works them out again, the second
+// and third parts times the finite elements alone (finite8). Looking for that
+// costs 0-2 %.
 //
 // v_mfma_f32_16x16x32_bf16: lane l supplies row (A) / column (B) l%16 and the
 // eight K slots 8*(l/16)..+7; result register i of lane l is row 4*(l/16)+i,
@@ -35,7 +39,8 @@ __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
 
 // x as the sum of three BF16 values, by cutting: each part takes the leading
 // eight mantissa bits of what the one before left, and the differences are
-// exact. An infinity or NaN goes into the first part whole.
+// exact (what lies below 2^-133, the least BF16 value, is cut off). An infinity
+// or NaN goes into the first part whole.
 __device__ __forceinline__ void split3(float x, uint32_t (&part)[3]) {
     const uint32_t b = __float_as_uint(x);
     const bool finite = (b & 0x7F800000u) != 0x7F800000u;
@@ -56,6 +61,46 @@ __device__ __forceinline__ void split8(const float (&v)[8], v4u (&op)[3]) {
 #pragma unroll
         for (int q = 0; q < 3; ++q) op[q][i] = lo[q] >> 16 | hi[q];
     }
+}
+
+// An operand's BF16 elements, zeros for those that are not finite. (The empty
+// statement keeps the compiler from working this out ahead of the branch it is
+// needed in, and holding it.)
+__device__ __forceinline__ v4u finite8(v4u w) {
+    asm volatile("" : "+v"(w));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] &= ((w[i] & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu) | ((w[i] & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u);
+    return w;
+}
+
+// acc + w times the three parts of a value, as mfma_bf16 of each adds them, but
+// w's infinities by the first part alone. (Nothing is moved across: the branches
+// that come here are not to cost the others registers.)
+template <class Part>
+__device__ __forceinline__ void mfma_again(v4u w, Part part, bool w_first, v4f &acc) {
+    __builtin_amdgcn_sched_barrier(0);
+    const v4u f = finite8(w);
+#pragma unroll
+    for (int q = 2; q >= 0; --q) {
+        const v4u o = q > 0 ? f : w;
+        acc = w_first ? mfma_bf16(o, part(q), acc) : mfma_bf16(part(q), o, acc);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Whether an infinity or NaN of the weights may have reached a wave's sums: it
+// reaches those of every token. ROWS: registers of an MFMA's result that differ
+// in the weights' row (1: they differ in the token alone).
+template <int ROWS, int N>
+__device__ __forceinline__ bool any_far(const v4f (&acc)[N]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if constexpr (ROWS == 1) s += acc[c][0];
+        else s += (acc[c][0] + acc[c][1]) + (acc[c][2] + acc[c][3]);
+    }
+    return __ballot(!(__builtin_fabsf(s) <= 3.40282347e38f)) != 0;
 }
 
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
@@ -89,9 +134,9 @@ constexpr int kCutChunk = 3 * 64 * 8;
 // acc[t][c] = the 32-K steps [k0, k1) of A_e's columns 16 c .. + 15 times the x
 // of token tile t. Each lane loads 16-byte pieces of the row of `token[t]` (place
 // lane / 4 of the tile) and of A's rows; an x piece is used by every column tile,
-// an A piece by every token tile.
-template <int CT, bool XB, int TT>
-__device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int (&token)[TT], int k0, int k1, int lane, v4f (&acc)[TT][CT]) {
+// an A piece by every token tile. AGAIN: where any_far says so, for an FP32 x.
+template <int CT, bool XB, int TT, bool AGAIN>
+__device__ __forceinline__ void low_steps_of(const AdapterArgs &a, int e, const int (&token)[TT], int k0, int k1, int lane, v4f (&acc)[TT][CT]) {
     const int lr = lane >> 2, lk = 8 * (lane & 3);           // row and columns that this lane loads
     size_t xrow[TT];
     const uint16_t *arow[CT];
@@ -151,14 +196,19 @@ __device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int
                 for (int c = 0; c < CT; ++c) {
                     const v4u b = to_operand(w[u][c], lane);
 #pragma unroll
-                    for (int t = 0; t < TT; ++t)
+                    for (int t = 0; t < TT; ++t) {
+                        if constexpr (AGAIN) {
+                            mfma_again(b, [&](int q) { return x[t][q]; }, false, acc[t][c]);
+                        } else {
 #pragma unroll
-                        for (int q = 2; q >= 0; --q) acc[t][c] = mfma_bf16(x[t][q], b, acc[t][c]);
+                            for (int q = 2; q >= 0; --q) acc[t][c] = mfma_bf16(x[t][q], b, acc[t][c]);
+                        }
+                    }
                 }
             }
         }
     };
-    constexpr int kSteps = CT * TT <= 2 ? 4 : CT <= 4 ? 2 : 1;
+    constexpr int kSteps = AGAIN ? 1 : CT * TT <= 2 ? 4 : CT <= 4 ? 2 : 1;
     int k = k0;
     for (; k + kSteps <= k1; k += kSteps) run(k, std::integral_constant<int, kSteps>{});
     if constexpr (kSteps > 2) {
@@ -167,8 +217,31 @@ __device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int
             k += 2;
         }
     }
+#pragma unroll 1
     for (; k < k1; ++k) run(k, std::integral_constant<int, 1>{});
 }
+
+template <int CT, bool XB, int TT>
+__device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int (&token)[TT], int k0, int k1, int lane, v4f (&acc)[TT][CT]) {
+    low_steps_of<CT, XB, TT, false>(a, e, token, k0, k1, lane, acc);
+    if constexpr (!XB) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            if (!any_far<1>(acc[t])) continue;
+            const int one[1] = {token[t]};
+            v4f sum[1][CT];
+            low_steps_of<CT, XB, 1, true>(a, e, one, k0, k1, lane, sum);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[t][c] = sum[0][c];
+        }
+    }
+}
+
+// Waves per SIMD that the registers are meant for, at most: no more than a
+// work-group of sixteen has where two chunks of FP32 x would be loaded in smaller
+// pieces for it (8,000 tokens of 12, K = 5120, M = 4096, r = 32 86.5 us, with the
+// compiler's own choice 92.4).
+constexpr int low_waves_most(int ct, int waves, bool xb, int tt) { return ct == 2 && waves == 16 && !xb && tt == 2 ? 4 : 8; }
 
 // low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
 // work-group takes 16 TT places of one adapter and part s, its WAVES waves
@@ -177,7 +250,8 @@ __device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int
 // launch's operand takes them. The places [p, p + 16) of adapter e are cut tile p
 // / 16 + e, a number of its own for each tile.
 template <int CT, int WAVES, bool XB, bool CUT, int TT>
-__global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
+__global__ __launch_bounds__(64 * WAVES)
+__attribute__((amdgpu_waves_per_eu(WAVES / 4, low_waves_most(CT, WAVES, XB, TT)))) void adapter_low_kernel(const AdapterArgs a) {
     __shared__ float part[WAVES - 1][CT][256];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -352,17 +426,20 @@ __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const Adapter
         }
         __syncthreads();
         if (!on) return;
+        // (MFMA c's rows of B, columns from k0 on)
+        auto load_b = [&](int k0, int c) {
+            const int k = k0 + 8 * (SPREAD ? lane & 3 : g);
+            v4u w = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(row(c, SPREAD ? lane >> 2 : n), a.M - 1)) * a.r + min(k, a.r - 8));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[x] = k < a.r ? w[x] : 0u;
+            return w;
+        };
         for (int k0 = 0; k0 < a.r; k0 += 32 * KC) {
             v4u b[KC][4];
 #pragma unroll
             for (int h = 0; h < KC; ++h)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int k = k0 + 32 * h + 8 * (SPREAD ? lane & 3 : g);
-                    const v4u w = *reinterpret_cast<const v4u *>(a.b + ((size_t)e * a.M + min(row(c, SPREAD ? lane >> 2 : n), a.M - 1)) * a.r + min(k, a.r - 8));
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) b[h][c][x] = k < a.r ? w[x] : 0u;
-                }
+                for (int c = 0; c < 4; ++c) b[h][c] = load_b(k0 + 32 * h, c);
 #pragma unroll
             for (int h = 0; h < KC; ++h) {
                 if (k0 + 32 * h >= a.r) break;
@@ -374,6 +451,19 @@ __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const Adapter
                     const v4u x = *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * pitch + k0 + 32 * h + 8 * g);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) acc[c] = mfma_bf16(b[h][c], x, acc[c]);
+                }
+            }
+        }
+        if (any_far<4>(acc)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int k0 = 0; k0 < a.r; k0 += 32) {
+                auto part = [&](int q) { return *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * pitch + k0 + 8 * g); };
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const v4u b = load_b(k0, c);
+                    mfma_again(SPREAD ? to_operand(b, lane) : b, part, true, acc[c]);
                 }
             }
         }
@@ -455,11 +545,19 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(const Adapt
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int x = 0; x < 4; ++x) b[c][x] = 8 * g < a.r ? b[c][x] : 0u;
+        v4u x[3];
 #pragma unroll
         for (int q = 2; q >= 0; --q) {
-            const v4u x = *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * PITCH + 8 * g);
+            x[q] = *reinterpret_cast<const v4u *>(cut + (q * kLowTile + n) * PITCH + 8 * g);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = mfma_bf16(b[c], x, acc[c]);
+            for (int c = 0; c < 4; ++c) acc[c] = mfma_bf16(b[c], x[q], acc[c]);
+        }
+        if (any_far<4>(acc)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                mfma_again(b[c], [&](int q) { return x[q]; }, true, acc[c]);
+            }
         }
     }
     if (!on || p0 + n >= p1) return;
@@ -570,6 +668,14 @@ __global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const Ada
                 for (int q = 2; q >= 0; --q)
 #pragma unroll
                     for (int c = 0; c < 8; ++c) acc[c] = mfma_bf16(x[h][q], b[h][c], acc[c]);
+            if (any_far<1>(acc)) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    acc[c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int h = 0; h < KC; ++h) mfma_again(b[h][c], [&](int q) { return x[h][q]; }, false, acc[c]);
+                }
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
