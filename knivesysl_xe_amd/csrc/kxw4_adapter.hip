@@ -339,9 +339,10 @@ constexpr int kUpWaves = 4, kUpRows = 64, kUpBlock = kUpWaves * kUpRows;
 __host__ __device__ constexpr int up_pitch(int r) { return 32 * chunks_of(r) + 8; }
 
 // out = y + acc for a lane's pieces of one token, rounded once; piece q's
-// outputs are acc[2 q], acc[2 q + 1] (BF16) or acc[q].
+// outputs are acc[2 q], acc[2 q + 1] (BF16) or acc[q]. Without `add` out = y, bit
+// for bit (-0 + 0 is another zero).
 template <int NY, bool YB, class Col>
-__device__ __forceinline__ void store_up(const AdapterArgs &a, size_t at, Col col, const v4u (&yv)[NY], const v4f (&acc)[4]) {
+__device__ __forceinline__ void store_up(const AdapterArgs &a, size_t at, Col col, const v4u (&yv)[NY], const v4f (&acc)[4], bool add) {
 #pragma unroll
     for (int q = 0; q < NY; ++q) {
         if (col(q) >= a.M) continue;
@@ -356,6 +357,7 @@ __device__ __forceinline__ void store_up(const AdapterArgs &a, size_t at, Col co
                 o[i] = __float_as_uint(__uint_as_float(yv[q][i]) + acc[q][i]);
             }
         }
+        if (!add) o = yv[q];
         *reinterpret_cast<v4u *>(static_cast<uint8_t *>(a.out) + (at + col(q)) * (YB ? 2 : 4)) = o;
     }
 }
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const Adapter
         }
     }
     if (!on || p0 + n >= p1) return;
-    store_up<NY, YB>(a, at, [&](int q) { return col(q); }, yv, acc);
+    store_up<NY, YB>(a, at, [&](int q) { return col(q); }, yv, acc, e >= 0);
 }
 
 // Both in one launch, for few tokens and small adapters: a work-group takes 16
@@ -561,7 +563,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(const Adapt
         }
     }
     if (!on || p0 + n >= p1) return;
-    store_up<NY, YB>(a, at, [&](int q) { return col(q); }, yv, acc);
+    store_up<NY, YB>(a, at, [&](int q) { return col(q); }, yv, acc, e >= 0);
 }
 
 // The same for many tokens. A wave takes 128 rows of B, whose operands stay in
@@ -692,6 +694,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void adapter_many_kernel(const Ada
                     else
                         o[j] = __float_as_uint(__uint_as_float(yv[i][q][j]) + acc[4 * q + j][i]);
                 }
+                if (e < 0) o = yv[i][q];
                 *reinterpret_cast<v4u *>(static_cast<uint8_t *>(a.out) + (at[i] + col(q)) * (YB ? 2 : 4)) = o;
             }
         }

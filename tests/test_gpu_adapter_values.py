@@ -1,6 +1,7 @@
 """Infinities among the weights of low-rank adapters (csrc/kxw4_adapter.hip): an
 output is the infinity or NaN that the definition gives in 64 bits, and those
-that no infinity reaches keep their bits."""
+that no infinity reaches keep their bits. Rows without an adapter are y, bit for
+bit."""
 import numpy as np
 import pytest
 import torch
@@ -95,3 +96,24 @@ def test_infinite_weights_and_inputs_and_padding():
                           ops.route_rows(ids.to(DEV), 2)).cpu()
     assert (got[[0, 1, 5, 8]] == INF).all() and (got[2] == -INF).all()
     assert (got[[3, 6]] == r * K).all() and (got[[4, 7]] == 0).all()
+
+
+@pytest.mark.parametrize("T,n,r,K,M", SIZES)
+@pytest.mark.parametrize("y_t", [torch.float32, torch.bfloat16])
+def test_rows_without_an_adapter_are_copied(T, n, r, K, M, y_t):
+    # any bit patterns: zeros of both signs, NaNs of every kind
+    bits = torch.int32 if y_t is torch.float32 else torch.int16
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(T)
+    y = torch.zeros(T, M, dtype=bits, device=DEV)
+    y.random_(-(1 << (8 * y.element_size() - 1)), (1 << (8 * y.element_size() - 1)) - 1, generator=gen)
+    y[:, ::3] = -(1 << (8 * y.element_size() - 1))                       # -0
+    y[:, 1::7] = 0x7F800001 if y_t is torch.float32 else 0x7F81
+    x = torch.randn(T, K, generator=gen, device=DEV)
+    ad = ops.Adapters(torch.randn(n, r, K, generator=gen, device=DEV).bfloat16(),
+                      torch.randn(n, M, r, generator=gen, device=DEV).bfloat16(), torch.ones(n, device=DEV))
+    ids = torch.randint(-1, n + 1, (T,), generator=gen, device=DEV)
+    none = (ids < 0) | (ids >= n)
+    none[0], ids[0] = True, -1
+    got = ops.adapter_add(y.view(y_t), x, ad, ops.route_rows(ids, n))
+    assert torch.equal(got.view(bits)[none], y[none])
