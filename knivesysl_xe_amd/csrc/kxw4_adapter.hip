@@ -17,7 +17,7 @@
 // A part that is zero makes a NaN of an infinity in A or B that the whole value
 // does not, so a wave whose sums are not finite works them out again, the second
 // and third parts times the finite elements alone (finite8). Looking for that
-// costs 0-2 %.
+// costs 0-2 %, 0.2 us of the shortest launches.
 //
 // v_mfma_f32_16x16x32_bf16: lane l supplies row (A) / column (B) l%16 and the
 // eight K slots 8*(l/16)..+7; result register i of lane l is row 4*(l/16)+i,
@@ -237,12 +237,6 @@ __device__ __forceinline__ void low_steps(const AdapterArgs &a, int e, const int
     }
 }
 
-// Waves per SIMD that the registers are meant for, at most: no more than a
-// work-group of sixteen has where two chunks of FP32 x would be loaded in smaller
-// pieces for it (8,000 tokens of 12, K = 5120, M = 4096, r = 32 86.5 us, with the
-// compiler's own choice 92.4).
-constexpr int low_waves_most(int ct, int waves, bool xb, int tt) { return ct == 2 && waves == 16 && !xb && tt == 2 ? 4 : 8; }
-
 // low[s][p][c] = sum over the s-th part of K of A[c][k] x[order[p]][k]: a
 // work-group takes 16 TT places of one adapter and part s, its WAVES waves
 // consecutive runs of 32-K steps, all r columns (CT tiles of 16). CUT: one part;
@@ -250,8 +244,7 @@ constexpr int low_waves_most(int ct, int waves, bool xb, int tt) { return ct == 
 // launch's operand takes them. The places [p, p + 16) of adapter e are cut tile p
 // / 16 + e, a number of its own for each tile.
 template <int CT, int WAVES, bool XB, bool CUT, int TT>
-__global__ __launch_bounds__(64 * WAVES)
-__attribute__((amdgpu_waves_per_eu(WAVES / 4, low_waves_most(CT, WAVES, XB, TT)))) void adapter_low_kernel(const AdapterArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void adapter_low_kernel(const AdapterArgs a) {
     __shared__ float part[WAVES - 1][CT][256];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -759,10 +752,11 @@ static int launch_one(const AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-template <int CT, int WAVES, bool CUT, int TT>
+// (WF: waves for an FP32 x)
+template <int CT, int WAVES, bool CUT, int TT, int WF = WAVES>
 static int launch_low(AdapterArgs &a, bool x_bf16, hipStream_t st) {
-    return launch_tiles(x_bf16 ? adapter_low_kernel<CT, WAVES, true, CUT, TT> : adapter_low_kernel<CT, WAVES, false, CUT, TT>, a,
-                        tiles_at_most(a.T, a.n, kLowTile * TT), 1, a.splits, 64 * WAVES, 0, st);
+    return launch_tiles(x_bf16 ? adapter_low_kernel<CT, WAVES, true, CUT, TT> : adapter_low_kernel<CT, WF, false, CUT, TT>, a,
+                        tiles_at_most(a.T, a.n, kLowTile * TT), 1, a.splits, 64 * (x_bf16 ? WAVES : WF), 0, st);
 }
 
 // The first launch for many tokens. One work-group of either takes about as long
@@ -770,11 +764,14 @@ static int launch_low(AdapterArgs &a, bool x_bf16, hipStream_t st) {
 // all of A, so two tiles, which share A, pay once there are more tiles than CUs
 // (us in all for one / two: 8,000 tokens of 12, K = 5120, M = 4096, r = 32 53.5 /
 // 48.8, r = 128 117 / 99, K = 12288, M = 1024, r = 64 71 / 58; 3,965 of 6, K =
-// 5120, r = 32 32 / 36).
+// 5120, r = 32 32 / 36). Two tiles of FP32 x at r = 32 take eight waves, whose
+// registers hold more loads (sixteen / eight: 9,000 tokens of 40, K = 5120, M =
+// 2560 112 / 105, 6,000 of 12, K = 2048, M = 4096 54.2 / 50.5, 12,000 of 6, K = M =
+// 5120 132 / 125).
 template <int TT>
 static int launch_cut(AdapterArgs &a, bool x_bf16, hipStream_t st) {
     if (a.r <= 16) return launch_low<1, 16, true, TT>(a, x_bf16, st);
-    if (a.r <= 32) return launch_low<2, 16, true, TT>(a, x_bf16, st);
+    if (a.r <= 32) return launch_low<2, 16, true, TT, TT == 2 ? 8 : 16>(a, x_bf16, st);
     if (a.r <= 64) return launch_low<4, 8, true, TT>(a, x_bf16, st);
     return launch_low<8, 8, true, TT>(a, x_bf16, st);
 }
