@@ -741,6 +741,14 @@ class Adapters:
                                self.scale.data_ptr())
 
 
+@functools.lru_cache(maxsize=4096)
+def _adapter_bytes(device: int, n: int, r: int, K: int, M: int, T: int) -> int:
+    """Scratch of adapter_add on a device (it goes by the CUs)."""
+    ad = _lib.AdapterSet(n, r, K, M)
+    with torch.cuda.device(device):
+        return lib().kxw4_adapter_workspace(C.byref(ad), T)
+
+
 def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: RowRoute, out=None) -> torch.Tensor:
     """y[t] + scale_e * b_e (a_e x[t]) for the adapter e of each token t (y[t]
     for a token without one): y [T][M] the projection's output and x [T][K] its
@@ -764,7 +772,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     _need(scale, "adapters.scale", torch.float32, (n,), dev)
     o = _need(out, "out", y.dtype, (T, M), dev) if out is not None else torch.empty_like(y)
     ref = C.byref(adapters.c())
-    nbytes = lib().kxw4_adapter_workspace(ref, T)
+    nbytes = _adapter_bytes(dev.index, n, r, K, M, T)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("kxw4_adapter_add", dev, y.data_ptr(), _dtype_code(y.dtype), x.data_ptr(), _dtype_code(x.dtype),
             ref, plan, o.data_ptr(), ws.data_ptr() if nbytes else None)

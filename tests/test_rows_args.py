@@ -263,3 +263,28 @@ def test_a_call_runs_on_its_tensors_device(monkeypatch):
     assert seen == [(0, (5, 100)), (1, (6, 101))] and current == [0]
     with pytest.raises(_lib.KxError, match="fails"):
         ops._launch("fails", torch.device("cuda:1"))
+
+
+def test_adapter_scratch_is_that_of_the_tensors_device(monkeypatch):
+    # (two launches or one go by the CUs of the current device)
+    import contextlib
+    current = [0]
+
+    @contextlib.contextmanager
+    def device(i):
+        before, current[0] = current[0], i
+        yield
+        current[0] = before
+
+    class Library:
+        @staticmethod
+        def kxw4_adapter_workspace(ad, T):
+            a = ad._obj
+            return 1000 * current[0] + T + a.n + a.r + a.K + a.M
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(ops, "lib", lambda: Library)
+    ops._adapter_bytes.cache_clear()
+    for i in (0, 3, 0):
+        assert ops._adapter_bytes(i, 2, 16, 128, 32, 5) == 1000 * i + 183 and current == [0]
+    ops._adapter_bytes.cache_clear()
