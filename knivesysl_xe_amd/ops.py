@@ -25,7 +25,10 @@ Rows with a weight of their own have no counterpart there (one dense model
 without adapters): route_rows sorts the rows of a batch by expert or adapter,
 dispatch_rows and combine_rows (with their gradients) move rows there and back,
 expert_gemm[_fanout] projects each by its expert, adapter_add adds a low-rank
-adapter per request to a projection's output.
+adapter per request to a projection's output. None of these calls records a
+gradient: dispatch_rows, combine_rows (the gradients of both are calls of their
+own) and adapter_add (which has none) refuse tensors that require grad unless
+gradients are off, as they are in a torch.autograd.Function.
 
 Torch provides device memory and the current stream only; every kernel is
 the HIP code in libkxw4.so, reached through ctypes. Tensors must live on a
@@ -523,6 +526,14 @@ def _launch(name: str, device: torch.device, *args) -> None:
         check(name, rc)
 
 
+def _detached(call: str) -> None:
+    """A tensor of `call` requires grad: refused while gradients are recorded,
+    since these calls record none and its own would be lost without a word."""
+    if torch.is_grad_enabled():
+        raise ValueError(f"{call} records no gradient, but one of its tensors requires grad: call it under "
+                         "torch.no_grad() or in the forward and backward of a torch.autograd.Function")
+
+
 _FLOATS = (torch.float32, torch.bfloat16)
 _IDS = (torch.int32, torch.int64)
 
@@ -556,8 +567,11 @@ class RowRoute:
     @classmethod
     def empty(cls, T: int, k: int, groups: int, device="cuda") -> "RowRoute":
         i32 = torch.int32
-        return cls(T, k, groups, torch.empty(groups + 1, dtype=i32, device=device),
-                   torch.empty(T * k, dtype=i32, device=device), torch.empty(T, k, dtype=i32, device=device))
+        r = cls.__new__(cls)                                 # (past the setters of a frozen class, a microsecond)
+        r.__dict__.update(T=T, k=k, groups=groups, offsets=torch.empty(groups + 1, dtype=i32, device=device),
+                          order=torch.empty(T * k, dtype=i32, device=device),
+                          position=torch.empty(T, k, dtype=i32, device=device))
+        return r
 
 
 def _plan(r: RowRoute, device):
@@ -572,8 +586,9 @@ def _plan(r: RowRoute, device):
 
 
 def _make_plan(r: RowRoute, device):
-    ref = C.byref(r.c())
-    r.__dict__["_made"] = (device, r.at(), ref)
+    at = r.at()
+    ref = C.byref(_lib.Route(r.T, r.k, r.groups, *at))
+    r.__dict__["_made"] = (device, at, ref)
     return ref
 
 
@@ -629,11 +644,14 @@ def dispatch_rows(x: torch.Tensor, route: RowRoute, out=None) -> torch.Tensor:
     if x.dim() != 2:
         raise ValueError("x must have shape (T, H)")
     T, H = x.shape
-    _need(x, "x", _FLOATS, (route.T, H), dev)
+    if T != route.T or x.dtype not in _FLOATS or not x.is_contiguous():
+        _need(x, "x", _FLOATS, (route.T, H), dev)
     N = route.T * route.k
     rows = _need(out, "out", x.dtype, (N, H), dev) if out is not None else torch.empty(N, H, dtype=x.dtype, device=dev)
+    if x.requires_grad or rows.requires_grad:
+        _detached("dispatch_rows")
     if N:
-        _launch("kxw4_dispatch_rows", dev, x.data_ptr(), _dtype_code(x.dtype), H, plan, rows.data_ptr())
+        _launch("kxw4_dispatch_rows", dev, x.data_ptr(), _DTYPE_CODES[x.dtype], H, plan, rows.data_ptr())
     return rows
 
 
@@ -646,14 +664,17 @@ def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Te
     plan = _plan(route, dev)
     if rows.dim() != 2:
         raise ValueError("rows must have shape (T*k, H)")
-    H = rows.shape[1]
-    _need(rows, "rows", _FLOATS, (route.T * route.k, H), dev)
+    N, H = rows.shape
+    if N != route.T * route.k or rows.dtype not in _FLOATS or not rows.is_contiguous():
+        _need(rows, "rows", _FLOATS, (route.T * route.k, H), dev)
     if weights is not None:
         _need(weights, "weights", torch.float32, (route.T, route.k), dev)
     y = _out(route.T, H, dtype or (out.dtype if out is not None else rows.dtype), dev, out)
+    if rows.requires_grad or (weights is not None and weights.requires_grad) or y.requires_grad:
+        _detached("combine_rows")
     if route.T:
-        _launch("kxw4_combine_rows", dev, rows.data_ptr(), _dtype_code(rows.dtype), H,
-                None if weights is None else weights.data_ptr(), plan, y.data_ptr(), _dtype_code(y.dtype))
+        _launch("kxw4_combine_rows", dev, rows.data_ptr(), _DTYPE_CODES[rows.dtype], H,
+                None if weights is None else weights.data_ptr(), plan, y.data_ptr(), _DTYPE_CODES[y.dtype])
     return y
 
 
@@ -670,10 +691,12 @@ def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, route: RowRoute,
     _need(dy, "dy", _FLOATS, (route.T, H), dev)
     _need(weights, "weights", torch.float32, (route.T, route.k), dev)
     drows = _need(out, "out", rows.dtype, (N, H), dev) if out is not None else torch.empty_like(rows)
+    if dy.requires_grad or rows.requires_grad or weights.requires_grad or drows.requires_grad:
+        _detached("combine_rows_backward")
     dweights = torch.empty(route.T, route.k, dtype=torch.float32, device=dev)
     if N:
-        _launch("kxw4_combine_rows_backward", dev, dy.data_ptr(), _dtype_code(dy.dtype), rows.data_ptr(),
-                _dtype_code(rows.dtype), H, weights.data_ptr(), plan, drows.data_ptr(), dweights.data_ptr())
+        _launch("kxw4_combine_rows_backward", dev, dy.data_ptr(), _DTYPE_CODES[dy.dtype], rows.data_ptr(),
+                _DTYPE_CODES[rows.dtype], H, weights.data_ptr(), plan, drows.data_ptr(), dweights.data_ptr())
     return drows, dweights
 
 
@@ -765,16 +788,20 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     if route.groups != n or route.k != 1:
         raise ValueError(f"the plan has {route.groups} groups and k {route.k} for {n} adapters")
     T = route.T
-    _need(y, "y", _FLOATS, (T, M), dev)
+    if y.shape != (T, M) or y.dtype not in _FLOATS or not y.is_contiguous():
+        _need(y, "y", _FLOATS, (T, M), dev)
     _need(x, "x", _FLOATS, (T, K), dev)
     _need(a, "adapters.a", torch.bfloat16, sa, dev)
     _need(b, "adapters.b", torch.bfloat16, (n, M, r), dev)
     _need(scale, "adapters.scale", torch.float32, (n,), dev)
     o = _need(out, "out", y.dtype, (T, M), dev) if out is not None else torch.empty_like(y)
+    if (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad or scale.requires_grad
+            or o.requires_grad):
+        _detached("adapter_add")
     ref = C.byref(adapters.c())
     nbytes = _adapter_bytes(dev.index, n, r, K, M, T)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch("kxw4_adapter_add", dev, y.data_ptr(), _dtype_code(y.dtype), x.data_ptr(), _dtype_code(x.dtype),
+    _launch("kxw4_adapter_add", dev, y.data_ptr(), _DTYPE_CODES[y.dtype], x.data_ptr(), _DTYPE_CODES[x.dtype],
             ref, plan, o.data_ptr(), ws.data_ptr() if nbytes else None)
     return o
 
