@@ -714,12 +714,18 @@ static int adapter_splits(int n, int T, int K) {
 }
 
 // One launch, while a work-group's waves have at most ten 32-K steps of one
-// column tile each and every CU at most one work-group: the host's second
-// launch costs more than what the GPU loses (us two launches / one, called in
-// turn; replayed from a graph: 1 to 8 tokens of as many adapters, K = M = 5120, r
-// = 16 14.2 / 10.1; 7.1 / 7.8; 64 of 64, 4,096 14.3 / 9.9; 8.4 / 8.1; 4 of 4, K =
-// 1024, M = 4096, float32 14.3 / 10.0; 8.0 / 6.1; 16 of 16, K = 17408 14.2 / 16.7;
-// 8.4 / 17.4; 200 of 100, r = 32 21.4 / 39.1).
+// column tile each and every CU at most one work-group: the host's second launch
+// costs more than what the GPU loses. Both sides, us two launches / one, 8 tokens
+// of 8, r = 16, M = 5120 (1 token, 32 of 16, and M = 1024 within 0.8 of these):
+//   K                       1,024      2,560      4,096      5,120      6,144      8,192
+//   BF16 called in turn   13.2/9.3   13.2/9.2   13.1/9.3   13.2/9.1   13.0/9.2   13.1/9.7
+//   BF16 from a graph      6.9/5.0    6.8/6.0    6.8/7.0    7.0/7.7    7.0/8.4    7.2/9.6
+//   FP32 called in turn   13.2/9.3   13.2/9.1   13.2/10.6  13.2/11.9  13.2/13.5  13.2/16.2
+//   FP32 from a graph      7.8/6.1    7.8/8.4    7.8/10.6   8.2/12.0   8.5/13.6   9.2/16.3
+// So the line is where FP32 calls stop gaining; a graph's replays would have it at
+// 2,000 to 4,000. At r = 32 half the K: BF16 2,560 13.2/9.2 and 7.2/7.1, 4,096
+// 13.2/9.2 and 7.2/8.8, FP32 2,560 13.2/10.1 and 8.5/10.1. 200 tokens of 100, r =
+// 32 21.4/39.1 in turn.
 static bool one_launch(int n, int T, int r, int K, int M) {
     const long long groups = (tiles_at_most(T, n, kLowTile) + 1) * ((M + kOneBlock - 1) / kOneBlock);
     return (long long)(r + 15) / 16 * K <= 5120 && r <= 32 && groups <= device_cus();

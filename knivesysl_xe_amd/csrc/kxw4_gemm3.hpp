@@ -697,9 +697,9 @@ __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void gemm3_kernel(const GemmArgs 
     gemm3_tile<TA, TB, WMW, WNW, UNIT, NST, OCC, XB, false>(a, tt * G3Shape<TA, TB, WMW, WNW, UNIT, XB>::BM, a.T, ntg, 0);
 }
 
-// The same over grouped rows, with one wave row: a tile of 128 places of one
-// group. The last tile of a group runs on the 64 or 32 places' worth of blocks
-// that hold its rows.
+// The same over grouped rows, with one wave row: a tile of 32 TA places of one
+// group. The last tile of a group runs on the half or quarter of its blocks that
+// holds its rows.
 template <int TA, int TB, int WNW, int UNIT, int NST, int OCC>
 __global__ __launch_bounds__(64 * WNW)
 __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void gemm3_group_kernel(const GemmArgs a) {
