@@ -294,8 +294,8 @@ size_t kxw4_route_workspace(int T, int k, int groups);
 int kxw4_route_rows(const void *ids, int ids_64, const kxw4_route_t *route, void *workspace, void *stream);
 
 /* rows[p] = x[order[p] / k] for the places of a group. x [T][H], rows [N][H]
- * of one type (KXW4_F32, KXW4_BF16); any H, and any alignment of the type's
- * own size. The gradient of x is kxw4_combine_rows without weights. */
+ * of one type (KXW4_F32, KXW4_BF16); any H up to 2^28, and any alignment of the
+ * type's own size. The gradient of x is kxw4_combine_rows without weights. */
 int kxw4_dispatch_rows(const void *x, int dtype, int H, const kxw4_route_t *route, void *rows, void *stream);
 
 /* y[t] = sum over j of weights[t][j] * rows[position[t][j]] (weights NULL: all
@@ -306,7 +306,7 @@ int kxw4_combine_rows(const void *rows, int rows_dtype, int H, const float *weig
 
 /* The gradient of kxw4_combine_rows: drows[position[t][j]] = weights[t][j] *
  * dy[t] (of rows' type), dweights[t][j] = <dy[t], rows[position[t][j]]> in
- * FP32, 0 for a slot without a group. */
+ * FP32, 0 for a slot without a group. k up to 2^26 - 4. */
 int kxw4_combine_rows_backward(const void *dy, int dy_dtype, const void *rows, int rows_dtype, int H,
                                const float *weights, const kxw4_route_t *route, void *drows, float *dweights,
                                void *stream);
@@ -334,8 +334,9 @@ int kxw4_expert_gemm(const kxw4_weight_t *const *ws, void *const *ys, int count,
  * Products are exact and summed in FP32, A x is held in FP32, out is rounded
  * once. K % 128 == 0, M % 16 == 0 (as the projection's weight), r a multiple
  * of 8 up to 256 (pad smaller ranks with zeros); 16-byte aligned pointers.
- * workspace: kxw4_adapter_workspace bytes (then it may be NULL when that is 0),
- * this call's own while it runs. */
+ * workspace: kxw4_adapter_workspace bytes (then it may be NULL when that is 0;
+ * asked with the call's device current, whose CUs it goes by), this call's own
+ * while it runs. */
 typedef struct kxw4_adapters {
     int32_t n, r, K, M;
     const uint16_t *a, *b;

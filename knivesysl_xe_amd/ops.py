@@ -534,6 +534,8 @@ def _detached(call: str) -> None:
                          "torch.no_grad() or in the forward and backward of a torch.autograd.Function")
 
 
+# (the C calls take 32-bit sizes, and ctypes cuts a longer one to that unseen)
+_MAX_SLOTS, _MAX_H = 1 << 30, 1 << 28
 _FLOATS = (torch.float32, torch.bfloat16)
 _IDS = (torch.int32, torch.int64)
 
@@ -619,6 +621,8 @@ def route_rows(ids: torch.Tensor, groups: int, out: Optional[RowRoute] = None) -
     if ids.dtype not in _IDS or not ids.is_contiguous():
         _need(ids, "ids", _IDS, shape, dev)
     T, k = shape if len(shape) == 2 else (shape[0], 1)
+    if T * k > _MAX_SLOTS or k > _MAX_SLOTS:
+        raise ValueError(f"a plan holds up to 2^30 slots, got {T} x {k}")
     if not 1 <= groups <= 1024:
         raise ValueError(f"groups must be 1 to 1024, got {groups}")
     if out is not None:
@@ -644,6 +648,8 @@ def dispatch_rows(x: torch.Tensor, route: RowRoute, out=None) -> torch.Tensor:
     if x.dim() != 2:
         raise ValueError("x must have shape (T, H)")
     T, H = x.shape
+    if H > _MAX_H:
+        raise ValueError(f"rows have up to 2^28 elements, got {H}")
     if T != route.T or x.dtype not in _FLOATS or not x.is_contiguous():
         _need(x, "x", _FLOATS, (route.T, H), dev)
     N = route.T * route.k
@@ -665,6 +671,8 @@ def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Te
     if rows.dim() != 2:
         raise ValueError("rows must have shape (T*k, H)")
     N, H = rows.shape
+    if H > _MAX_H:
+        raise ValueError(f"rows have up to 2^28 elements, got {H}")
     if N != route.T * route.k or rows.dtype not in _FLOATS or not rows.is_contiguous():
         _need(rows, "rows", _FLOATS, (route.T * route.k, H), dev)
     if weights is not None:
@@ -687,6 +695,8 @@ def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, route: RowRoute,
     if rows.dim() != 2:
         raise ValueError("rows must have shape (T*k, H)")
     N, H = route.T * route.k, rows.shape[1]
+    if H > _MAX_H:
+        raise ValueError(f"rows have up to 2^28 elements, got {H}")
     _need(rows, "rows", _FLOATS, (N, H), dev)
     _need(dy, "dy", _FLOATS, (route.T, H), dev)
     _need(weights, "weights", torch.float32, (route.T, route.k), dev)
@@ -785,6 +795,8 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
         raise ValueError("adapters must have shapes (n, r, K) and (n, M, r)")
     n, r, K = sa
     M = sb[1]
+    if (r | K | M) >> 31:
+        raise ValueError(f"adapters of r {r}, K {K}, M {M}: a size past 31 bits")
     if route.groups != n or route.k != 1:
         raise ValueError(f"the plan has {route.groups} groups and k {route.k} for {n} adapters")
     T = route.T

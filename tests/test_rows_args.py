@@ -288,3 +288,28 @@ def test_adapter_scratch_is_that_of_the_tensors_device(monkeypatch):
     for i in (0, 3, 0):
         assert ops._adapter_bytes(i, 2, 16, 128, 32, 5) == 1000 * i + 183 and current == [0]
     ops._adapter_bytes.cache_clear()
+
+
+def test_sizes_past_32_bits_are_refused(monkeypatch):
+    # (tensors without memory; a call that went on would reach the launch)
+    monkeypatch.setattr(ops, "_gpu", lambda t, name: t.device)
+    monkeypatch.setattr(ops, "_launch", lambda *args: pytest.fail("launched"))
+    monkeypatch.setattr(ops, "_adapter_bytes", lambda *args: 0)
+    meta = torch.device("meta")
+
+    def empty(*shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device=meta)
+
+    for shape in ((1 << 32,), ((1 << 30) + 1, 1), (2, 1 << 32), (1 << 32, 2), (0, 1 << 32)):
+        with pytest.raises(ValueError, match="up to 2\\^30 slots"):
+            ops.route_rows(empty(*shape, dtype=torch.int32), 4)
+    H = (1 << 32) + 64
+    r = ops.RowRoute.empty(2, 1, 4, meta)
+    for call in (lambda: ops.dispatch_rows(empty(2, H), r), lambda: ops.combine_rows(empty(2, H), r),
+                 lambda: ops.combine_rows_backward(empty(2, H), empty(2, H), r, empty(2, 1))):
+        with pytest.raises(ValueError, match="up to 2\\^28 elements"):
+            call()
+    for K, M in ((H, 64), (128, H)):
+        ad = ops.Adapters(empty(4, 8, K, dtype=torch.bfloat16), empty(4, M, 8, dtype=torch.bfloat16), empty(4))
+        with pytest.raises(ValueError, match="past 31 bits"):
+            ops.adapter_add(empty(2, M), empty(2, K), ad, r)
