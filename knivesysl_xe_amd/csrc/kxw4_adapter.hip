@@ -356,9 +356,9 @@ __device__ __forceinline__ void store_up(const AdapterArgs &a, size_t at, Col co
 }
 
 // KC: 32-column chunks of B requested together; from two on a row of B is long
-// enough for the loads of to_operand (1,500 tokens of 8, K = 5120, M = 8192, r =
-// 128 56.5 / 49.5 us, r = 64 35.9 / 32.3; r = 32 stays at 24, 250 tokens 9.2 /
-// 9.5).
+// enough for the loads of to_operand (us in all for KC = 1 / 2, 1,500 tokens of 8,
+// all in use, K = 5120, M = 8192, r = 128 70.0 / 63.0, r = 64 39.8 / 36.0; r = 32
+// 26.8 / 26.7, 250 tokens 9.7 / 10.1).
 template <int KC, bool YB>
 __global__ __launch_bounds__(64 * kUpWaves) void adapter_up_kernel(const AdapterArgs a) {
     constexpr int NY = YB ? 2 : 4;                           // 16-byte pieces of a lane's 16 outputs
@@ -768,9 +768,9 @@ static int launch_low(AdapterArgs &a, bool x_bf16, hipStream_t st) {
 // The first launch for many tokens. One work-group of either takes about as long
 // as it has bytes to fetch through its CU's L1 (24 a clock): x of its tokens and
 // all of A, so two tiles, which share A, pay once there are more tiles than CUs
-// (us in all for one / two: 8,000 tokens of 12, K = 5120, M = 4096, r = 32 53.5 /
-// 48.8, r = 128 117 / 99, K = 12288, M = 1024, r = 64 71 / 58; 3,965 of 6, K =
-// 5120, r = 32 32 / 36). Two tiles of FP32 x at r = 32 take eight waves, whose
+// (us in all for one / two, all adapters in use: 8,000 tokens of 12, K = 5120, M =
+// 4096, r = 32 51.8 / 47.9, but r = 128 121 / 128; 21,000 of 12, K = 12288, M =
+// 1024, r = 64 261 / 205; 3,965 of 6, K = 5120, M = 17408, r = 32 77 / 83). Two tiles of FP32 x at r = 32 take eight waves, whose
 // registers hold more loads (sixteen / eight: 9,000 tokens of 40, K = 5120, M =
 // 2560 112 / 105, 6,000 of 12, K = 2048, M = 4096 54.2 / 50.5, 12,000 of 6, K = M =
 // 5120 132 / 125).
@@ -811,9 +811,11 @@ int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st) {
     if (one_launch(a.n, a.T, a.r, a.K, a.M)) return a.r <= 16 ? launch_one<1>(a, x_bf16, y_bf16, st) : launch_one<2>(a, x_bf16, y_bf16, st);
     a.splits = adapter_splits(a.n, a.T, a.K);
     // Two token tiles share A where many tiles read a long one (us in all for
-    // one / two: 2,520 tokens of 24, M = 1024, K = 12288, r = 128 70.4 / 49.6, r =
-    // 64 37.8 / 31.0; 1,536 of 8 48.3 / 40.0, M = 4096, K = 5120 40.1 / 38.6; K =
-    // 2048 25.2 / 26.9; 1,100 of 2, K = 5120 33.2 / 34.5; r = 16 alike).
+    // one / two, all adapters in use: 2,520 tokens of 24, M = 1024, K = 12288, r =
+    // 128 171 / 96, r = 64 67.1 / 47.5; 1,536 of 8, r = 128 83.0 / 62.0, M = 4096, K
+    // = 5120 52.6 / 48.4; K = 2048 32.2 / 33.4; 1,100 of 2, K = 5120 33.3 / 34.6;
+    // r = 16 alike. Below 1,536 tokens M decides too: 1,500 of 8, K = 5120, M =
+    // 8192, r = 128 63.0 / 56.0).
     const bool two = a.T >= 1536 && a.K >= 4096;
     int rc;
     if (a.r <= 16) rc = launch_low<1, kFewWaves, false, 1>(a, x_bf16, st);
