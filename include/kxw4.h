@@ -346,6 +346,101 @@ size_t kxw4_adapter_workspace(const kxw4_adapters_t *adapters, int T);
 int kxw4_adapter_add(const void *y, int y_dtype, const void *x, int x_dtype, const kxw4_adapters_t *adapters,
                      const kxw4_route_t *route, void *out, void *workspace, void *stream);
 
+/* ---- the 8-bit floating tier ----------------------------------------------
+ * No counterpart in the reference, whose tiers are integer. Weights and rows
+ * are e4m3 codes (1 sign, 4 exponent, 3 mantissa bits, no infinities) with an
+ * FP32 scale for each block of 128: 128 x 128 of a weight, 128 columns of one
+ * row of activations. M and K are multiples of 16, up to 2^22; the last block
+ * of either may be shorter.
+ *
+ *   y[t][m] = sum over blocks j of P_j * (sx[t][j] * sw[m / 128][j]),
+ *   P_j = sum over the columns k of block j of q[t][k] * c[m][k]
+ *
+ * added up over j in FP32. The products of a P_j are exact and summed in FP32
+ * where the output is FP32 or the rows are few; with BF16 outputs and many
+ * rows the matrix core cuts each to 2^-13 of the largest power of two among
+ * eight neighbouring columns' products, which is far below a BF16 rounding.
+ *
+ * A weight stacks `groups` of M rows and K columns (1: one projection; the
+ * experts of a plan).
+ *   codes : kxw4_f8_code_bytes(groups, M, K) bytes in tiles of 16 rows x 128
+ *           columns, 2,048 bytes, tile (g, rg, kb) at ((g*(M/16) + rg) *
+ *           ceil(K/128) + kb)*2048; byte 1024h + 16l + b holds row l%16 and
+ *           column kb*128 + 64h + 16(l/16) + b. Columns past K are 0.
+ *   scales: [groups][ceil(M/128)][ceil(K/128)] */
+typedef struct kxw4_weight_f8 {
+    int32_t groups, M, K;
+    const uint8_t *codes;
+    const float *scales;
+} kxw4_weight_f8_t;
+
+/* Rows of activations: codes (kxw4_quantize_act_f8), or with q NULL the values
+ * x [T][K] of x_dtype, which the call quantizes.
+ *   q     : [T][128 * ceil(K/128)], columns past K are 0
+ *   scale : [ceil(K/128)][T] */
+typedef struct kxw4_act_f8 {
+    int32_t T, K, x_dtype;
+    const uint8_t *q;
+    const float *scale;
+    const void *x;
+} kxw4_act_f8_t;
+
+size_t kxw4_f8_code_bytes(int groups, int M, int K);
+
+/* Codes [groups][M][K] in their order <-> the tiles (scales have one order). */
+int kxw4_pack_weight_f8(const uint8_t *codes, int groups, int M, int K, uint8_t *out_codes, void *stream);
+int kxw4_unpack_weight_f8(const kxw4_weight_f8_t *w, uint8_t *codes, void *stream);
+
+/* w [groups][M][K] (KXW4_F32 or KXW4_BF16) -> codes and scales, by the rule of
+ * kxw4_quantize_act_f8 over blocks of 128 x 128. */
+int kxw4_quantize_weight_f8(const void *w, int dtype, int groups, int M, int K, uint8_t *out_codes,
+                            float *out_scales, void *stream);
+
+/* The transposed weight ([groups] of K rows and M columns), the same values: the
+ * gradient of a projection's input is the product of dy's rows with it.
+ * out_codes: kxw4_f8_code_bytes(groups, K, M). */
+int kxw4_transpose_weight_f8(const kxw4_weight_f8_t *w, uint8_t *out_codes, float *out_scales, void *stream);
+
+/* x[T][K] -> q, scale: top = max(max |x|, 2^-100) of a block, scale = top / 448,
+ * q = e4m3(x * (448 / top)) to nearest even, in FP32 with one rounding an
+ * operation. A NaN or an infinity makes a NaN code: products of that row are
+ * NaN. T may be 0. */
+int kxw4_quantize_act_f8(const void *x, int x_dtype, int T, int K, uint8_t *q, float *scale, void *stream);
+
+/* silu(gate) * up of [T][K] rows of one type, in FP32, quantized; the values to
+ * out[T][K] (may be NULL). */
+int kxw4_silu_mul_quant_f8(float *out, const void *gate, const void *up, int dtype, int T, int K, uint8_t *q,
+                           float *scale, void *stream);
+
+/* y[T][M] = the product (+ FP32 residual[T][M]) for up to 4 weights of one K
+ * and groups = 1 over one activation. T may be 0. workspace:
+ * kxw4_gemm_f8_workspace bytes (asked with the call's device current; then it
+ * may be NULL when that is 0), the call's own while it runs. 16-byte aligned
+ * pointers (4 for scales). */
+size_t kxw4_gemm_f8_workspace(const kxw4_weight_f8_t *const *ws, int count, const kxw4_act_f8_t *a, int y_dtype);
+int kxw4_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a, int y_dtype,
+                 const float *residual, void *workspace, void *stream);
+
+/* The experts' products over a plan, as kxw4_expert_gemm: ys[i] [N][M] in the
+ * plan's order, written up to offsets[groups]; a holds T rows, or with
+ * sorted_rows N rows in the plan's order. a's rows * 128 ceil(K/128) < 2^31; -2
+ * too where the launch would take 2^32 threads. */
+size_t kxw4_expert_gemm_f8_workspace(const kxw4_weight_f8_t *const *ws, int count, const kxw4_act_f8_t *a,
+                                     const kxw4_route_t *route, int sorted_rows, int y_dtype);
+int kxw4_expert_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a,
+                        const kxw4_route_t *route, int sorted_rows, int y_dtype, void *workspace, void *stream);
+
+/* The gradient of a weight: dw[g][m][k] = sum over the rows p of group g of
+ * dy[p][m] * x[p][k] (+ add, of dw's type, which may be dw itself). dy [N][M]
+ * and x [N][K] BF16 in the plan's order, N = T*k (rows past offsets[groups] are
+ * not read); without a plan one group of all N rows. Products are exact, sums
+ * FP32, dw [groups][M][K] of dw_dtype is rounded once. A group without rows has
+ * 0 (+ add). M and K multiples of 16 up to 2^22; N may be 0. Workspace as
+ * above. */
+size_t kxw4_grad_weight_workspace(int N, int groups, int M, int K);
+int kxw4_grad_weight(const uint16_t *dy, const uint16_t *x, int N, int M, int K, const kxw4_route_t *route,
+                     const void *add, void *dw, int dw_dtype, void *workspace, void *stream);
+
 /* No counterpart in the reference. For callers that cannot allocate (code
  * under HIP graph capture, tight serving loops): x[T][K] (KXW4_F32 or
  * KXW4_BF16) is quantized per K32 block into a fixed device array of this

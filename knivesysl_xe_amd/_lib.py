@@ -43,12 +43,24 @@ class AdapterSet(C.Structure):
                 ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p)]
 
 
+class WeightF8(C.Structure):
+    _fields_ = [("groups", C.c_int32), ("M", C.c_int32), ("K", C.c_int32),
+                ("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class ActF8(C.Structure):
+    _fields_ = [("T", C.c_int32), ("K", C.c_int32), ("x_dtype", C.c_int32),
+                ("q", C.c_void_p), ("scale", C.c_void_p), ("x", C.c_void_p)]
+
+
 # name -> (restype, argtypes); the exported C ABI, in header order
 P, I, F = C.c_void_p, C.c_int, C.c_float
 WP = C.POINTER(Weight)
 AP = C.POINTER(Act)
 RP = C.POINTER(Route)
 DP = C.POINTER(AdapterSet)
+FP = C.POINTER(WeightF8)
+QP = C.POINTER(ActF8)
 SIGNATURES = {
     "kxw4_abi_version": (I, []),
     "kxw4_error_string": (C.c_char_p, [I]),
@@ -81,6 +93,19 @@ SIGNATURES = {
     "kxw4_expert_gemm": (I, [C.POINTER(WP), C.POINTER(P), I, AP, RP, I, I, P]),
     "kxw4_adapter_workspace": (C.c_size_t, [DP, I]),
     "kxw4_adapter_add": (I, [P, I, P, I, DP, RP, P, P, P]),
+    "kxw4_f8_code_bytes": (C.c_size_t, [I, I, I]),
+    "kxw4_pack_weight_f8": (I, [P, I, I, I, P, P]),
+    "kxw4_unpack_weight_f8": (I, [FP, P, P]),
+    "kxw4_quantize_weight_f8": (I, [P, I, I, I, I, P, P, P]),
+    "kxw4_transpose_weight_f8": (I, [FP, P, P, P]),
+    "kxw4_quantize_act_f8": (I, [P, I, I, I, P, P, P]),
+    "kxw4_silu_mul_quant_f8": (I, [P, P, P, I, I, I, P, P, P]),
+    "kxw4_gemm_f8_workspace": (C.c_size_t, [C.POINTER(FP), I, QP, I]),
+    "kxw4_gemm_f8": (I, [C.POINTER(FP), C.POINTER(P), I, QP, I, P, P, P]),
+    "kxw4_expert_gemm_f8_workspace": (C.c_size_t, [C.POINTER(FP), I, QP, RP, I, I]),
+    "kxw4_expert_gemm_f8": (I, [C.POINTER(FP), C.POINTER(P), I, QP, RP, I, I, P, P]),
+    "kxw4_grad_weight_workspace": (C.c_size_t, [I, I, I, I]),
+    "kxw4_grad_weight": (I, [P, P, I, I, I, RP, P, P, I, P, P]),
     "kxw4_gemv_x_noalloc": (I, [WP, P, I, I, P, I, P, P]),
     "kxw4_tqf_open": (I, [C.c_char_p, C.POINTER(P)]),
     "kxw4_tqf_close": (None, [P]),

@@ -2,6 +2,7 @@
 // argument checks with the reference's return codes, split plans, and
 // dispatch to the kernels.
 #include "../../include/kxw4.h"
+#include "kxw4_checks.hpp"
 #include "kxw4_internal.hpp"
 
 #include <algorithm>
@@ -69,8 +70,6 @@ const Options &options() { return mutable_options(); }
 }  // namespace kxw4
 
 namespace {
-
-hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
 // 16 is the K16 tier (FP16|zp scales, GEMV only)
 bool valid_group(int g) { return g == 16 || g == 32 || g == 64 || g == 128; }
@@ -216,31 +215,11 @@ int decode_uniform(const kxw4_weight_t *const *ws, void *const *ys, int count,
 
 // ---- rows with a weight of their own -----------------------------------------
 
-bool valid_dtype(int d) { return d == KXW4_F32 || d == KXW4_BF16; }
-bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-
-constexpr int kMaxGroups = 1024;
-constexpr long long kMaxSlots = 1ll << 30;
-
-bool valid_plan(int T, int k, int groups) {
-    return T >= 0 && k > 0 && groups > 0 && groups <= kMaxGroups && (long long)T * k <= kMaxSlots;
-}
-
-// A plan that kxw4_route_rows filled. (With T = 0 only its sizes count.)
-int check_route(const kxw4_route_t *r) {
-    if (!r) return KXW4_EARG;
-    if (!valid_plan(r->T, r->k, r->groups)) return KXW4_ESHAPE;
-    if (r->T > 0 && (!r->offsets || !r->order || !r->position)) return KXW4_EPREP;
-    return KXW4_OK;
-}
-
 int check_rows(const kxw4_route_t *r, int H) {
     const int rc = check_route(r);
     if (rc) return rc;
     return H <= 0 || H > (1 << 28) ? KXW4_ESHAPE : KXW4_OK;
 }
-
-int elem_bytes(int dtype) { return dtype == KXW4_BF16 ? 2 : 4; }
 
 }  // namespace
 

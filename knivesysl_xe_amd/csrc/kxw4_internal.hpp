@@ -233,6 +233,71 @@ struct AdapterArgs {
 size_t adapter_scratch(int n, int T, int r, int K, int M);      // bytes of `low`
 int launch_adapter(AdapterArgs &a, bool x_bf16, bool y_bf16, hipStream_t st);
 
+// The 8-bit floating tier (kxw4_f8.hpp): codes in tiles, scales of 128 x 128
+// blocks, M and K multiples of 16.
+int launch_f8_quantize(const void *x, bool bf16, int T, int K, uint8_t *q, float *scale, hipStream_t st);
+int launch_f8_silu_mul(float *out, const void *gate, const void *up, bool bf16, int T, int K, uint8_t *q, float *scale,
+                       hipStream_t st);
+int launch_f8_pack(const uint8_t *codes, int groups, int M, int K, uint8_t *out, hipStream_t st);
+int launch_f8_unpack(const uint8_t *tiles, int groups, int M, int K, uint8_t *codes, hipStream_t st);
+int launch_f8_weight(const void *w, bool bf16, int groups, int M, int K, uint8_t *codes, float *scales, hipStream_t st);
+int launch_f8_transpose(const uint8_t *tiles, const float *scales, int groups, int M, int K, uint8_t *out, float *out_scales,
+                        hipStream_t st);
+
+struct F8StreamWeight {
+    const uint8_t *codes;
+    const float *scales;
+    void *y;
+    int M, blk;                       // blk: first row block (set by the launcher)
+};
+struct F8StreamArgs {
+    F8StreamWeight w[kMaxWeights];
+    int count;
+    const uint8_t *q;                 // codes [rows][128 KB] and scales [KB][rows], or x
+    const float *sx;
+    const void *x;
+    const float *residual;
+    int rows, K, KB, y_bf16;
+    // rows sorted by group, as in ExpertArgs (groups 0: one weight for all)
+    const int *offsets, *order;
+    int N, groups, k;
+    int row_blocks;                   // (set by the launcher)
+};
+int launch_f8_stream(F8StreamArgs &a, int x, hipStream_t st);
+
+struct F8GemmWeight {
+    const uint8_t *codes;
+    const float *scales;
+    void *y;
+    int M, nt_begin;                  // nt_begin: first weight tile (set by the launcher)
+};
+struct F8GemmArgs {
+    F8GemmWeight w[kMaxWeights];
+    int count;
+    const uint8_t *q;
+    const float *sx;
+    const float *residual;
+    int rows, K, KB, y_bf16;
+    const int *offsets, *order;
+    int N, groups, k;
+    int n_tiles;                      // (set by the launcher)
+};
+int launch_f8_gemm(F8GemmArgs &a, hipStream_t st);
+
+// dw[g][m][k] = sum over the rows p of group g of dy[p][m] x[p][k] (+ add), BF16
+// rows (kxw4_grad.hip); offsets NULL: one group of all N rows.
+struct GradArgs {
+    const uint16_t *dy, *x;
+    const void *add;
+    void *dw;
+    float *part;                      // scratch: the parts of a split sum
+    const int *offsets;
+    int N, groups, M, K, dw_bf16;
+    int splits, m_tiles, k_tiles;     // (set by the launcher)
+};
+size_t grad_scratch(int N, int groups, int M, int K);
+int launch_grad(GradArgs &a, hipStream_t st);
+
 // Returns 1 (nothing launched) outside the per-token, one-split-per-token mode.
 int launch_gemm3(GemmArgs &a, hipStream_t st);
 // Returns 1 (nothing launched) outside the reference mode (K32 activation

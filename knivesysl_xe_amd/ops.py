@@ -30,6 +30,13 @@ gradient: dispatch_rows, combine_rows (the gradients of both are calls of their
 own) and adapter_add (which has none) refuse tensors that require grad unless
 gradients are off, as they are in a torch.autograd.Function.
 
+The 8-bit floating tier has none either (its tiers are integer): F8Weight holds
+e4m3 codes with a scale for each 128 x 128 block, gemm_f8[_fanout] and
+expert_gemm_f8[_fanout] project rows of values or of codes (quantize_act_f8,
+silu_mul_quant_f8). The gradient of a projection's input is the same product
+with F8Weight.transposed(), that of its weight grad_weight or
+expert_grad_weight.
+
 Torch provides device memory and the current stream only; every kernel is
 the HIP code in libkxw4.so, reached through ctypes. Tensors must live on a
 GPU; nothing here falls back to the CPU.
@@ -816,6 +823,343 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     _launch("kxw4_adapter_add", dev, y.data_ptr(), _DTYPE_CODES[y.dtype], x.data_ptr(), _DTYPE_CODES[x.dtype],
             ref, plan, o.data_ptr(), ws.data_ptr() if nbytes else None)
     return o
+
+
+# ---- the 8-bit floating tier ----------------------------------------------
+
+
+def _blocks(n: int) -> int:
+    return (n + 127) // 128
+
+
+@dataclass
+class F8Weight:
+    """`groups` weights (an expert's each; 1: one projection) of M rows and K
+    columns as e4m3 codes in the gfx950 tile layout, with an FP32 scale for each
+    128 x 128 block. M and K are multiples of 16."""
+    groups: int
+    M: int
+    K: int
+    codes: torch.Tensor      # uint8 [groups * M * 128 ceil(K / 128)]
+    scales: torch.Tensor     # float32 [groups][ceil(M / 128)][ceil(K / 128)]
+
+    def __post_init__(self):
+        self._made = None    # (device, addresses, C struct) once checked
+
+    def at(self) -> tuple:
+        return self.codes.data_ptr(), self.scales.data_ptr()
+
+    def c(self) -> _lib.WeightF8:
+        return _lib.WeightF8(self.groups, self.M, self.K, *self.at())
+
+    def __reduce__(self):    # (a copy is checked anew)
+        return F8Weight, (self.groups, self.M, self.K, self.codes, self.scales)
+
+    @classmethod
+    def empty(cls, groups: int, M: int, K: int, device="cuda") -> "F8Weight":
+        if not (1 <= groups <= 1024 and 16 <= M <= _MAX_F8 and 16 <= K <= _MAX_F8) or M % 16 or K % 16:
+            raise ValueError(f"groups {groups} (1 to 1024) of {M} rows and {K} columns (multiples of 16, up to 2^22)")
+        codes = torch.empty(groups * M * 128 * _blocks(K), dtype=torch.uint8, device=device)
+        scales = torch.empty(groups, _blocks(M), _blocks(K), dtype=torch.float32, device=device)
+        return cls(groups, M, K, codes, scales)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "F8Weight":
+        """codes: float8_e4m3fn (or its bits as uint8) [M][K] or [groups][M][K];
+        scales: float32, one for each 128 x 128 block of a weight."""
+        dev = _gpu(codes, "codes")
+        if codes.dim() not in (2, 3):
+            raise ValueError(f"codes must have shape (M, K) or (groups, M, K), got {tuple(codes.shape)}")
+        _need(codes, "codes", _F8, codes.shape, dev)
+        groups, (M, K) = codes.shape[0] if codes.dim() == 3 else 1, codes.shape[-2:]
+        w = cls.empty(groups, M, K, dev)
+        _need(scales, "scales", torch.float32, codes.shape[:-2] + (_blocks(M), _blocks(K)), dev)
+        w.scales.copy_(scales.view_as(w.scales))
+        _launch("kxw4_pack_weight_f8", dev, codes.data_ptr(), groups, M, K, w.codes.data_ptr())
+        return w
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, out: Optional["F8Weight"] = None) -> "F8Weight":
+        """Weights [M][K] or [groups][M][K] (f32 / bf16) by quantize_act_f8's
+        rule over blocks of 128 x 128; `out` (same sizes) is reused when given."""
+        dev = _gpu(w, "w")
+        if w.dim() not in (2, 3):
+            raise ValueError(f"w must have shape (M, K) or (groups, M, K), got {tuple(w.shape)}")
+        _need(w, "w", _FLOATS, w.shape, dev)
+        groups, (M, K) = w.shape[0] if w.dim() == 3 else 1, w.shape[-2:]
+        if w.requires_grad:
+            _detached("F8Weight.quantize")
+        o = _f8_out(out, groups, M, K, dev)
+        _launch("kxw4_quantize_weight_f8", dev, w.data_ptr(), _DTYPE_CODES[w.dtype], groups, M, K, o.codes.data_ptr(),
+                o.scales.data_ptr())
+        return o
+
+    def transposed(self, out: Optional["F8Weight"] = None) -> "F8Weight":
+        """The transposed weights, the same values: gemm_f8 of them and of dy's
+        rows is the gradient of the projection's input."""
+        dev = self.codes.device
+        ref = C.byref(_f8_weight(self, dev))
+        o = _f8_out(out, self.groups, self.K, self.M, dev)
+        _launch("kxw4_transpose_weight_f8", dev, ref, o.codes.data_ptr(), o.scales.data_ptr())
+        return o
+
+    def unpack(self):
+        """(codes as float8_e4m3fn [groups][M][K], scales)."""
+        dev = self.codes.device
+        ref = C.byref(_f8_weight(self, dev))
+        codes = torch.empty(self.groups, self.M, self.K, dtype=torch.uint8, device=dev)
+        _launch("kxw4_unpack_weight_f8", dev, ref, codes.data_ptr())
+        return codes.view(torch.float8_e4m3fn), self.scales
+
+
+_MAX_F8 = 1 << 22
+_F8 = (torch.uint8, torch.float8_e4m3fn)
+
+
+def _f8_out(out, groups: int, M: int, K: int, device) -> F8Weight:
+    if out is None:
+        return F8Weight.empty(groups, M, K, device)
+    _f8_weight(out, device)
+    if (out.groups, out.M, out.K) != (groups, M, K):
+        raise ValueError("out does not match the weights' sizes")
+    return out
+
+
+def _f8_weight(w: F8Weight, device) -> _lib.WeightF8:
+    """The C struct of a weight on `device`: the one made before while its
+    tensors lie where they did."""
+    if w.__class__ is F8Weight:
+        made = w._made
+        if made is not None and made[0] == device and made[1] == w.at() and (made[2].groups, made[2].M, made[2].K) == (
+                w.groups, w.M, w.K):
+            return made[2]
+    if not isinstance(w, F8Weight):
+        raise ValueError("weights must be F8Weight")
+    if device.type != "cuda":
+        raise ValueError("weights must be on the GPU")
+    _need(w.codes, "weight codes", torch.uint8, (w.groups * w.M * 128 * _blocks(w.K),), device)
+    _need(w.scales, "weight scales", torch.float32, (w.groups, _blocks(w.M), _blocks(w.K)), device)
+    c = w.c()
+    w._made = (device, w.at(), c)
+    return c
+
+
+@dataclass
+class QuantActF8:
+    """Rows as e4m3 codes q [T][128 ceil(K / 128)] (zeros past K) and scales
+    [ceil(K / 128)][T]."""
+    T: int
+    K: int
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, T: int, K: int, device="cuda") -> "QuantActF8":
+        q = torch.empty(T, 128 * _blocks(K), dtype=torch.uint8, device=device)
+        return cls(T, K, q, torch.empty(_blocks(K), T, dtype=torch.float32, device=device))
+
+
+def _check_act_f8(a: QuantActF8, device):
+    _need(a.q, "activation codes", torch.uint8, (a.T, 128 * _blocks(a.K)), device)
+    _need(a.scale, "activation scales", torch.float32, (_blocks(a.K), a.T), device)
+
+
+def _f8_rows(T: int, K: int, device, out) -> QuantActF8:
+    if K < 16 or K % 16 or K > _MAX_F8:
+        raise ValueError(f"K must be a multiple of 16 up to 2^22, got {K}")
+    if T > _MAX_SLOTS:
+        raise ValueError(f"up to 2^30 rows, got {T}")
+    if out is None:
+        return QuantActF8.empty(T, K, device)
+    if (out.T, out.K) != (T, K):
+        raise ValueError("out does not match the activation shape")
+    _check_act_f8(out, device)
+    return out
+
+
+def quantize_act_f8(x: torch.Tensor, out: Optional[QuantActF8] = None) -> QuantActF8:
+    """Rows [T][K] (f32 / bf16) as e4m3 codes with a scale for each row and block
+    of 128 columns; `out` (same T, K) is reused when given."""
+    dev = _gpu(x, "x")
+    if x.dim() != 2:
+        raise ValueError("x must have shape (T, K)")
+    T, K = x.shape
+    _need(x, "x", _FLOATS, (T, K), dev)
+    if x.requires_grad:
+        _detached("quantize_act_f8")
+    a = _f8_rows(T, K, dev, out)
+    _launch("kxw4_quantize_act_f8", dev, x.data_ptr(), _DTYPE_CODES[x.dtype], T, K, a.q.data_ptr(), a.scale.data_ptr())
+    return a
+
+
+def silu_mul_quant_f8(gate: torch.Tensor, up: torch.Tensor, keep_hidden=True, out: Optional[QuantActF8] = None):
+    """SiLU(gate) * up of [T][K] rows (f32 / bf16), computed in FP32 and
+    quantized: (hidden [T][K] f32 or None, the codes)."""
+    dev = _gpu(gate, "gate")
+    if gate.dim() != 2:
+        raise ValueError("gate must have shape (T, K)")
+    T, K = gate.shape
+    _need(gate, "gate", _FLOATS, (T, K), dev)
+    _need(up, "up", gate.dtype, (T, K), dev)
+    if gate.requires_grad or up.requires_grad:
+        _detached("silu_mul_quant_f8")
+    a = _f8_rows(T, K, dev, out)
+    hidden = torch.empty(T, K, dtype=torch.float32, device=dev) if keep_hidden else None
+    _launch("kxw4_silu_mul_quant_f8", dev, hidden.data_ptr() if keep_hidden else None, gate.data_ptr(), up.data_ptr(),
+            _DTYPE_CODES[gate.dtype], T, K, a.q.data_ptr(), a.scale.data_ptr())
+    return hidden, a
+
+
+_F8_ARRAYS = tuple(C.POINTER(_lib.WeightF8) * n for n in range(5))
+
+
+@functools.lru_cache(maxsize=4096)
+def _f8_bytes(device: int, Ms: tuple, K: int, T: int, codes: bool, dtype: int, plan: Optional[tuple]) -> int:
+    """Scratch of a product on a device (it goes by the CUs)."""
+    groups = plan[2] if plan else 1
+    ws = [_lib.WeightF8(groups, M, K) for M in Ms]
+    warr = _F8_ARRAYS[len(ws)](*[C.pointer(w) for w in ws])
+    a = _lib.ActF8(T, K, 0, 1 if codes else None)
+    with torch.cuda.device(device):
+        if plan:
+            r = _lib.Route(plan[0], plan[1], groups)
+            return lib().kxw4_expert_gemm_f8_workspace(warr, len(ws), C.byref(a), C.byref(r), plan[3], dtype)
+        return lib().kxw4_gemm_f8_workspace(warr, len(ws), C.byref(a), dtype)
+
+
+def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: bool):
+    n = len(ws)
+    if not 1 <= n <= 4:
+        raise ValueError(f"one to four weights, got {n}")
+    dev = ws[0].codes.device
+    cs = [_f8_weight(w, dev) for w in ws]
+    plan = None
+    if route is not None:
+        plan = _plan(route, dev)
+        for w in ws:
+            if w.groups != route.groups:
+                raise ValueError(f"a weight has {w.groups} groups, the plan {route.groups}")
+        N = route.T * route.k
+        rows = N if sorted_rows else route.T
+    if isinstance(a, QuantActF8):
+        T, K = a.T, a.K
+        _check_act_f8(a, dev)
+        ac = _lib.ActF8(T, K, 0, a.q.data_ptr(), a.scale.data_ptr(), None)
+        codes = True
+    else:
+        if not isinstance(a, torch.Tensor) or a.dim() != 2:
+            raise ValueError("the activation must be a QuantActF8 or a tensor (T, K)")
+        T, K = a.shape
+        if a.dtype not in _FLOATS or not a.is_contiguous() or a.device != dev:
+            _need(a, "x", _FLOATS, (T, K), dev)
+        if a.requires_grad:
+            _detached(name)
+        ac = _lib.ActF8(T, K, _DTYPE_CODES[a.dtype], None, None, a.data_ptr())
+        codes = False
+    if T > _MAX_SLOTS:
+        raise ValueError(f"up to 2^30 rows, got {T}")
+    if route is None:
+        N = T
+    elif T != rows:
+        raise ValueError(f"the activation has {T} rows for {rows} of the plan")
+    for w in ws:
+        if w.K != K:
+            raise ValueError(f"the activation has {K} columns, a weight {w.K}")
+    if outs is not None and len(outs) != n:
+        raise ValueError(f"outs has {len(outs)} tensors for {n} weights")
+    ys = [_out(N, w.M, dtype, dev, None if outs is None else outs[i], _OUTS[i]) for i, w in enumerate(ws)]
+    for y in ys:
+        if y.requires_grad:
+            _detached(name)
+    code = _dtype_code(dtype)
+    nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, codes, code,
+                       None if route is None else (route.T, route.k, route.groups, bool(sorted_rows)))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    warr = _F8_ARRAYS[n](*[C.pointer(c) for c in cs])
+    yarr = _POINTER_ARRAYS[n](*[y.data_ptr() for y in ys])
+    at = scratch.data_ptr() if nbytes else None
+    if route is None:
+        _launch("kxw4_gemm_f8", dev, warr, yarr, n, C.byref(ac), code, _ptr(_residual(residual, T, ws[0].M, dev)), at)
+    else:
+        _launch("kxw4_expert_gemm_f8", dev, warr, yarr, n, C.byref(ac), plan, bool(sorted_rows), code, at)
+    return ys
+
+
+def gemm_f8_fanout(ws: Sequence[F8Weight], a, dtype=torch.float32, outs=None):
+    """Up to 4 weights over one activation: outputs [T][M] of `dtype` (f32 /
+    bf16). `a` is a QuantActF8, or values [T][K] (f32 / bf16) that the call
+    quantizes. With f32 outputs the products are exact and summed in FP32; with
+    bf16 outputs and many rows the matrix core cuts each product to 2^-13 of the
+    largest near it first."""
+    return _f8_product("gemm_f8", ws, a, dtype, outs, None, None, False)
+
+
+def gemm_f8(w: F8Weight, a, dtype=torch.float32, residual=None, out=None) -> torch.Tensor:
+    """One weight of gemm_f8_fanout, plus an optional f32 residual [T][M]."""
+    return _f8_product("gemm_f8", [w], a, dtype, None if out is None else [out], residual, None, False)[0]
+
+
+def expert_gemm_f8_fanout(ws: Sequence[F8Weight], a, route: RowRoute, dtype=torch.float32, sorted_rows: bool = False,
+                          outs=None):
+    """gemm_f8_fanout with each row projected by its expert, as
+    expert_gemm_fanout: outputs [T*k][M] in the plan's order, of which the first
+    offsets[groups] rows are written. `a` holds the T tokens, or with
+    sorted_rows the T*k rows in the plan's order."""
+    return _f8_product("expert_gemm_f8", ws, a, dtype, outs, None, route, sorted_rows)
+
+
+def expert_gemm_f8(w: F8Weight, a, route: RowRoute, dtype=torch.float32, sorted_rows: bool = False,
+                   out=None) -> torch.Tensor:
+    """One weight of expert_gemm_f8_fanout."""
+    return _f8_product("expert_gemm_f8", [w], a, dtype, None if out is None else [out], None, route, sorted_rows)[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _grad_bytes(device: int, N: int, groups: int, M: int, K: int) -> int:
+    with torch.cuda.device(device):
+        return lib().kxw4_grad_weight_workspace(N, groups, M, K)
+
+
+def _grad_weight(name: str, dy, x, route, dtype, add, out):
+    dev = _gpu(dy, "dy")
+    if dy.dim() != 2 or not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("dy and x must have shapes (N, M) and (N, K)")
+    (N, M), K = dy.shape, x.shape[1]
+    if not (16 <= M <= _MAX_F8 and 16 <= K <= _MAX_F8) or M % 16 or K % 16 or N > _MAX_SLOTS:
+        raise ValueError(f"up to 2^30 rows of {M} and {K} columns (multiples of 16, up to 2^22), got {N}")
+    plan, groups, shape = None, 1, (M, K)
+    if route is not None:
+        plan, groups = _plan(route, dev), route.groups
+        shape = (groups, M, K)
+        if N != route.T * route.k:
+            raise ValueError(f"dy has {N} rows for {route.T * route.k} of the plan")
+    _need(dy, "dy", torch.bfloat16, (N, M), dev)
+    _need(x, "x", torch.bfloat16, (N, K), dev)
+    code = _dtype_code(dtype)
+    if add is not None:
+        _need(add, "add", dtype, shape, dev)
+    dw = _need(out, "out", dtype, shape, dev) if out is not None else torch.empty(shape, dtype=dtype, device=dev)
+    if dy.requires_grad or x.requires_grad or dw.requires_grad or (add is not None and add.requires_grad):
+        _detached(name)
+    nbytes = _grad_bytes(dev.index, N, groups, M, K)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch("kxw4_grad_weight", dev, dy.data_ptr(), x.data_ptr(), N, M, K, plan, None if add is None else add.data_ptr(),
+            dw.data_ptr(), code, scratch.data_ptr() if nbytes else None)
+    return dw
+
+
+def grad_weight(dy: torch.Tensor, x: torch.Tensor, dtype=torch.float32, add=None, out=None) -> torch.Tensor:
+    """The gradient of a projection's weight: dw [M][K] = dy^T x (+ add) of rows
+    dy [N][M] and x [N][K] (bf16), summed in FP32; `add` (of `dtype`, the
+    gradient so far) may be `out`."""
+    return _grad_weight("grad_weight", dy, x, None, dtype, add, out)
+
+
+def expert_grad_weight(dy: torch.Tensor, x: torch.Tensor, route: RowRoute, dtype=torch.float32, add=None,
+                       out=None) -> torch.Tensor:
+    """grad_weight of each expert's rows: dw [groups][M][K], rows in the plan's
+    order (dispatch_rows), those past offsets[groups] left out."""
+    return _grad_weight("expert_grad_weight", dy, x, route, dtype, add, out)
 
 
 class TqfFile:
