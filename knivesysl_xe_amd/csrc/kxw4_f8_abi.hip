@@ -2,6 +2,7 @@
 // gradient (include/kxw4.h): argument checks and the choice of kernel.
 #include "kxw4_checks.hpp"
 #include "kxw4_f8.hpp"
+#include "kxw4_f8_route.hpp"
 
 using namespace kxw4;
 
@@ -43,65 +44,102 @@ int check_product(const kxw4_weight_f8_t *const *ws, void *const *ys, int count,
     return KXW4_OK;
 }
 
-// Rows few enough that the weights' stream bounds the product: a tile of 16.
-bool few_rows(long long rows, int groups) { return rows <= 16ll * groups; }
-
 size_t codes_bytes(long long rows, int K) { return (size_t)rows * f8_blocks(K) * kF8Block; }
-size_t act_bytes(long long rows, int K) { return codes_bytes(rows, K) + (size_t)rows * f8_blocks(K) * sizeof(float); }
+// (multiples of 16 bytes)
+size_t act_bytes(long long rows, int K) {
+    return codes_bytes(rows, K) + ((size_t)rows * f8_blocks(K) * sizeof(float) + 15) / 16 * 16;
+}
 
 struct Rows {                                                // the rows sorted by group, or groups 0
     const int *offsets, *order;
     int N, groups, k;
 };
 
-int product(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a, int y_dtype,
-            const float *residual, const Rows &r, void *workspace, hipStream_t st) {
-    const int KB = f8_blocks(a->K);
-    const bool few = few_rows(r.groups ? r.N : a->T, r.groups ? r.groups : 1);
-    const uint8_t *q = a->q;
-    const float *sx = a->scale;
-    if (!q && !few) {
-        uint8_t *codes = static_cast<uint8_t *>(workspace);
-        float *scales = reinterpret_cast<float *>(codes + codes_bytes(a->T, a->K));
-        const int rc = launch_f8_quantize(a->x, a->x_dtype == KXW4_BF16, a->T, a->K, codes, scales, st);
-        if (rc) return rc;
-        q = codes;
-        sx = scales;
-    }
-    if (few) {
-        F8StreamArgs x{};
-        for (int i = 0; i < count; ++i) x.w[i] = F8StreamWeight{ws[i]->codes, ws[i]->scales, ys[i], ws[i]->M, 0};
-        x.count = count;
-        x.q = q;
-        x.sx = sx;
-        x.x = a->x;
-        x.residual = residual;
-        x.rows = a->T;
-        x.K = a->K;
-        x.KB = KB;
-        x.y_bf16 = y_dtype == KXW4_BF16 ? 1 : 0;
-        x.offsets = r.offsets;
-        x.order = r.order;
-        x.N = r.N;
-        x.groups = r.groups;
-        x.k = r.k;
-        return launch_f8_stream(x, q ? 0 : a->x_dtype == KXW4_BF16 ? 1 : 2, st);
-    }
+F8GemmArgs gemm_args(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a, int y_dtype,
+                     const Rows &r) {
     F8GemmArgs x{};
-    for (int i = 0; i < count; ++i) x.w[i] = F8GemmWeight{ws[i]->codes, ws[i]->scales, ys[i], ws[i]->M, 0};
+    for (int i = 0; i < count; ++i) x.w[i] = F8GemmWeight{ws[i]->codes, ws[i]->scales, ys ? ys[i] : nullptr, ws[i]->M, 0, 0};
     x.count = count;
-    x.q = q;
-    x.sx = sx;
-    x.residual = residual;
+    x.q = a->q;
+    x.sx = a->scale;
     x.rows = a->T;
     x.K = a->K;
-    x.KB = KB;
+    x.KB = f8_blocks(a->K);
     x.y_bf16 = y_dtype == KXW4_BF16 ? 1 : 0;
     x.offsets = r.offsets;
     x.order = r.order;
     x.N = r.N;
     x.groups = r.groups;
     x.k = r.k;
+    return x;
+}
+
+// The kernel of a product: rows of a stream tile or 0, and whether values are
+// quantized by a launch of their own.
+struct Way {
+    int rows;
+    bool quantizes;
+};
+
+Way way_of(const F8GemmArgs &x, const kxw4_act_f8_t *a) {
+    F8Sizes s{device_cus(), x.groups ? x.N : x.rows, x.KB, x.count, {}, x.groups, x.y_bf16 != 0};
+    for (int i = 0; i < x.count; ++i) s.M[i] = x.w[i].M;
+    Way w{f8_stream_rows(s), false};
+    // (the stream kernel takes values with 32-bit offsets, in tiles of 16)
+    if (!a->q)
+        w.quantizes = !(w.rows == 16 && f8_stream_quantizes(s) && (long long)a->T * a->K * elem_bytes(a->x_dtype) < (1ll << 31));
+    return w;
+}
+
+// Scratch of a product: the codes and scales of values, then the parts of
+// split sums.
+size_t workspace_of(const kxw4_weight_f8_t *const *ws, int count, const kxw4_act_f8_t *a, int y_dtype, const Rows &r) {
+    if (!ws || count <= 0 || count > kMaxWeights || !a || a->T <= 0 || !valid_f8(1, 16, a->K) || !valid_dtype(y_dtype)) return 0;
+    for (int i = 0; i < count; ++i)
+        if (!ws[i] || !valid_f8(1, ws[i]->M, a->K)) return 0;
+    const F8GemmArgs x = gemm_args(ws, nullptr, count, a, y_dtype, r);
+    const Way way = way_of(x, a);
+    return (way.quantizes ? act_bytes(a->T, a->K) : 0) + (way.rows ? 0 : f8_gemm_scratch(x));
+}
+
+int product(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a, int y_dtype,
+            const float *residual, const Rows &r, void *workspace, hipStream_t st) {
+    F8GemmArgs x = gemm_args(ws, ys, count, a, y_dtype, r);
+    const Way way = way_of(x, a);
+    const uint8_t *q = a->q;
+    const float *sx = a->scale;
+    uint8_t *scratch = static_cast<uint8_t *>(workspace);
+    if (way.quantizes) {
+        float *scales = reinterpret_cast<float *>(scratch + codes_bytes(a->T, a->K));
+        const int rc = launch_f8_quantize(a->x, a->x_dtype == KXW4_BF16, a->T, a->K, scratch, scales, st);
+        if (rc) return rc;
+        q = scratch;
+        sx = scales;
+        scratch += act_bytes(a->T, a->K);
+    }
+    if (way.rows) {
+        F8StreamArgs s{};
+        for (int i = 0; i < count; ++i) s.w[i] = F8StreamWeight{ws[i]->codes, ws[i]->scales, ys[i], ws[i]->M, 0};
+        s.count = count;
+        s.q = q;
+        s.sx = sx;
+        s.x = a->x;
+        s.residual = residual;
+        s.rows = x.rows;
+        s.K = x.K;
+        s.KB = x.KB;
+        s.y_bf16 = x.y_bf16;
+        s.offsets = r.offsets;
+        s.order = r.order;
+        s.N = r.N;
+        s.groups = r.groups;
+        s.k = r.k;
+        return launch_f8_stream(s, q ? 0 : a->x_dtype == KXW4_BF16 ? 1 : 2, way.rows, st);
+    }
+    x.q = q;
+    x.sx = sx;
+    x.residual = residual;
+    x.part = reinterpret_cast<float *>(scratch);
     return launch_f8_gemm(x, st);
 }
 
@@ -161,8 +199,7 @@ int kxw4_silu_mul_quant_f8(float *out, const void *gate, const void *up, int dty
 }
 
 size_t kxw4_gemm_f8_workspace(const kxw4_weight_f8_t *const *ws, int count, const kxw4_act_f8_t *a, int y_dtype) {
-    if (!ws || count <= 0 || count > kMaxWeights || !a || a->T <= 0 || !valid_f8(1, 16, a->K)) return 0;
-    return a->q || few_rows(a->T, 1) ? 0 : act_bytes(a->T, a->K);
+    return workspace_of(ws, count, a, y_dtype, Rows{});
 }
 
 int kxw4_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a, int y_dtype,
@@ -177,10 +214,8 @@ int kxw4_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, 
 
 size_t kxw4_expert_gemm_f8_workspace(const kxw4_weight_f8_t *const *ws, int count, const kxw4_act_f8_t *a,
                                      const kxw4_route_t *route, int sorted_rows, int y_dtype) {
-    if (!ws || count <= 0 || count > kMaxWeights || !a || a->T <= 0 || !valid_f8(1, 16, a->K) || !route ||
-        !valid_plan(route->T, route->k, route->groups))
-        return 0;
-    return a->q || few_rows((long long)route->T * route->k, route->groups) ? 0 : act_bytes(a->T, a->K);
+    if (!route || !valid_plan(route->T, route->k, route->groups)) return 0;
+    return workspace_of(ws, count, a, y_dtype, Rows{nullptr, nullptr, route->T * route->k, route->groups, route->k});
 }
 
 int kxw4_expert_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a,

@@ -1,6 +1,7 @@
 // kxw4_f8_gemm.hip — launches of the 8-bit floating tier's large tiles
 // (kxw4_f8_gemm.hpp).
 #include "kxw4_f8_gemm.hpp"
+#include "kxw4_f8_route.hpp"
 
 namespace kxw4 {
 
@@ -24,11 +25,20 @@ static int f8_plan(F8GemmArgs &a, int rgs) {
     return nt;
 }
 
+// Work-groups that the card holds at once, a multiple of eight.
+template <class S, int NST, int OCC>
+static long long f8_slots() {
+    constexpr int per_cu = std::min(4 * OCC / S::NW, 160 * 1024 / S::template lds_bytes<NST>());
+    static_assert(per_cu >= 1, "");
+    return (long long)std::max(8, device_cus() / 8 * 8) * per_cu;
+}
+
 template <int TA, int TB, int WT, int WR, int NST, int EX, int OCC>
 static int f8_dense(F8GemmArgs &a, hipStream_t st) {
     using S = F8Shape<TA, TB, WT, WR>;
-    const long long grid = (long long)f8_plan(a, S::BR / 16) * ((a.rows + S::BT - 1) / S::BT);
-    if (grid > grid_limit(S::NTH)) return -2;
+    const long long tiles = (long long)f8_plan(a, S::BR / 16) * ((a.rows + S::BT - 1) / S::BT) * a.splits;
+    if (tiles >= (1ll << 31) - (1 << 16)) return -2;         // (32-bit tile numbers)
+    const long long grid = std::min<long long>(tiles, f8_slots<S, NST, OCC>());
     auto k = f8_gemm_kernel<TA, TB, WT, WR, NST, EX, OCC>;
     constexpr size_t lds = S::template lds_bytes<NST>();
     static_assert(lds <= 160 * 1024, "LDS");
@@ -39,14 +49,14 @@ static int f8_dense(F8GemmArgs &a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-template <int TA, int TB, int WR, int NST, int EX, int OCC>
+template <int TA, int TB, int WT, int WR, int NST, int EX, int OCC>
 static int f8_grouped(F8GemmArgs &a, hipStream_t st) {
-    using S = F8Shape<TA, TB, 1, WR>;
-    const long long grid = tiles_at_most(a.N, a.groups, S::BT) * f8_plan(a, S::BR / 16);
-    if (grid > grid_limit(S::NTH)) return -2;
-    auto k = f8_group_kernel<TA, TB, WR, NST, EX, OCC>;
-    constexpr size_t lds = std::max({S::template lds_bytes<NST>(), F8Shape<(TA > 1 ? TA / 2 : 1), TB, 1, WR>::template lds_bytes<NST>(),
-                                     F8Shape<1, TB, 1, WR>::template lds_bytes<NST>()});
+    using S = F8Shape<TA, TB, WT, WR>;
+    const long long tiles = tiles_at_most(a.N, a.groups, S::BT) * f8_plan(a, S::BR / 16);
+    if (tiles >= (1ll << 31) - (1 << 20)) return -2;         // (32-bit tile numbers)
+    const long long grid = std::min<long long>((tiles + 7) / 8 * 8, f8_slots<S, NST, OCC>());
+    auto k = f8_group_kernel<TA, TB, WT, WR, NST, EX, OCC>;
+    constexpr size_t lds = S::template lds_bytes<NST>();
     static_assert(lds <= 160 * 1024, "LDS");
     static bool done[64] = {};
     const int rc = f8_lds(reinterpret_cast<const void *>(k), lds, done);
@@ -55,10 +65,53 @@ static int f8_grouped(F8GemmArgs &a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
+static F8Sizes f8_sizes(const F8GemmArgs &a) {
+    F8Sizes s{device_cus(), a.groups ? a.N : a.rows, a.KB, a.count, {}, a.groups, a.y_bf16 != 0};
+    for (int i = 0; i < a.count; ++i) s.M[i] = a.w[i].M;
+    return s;
+}
+
+size_t f8_gemm_scratch(const F8GemmArgs &a) {
+    if (a.groups) return 0;
+    const F8Choice c = f8_choose(f8_sizes(a));
+    size_t outputs = 0;
+    for (int i = 0; i < a.count; ++i) outputs += (size_t)a.rows * a.w[i].M;
+    return c.splits > 1 ? outputs * c.splits * sizeof(float) : 0;
+}
+
+static int f8_config(F8GemmArgs &a, int id, hipStream_t st) {
+    switch (id) {
+    case 0: return f8_dense<4, 2, 2, 4, 2, 0, 2>(a, st);
+    case 1: return f8_dense<2, 2, 4, 2, 3, 0, 2>(a, st);
+    case 2: return f8_dense<2, 2, 2, 2, 4, 0, 2>(a, st);
+    case 3: return f8_dense<1, 2, 2, 2, 3, 0, 2>(a, st);
+    case 4: return f8_dense<2, 2, 2, 2, 2, 1, 2>(a, st);
+    default: return f8_dense<1, 2, 2, 2, 3, 1, 2>(a, st);
+    }
+}
+
 int launch_f8_gemm(F8GemmArgs &a, hipStream_t st) {
-    if (a.groups) return a.y_bf16 ? f8_grouped<2, 2, 2, 2, 0, 2>(a, st) : f8_grouped<2, 2, 2, 2, 1, 2>(a, st);
-    if (a.y_bf16) return f8_dense<4, 2, 2, 4, 2, 0, 2>(a, st);
-    return f8_dense<2, 2, 2, 2, 2, 1, 2>(a, st);
+    if (!a.groups) {
+        const F8Choice c = f8_choose(f8_sizes(a));
+        a.splits = c.splits;
+        long long outputs = 0;
+        for (int i = 0; i < a.count; ++i) {
+            a.w[i].part = outputs * a.splits;
+            outputs += (long long)a.rows * a.w[i].M;
+        }
+        if (a.splits == 1) a.part = nullptr;
+        const int rc = f8_config(a, c.id, st);
+        if (rc || a.splits == 1) return rc;
+        const long long grid = (outputs / 4 + 255) / 256;
+        if (grid > grid_limit(256)) return -2;
+        hipLaunchKernelGGL(f8_join_kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
+        return hipGetLastError() == hipSuccess ? 0 : -6;
+    }
+    a.splits = 1;
+    a.part = nullptr;
+    const bool long_runs = f8_long_groups(f8_sizes(a));
+    if (a.y_bf16) return long_runs ? f8_grouped<2, 2, 2, 4, 3, 0, 2>(a, st) : f8_grouped<1, 2, 2, 2, 3, 0, 2>(a, st);
+    return long_runs ? f8_grouped<2, 2, 2, 2, 2, 1, 2>(a, st) : f8_grouped<1, 2, 2, 2, 3, 1, 2>(a, st);
 }
 
 }  // namespace kxw4

@@ -33,24 +33,38 @@ struct F8Rows<kF8F32> {
     v4u x[8];
 };
 
+// Loads through a buffer descriptor: what lies past its range reads as zero and
+// moves nothing, so the loads ahead of a wave's last blocks need no branch.
+constexpr int kF8Word3 = 0x00020000;                         // untyped buffer, format 32
+constexpr uint32_t kF8Past = 0x80000000u;                    // an offset past every range (all are below 2^31)
+constexpr int kF8Stream = 2;                                 // non-temporal: the weights are read once
+template <int AUX>
+__device__ __forceinline__ v4u f8_buffer(const void *base, uint32_t range, uint32_t lane, uint32_t at) {
+    return __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc((void *)base, 0, range, kF8Word3), lane, at, AUX);
+}
+
+// xp: the first row's address, row: this lane's from it; both within 2^31 bytes
+// of the descriptor's base.
 template <int X>
-__device__ __forceinline__ void f8_rows_load(F8Rows<X> &f, const F8StreamArgs &a, long long row, int kb, int g) {
+__device__ __forceinline__ void f8_rows_load(F8Rows<X> &f, const F8StreamArgs &a, const void *xp, uint32_t range, const float *sp,
+                                             uint32_t s_range, uint32_t row, int kb, int g) {
     if constexpr (X == kF8Codes) {
-        const uint8_t *p = a.q + (row * a.KB + kb) * kF8Block + 16 * g;
-        f.q[0] = *reinterpret_cast<const v4u *>(p);
-        f.q[1] = *reinterpret_cast<const v4u *>(p + 64);
-        f.scale = a.sx[(size_t)kb * a.rows + row];
+        const uint32_t at = kb < a.KB ? kb * kF8Block : kF8Past, off = row * (uint32_t)(a.KB * kF8Block) + 16 * g;
+        f.q[0] = f8_buffer<0>(xp, range, off, at);
+        f.q[1] = f8_buffer<0>(xp, range, off + 64, at);
+        const uint32_t sat = kb < a.KB ? (uint32_t)kb * (uint32_t)a.rows * 4 : kF8Past;
+        f.scale = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(__builtin_amdgcn_make_buffer_rsrc((void *)sp, 0, s_range, kF8Word3),
+                                                                      row * 4, sat, 0));
     } else {
         constexpr int N = X == kF8Bf16 ? 2 : 4, B = X == kF8Bf16 ? 2 : 4;
+        const uint32_t at = (uint32_t)kb * (kF8Block * B);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int k = kb * kF8Block + 64 * h + 16 * g;
-            const uint8_t *p = static_cast<const uint8_t *>(a.x) + (row * a.K + k) * B;
+            const int k = 64 * h + 16 * g;
+            // (columns past K, and with them blocks past the last)
+            const uint32_t off = kb * kF8Block + k < a.K ? (row * (uint32_t)a.K + k) * B : kF8Past;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                f.x[h * N + i] = v4u{0, 0, 0, 0};
-                if (k < a.K) f.x[h * N + i] = *reinterpret_cast<const v4u *>(p + 16 * i);
-            }
+            for (int i = 0; i < N; ++i) f.x[h * N + i] = f8_buffer<0>(xp, range, off + 16 * i, at);
         }
     }
 }
@@ -92,9 +106,8 @@ __device__ __forceinline__ float f8_rows_operands(const F8Rows<X> &f, v8bf (&b)[
     }
 }
 
-constexpr int kF8StreamDepth = 2;                            // column blocks in flight per wave
-
-template <int R, int TB, int X, bool GRP>
+// D: column blocks in flight per wave
+template <int R, int TB, int X, bool GRP, int D>
 __global__ __launch_bounds__(512) void f8_stream_kernel(const F8StreamArgs a) {
     extern __shared__ __attribute__((aligned(16))) float red[];
     const int lane = threadIdx.x & 63, m16 = lane & 15, g = lane >> 4;
@@ -121,22 +134,27 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8StreamArgs a) {
         if (rb >= a.w[i].blk) wi = i;
     const F8StreamWeight W = a.w[wi];
     const int RG = W.M / 16, rg0 = (rb - W.blk) * R;
-    const uint8_t *codes = W.codes + (size_t)e * RG * a.KB * kF8Tile + lane * 16;
+    const uint8_t *codes = W.codes + ((size_t)e * RG + rg0) * a.KB * kF8Tile;
     // (R divides 8, so the row-groups share a block of 128 rows)
     const float *sw = W.scales + ((size_t)e * f8_blocks(W.M) + rg0 / 8) * a.KB;
-    size_t wrow[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) wrow[r] = (size_t)min(rg0 + r, RG - 1) * a.KB * kF8Tile;
-    // the lane's row of x in each block of 16 (past the tile: its last)
-    long long xrow[TB];
+    const uint32_t w_range = min(R, RG - rg0) * a.KB * kF8Tile, lane16 = lane * 16;
+    // the lane's row of x in each block of 16 (past the tile: its last), from
+    // the tile's first row (dense) or row 0
+    uint32_t xrow[TB];
 #pragma unroll
     for (int b = 0; b < TB; ++b) {
         const int t = min(t0 + 16 * b + m16, t_end - 1);
         if constexpr (GRP) xrow[b] = a.order ? (uint32_t)a.order[t] / (uint32_t)a.k : t;
-        else xrow[b] = t;
+        else xrow[b] = t - t0;
     }
+    constexpr int XB = X == kF8F32 ? 4 : X == kF8Bf16 ? 2 : 1;
+    const size_t x_stride = X == kF8Codes ? (size_t)a.KB * kF8Block : (size_t)a.K * XB;
+    const int x_first = GRP ? 0 : t0;
+    const uint8_t *xp = static_cast<const uint8_t *>(X == kF8Codes ? a.q : a.x) + x_first * x_stride;
+    const uint32_t x_range = (uint32_t)((GRP ? a.rows : t_end - t0) * x_stride);
+    const float *sp = a.sx + x_first;
+    const uint32_t s_range = (uint32_t)(((size_t)(a.KB - 1) * a.rows + (GRP ? a.rows : t_end - t0)) * 4);
 
-    constexpr int D = kF8StreamDepth;
     v4u wt[D][R][2];
     F8Rows<X> xs[D][TB];
     float ws[D];
@@ -146,15 +164,17 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8StreamArgs a) {
 #pragma unroll
         for (int b = 0; b < TB; ++b) acc[r][b] = v4f{0, 0, 0, 0};
     auto load = [&](int d, int kb) {
-        kb = min(kb, a.KB - 1);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                wt[d][r][h] = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(codes + wrow[r] + (size_t)kb * kF8Tile + 1024 * h));
-        ws[d] = sw[kb];
+            for (int h = 0; h < 2; ++h) {
+                // (row-groups past M and blocks past the last: nothing is read)
+                const uint32_t at = kb < a.KB ? (uint32_t)(r * a.KB + kb) * kF8Tile + 1024 * h : kF8Past;
+                wt[d][r][h] = f8_buffer<kF8Stream>(codes, w_range, lane16, at);
+            }
+        ws[d] = sw[min(kb, a.KB - 1)];
 #pragma unroll
-        for (int b = 0; b < TB; ++b) f8_rows_load<X>(xs[d][b], a, xrow[b], kb, g);
+        for (int b = 0; b < TB; ++b) f8_rows_load<X>(xs[d][b], a, xp, x_range, sp, s_range, xrow[b], kb, g);
     };
 #pragma unroll
     for (int d = 0; d < D; ++d) load(d, wave + d * nw);
@@ -219,7 +239,7 @@ __global__ __launch_bounds__(512) void f8_stream_kernel(const F8StreamArgs a) {
     }
 }
 
-template <int R, int TB, int X, bool GRP>
+template <int R, int TB, int X, bool GRP, int D>
 static int f8_stream(F8StreamArgs &a, int nw, hipStream_t st) {
     int blk = 0;
     for (int i = 0; i < a.count; ++i) {
@@ -231,22 +251,33 @@ static int f8_stream(F8StreamArgs &a, int nw, hipStream_t st) {
     const long long grid = tiles * blk;
     if (grid > grid_limit(64 * nw)) return -2;
     const size_t lds = (size_t)nw * R * TB * 1024;
-    hipLaunchKernelGGL((f8_stream_kernel<R, TB, X, GRP>), dim3((unsigned)grid), dim3(64 * nw), lds, st, a);
+    hipLaunchKernelGGL((f8_stream_kernel<R, TB, X, GRP, D>), dim3((unsigned)grid), dim3(64 * nw), lds, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-template <int X, bool GRP>
-static int f8_stream_x(F8StreamArgs &a, hipStream_t st) {
-    return f8_stream<2, 1, X, GRP>(a, 8, st);
+// Two row-groups a work-group, or one where they do not fill the CUs; four waves,
+// or eight for long sums of few work-groups (codes, one row: 5120 x 17408 19 us
+// for 25, 17408 x 5120 33 for 35, 4096 x 4096 6.2 either way).
+template <int TB, int X, bool GRP>
+static int f8_stream_shape(F8StreamArgs &a, hipStream_t st) {
+    long long rgs = 0;
+    for (int i = 0; i < a.count; ++i) rgs += a.w[i].M / 16;
+    rgs *= GRP ? tiles_at_most(a.N, a.groups, 16 * TB) : (a.rows + 16 * TB - 1) / (16 * TB);
+    const long long cus = device_cus();
+    if (rgs <= cus) return f8_stream<1, TB, X, GRP, 2>(a, 4, st);
+    if (a.KB >= 64 && rgs < 4 * cus) return f8_stream<2, TB, X, GRP, 2>(a, 8, st);
+    return f8_stream<2, TB, X, GRP, 2>(a, 4, st);
 }
 
-int launch_f8_stream(F8StreamArgs &a, int x, hipStream_t st) {
-    if (a.groups) {
-        if (x == kF8Codes) return f8_stream_x<kF8Codes, true>(a, st);
-        return x == kF8Bf16 ? f8_stream_x<kF8Bf16, true>(a, st) : f8_stream_x<kF8F32, true>(a, st);
-    }
-    if (x == kF8Codes) return f8_stream_x<kF8Codes, false>(a, st);
-    return x == kF8Bf16 ? f8_stream_x<kF8Bf16, false>(a, st) : f8_stream_x<kF8F32, false>(a, st);
+template <bool GRP>
+static int f8_stream_rows(F8StreamArgs &a, int x, int rows, hipStream_t st) {
+    if (x == kF8Bf16) return f8_stream_shape<1, kF8Bf16, GRP>(a, st);
+    if (x == kF8F32) return f8_stream_shape<1, kF8F32, GRP>(a, st);
+    return rows == 16 ? f8_stream_shape<1, kF8Codes, GRP>(a, st) : f8_stream_shape<2, kF8Codes, GRP>(a, st);
+}
+
+int launch_f8_stream(F8StreamArgs &a, int x, int rows, hipStream_t st) {
+    return a.groups ? f8_stream_rows<true>(a, x, rows, st) : f8_stream_rows<false>(a, x, rows, st);
 }
 
 }  // namespace kxw4

@@ -263,13 +263,15 @@ struct F8StreamArgs {
     int N, groups, k;
     int row_blocks;                   // (set by the launcher)
 };
-int launch_f8_stream(F8StreamArgs &a, int x, hipStream_t st);
+// x: what the rows come as (codes, BF16, FP32); rows: of a tile, 16 or (codes) 32
+int launch_f8_stream(F8StreamArgs &a, int x, int rows, hipStream_t st);
 
 struct F8GemmWeight {
     const uint8_t *codes;
     const float *scales;
     void *y;
     int M, nt_begin;                  // nt_begin: first weight tile (set by the launcher)
+    long long part;                   // its parts in F8GemmArgs::part (set by the launcher)
 };
 struct F8GemmArgs {
     F8GemmWeight w[kMaxWeights];
@@ -280,8 +282,10 @@ struct F8GemmArgs {
     int rows, K, KB, y_bf16;
     const int *offsets, *order;
     int N, groups, k;
-    int n_tiles;                      // (set by the launcher)
+    float *part;                      // scratch of f8_gemm_scratch bytes
+    int n_tiles, splits;              // (set by the launcher)
 };
+size_t f8_gemm_scratch(const F8GemmArgs &a);
 int launch_f8_gemm(F8GemmArgs &a, hipStream_t st);
 
 // dw[g][m][k] = sum over the rows p of group g of dy[p][m] x[p][k] (+ add), BF16

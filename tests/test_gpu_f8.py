@@ -171,6 +171,21 @@ def test_fanout_gives_each_weights_product():
                 assert torch.equal(y, ops.gemm_f8(w, x, out))
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("T,K,Ms", [(1100, 144, (16400,)), (2600, 16, (4112, 4240)), (1025, 528, (8192, 8208)), (70000, 128, (272,))])
+def test_products_of_more_tiles_than_work_groups(T, K, Ms, out):
+    # (a work-group takes several tiles, one after another, of either weight)
+    cs = [exact_weight(1, M, K, M) for M in Ms]
+    ws = [ops.F8Weight.from_codes(c[0], s[0]) for c, s in cs]
+    x = exact_rows(T, K, T)
+    for y, c in zip(ops.gemm_f8_fanout(ws, x, out), cs):
+        want = torch.empty_like(y)
+        wt = weight_values(*c)[0].t().contiguous()
+        for t in range(0, T, 8192):
+            want[t:t + 8192] = (x[t:t + 8192].double() @ wt).to(out)
+        assert torch.equal(y, want)
+
+
 def test_products_of_no_rows():
     codes, scales = normal_weight(1, 64, 128, 1)
     w = ops.F8Weight.from_codes(codes[0], scales[0])
