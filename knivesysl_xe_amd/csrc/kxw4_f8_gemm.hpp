@@ -49,8 +49,9 @@ struct F8Shape {
     static constexpr int X_LOADS = (X_CHUNKS + NW - 1) / NW, W_LOADS = (W_CHUNKS + NW - 1) / NW;
     static constexpr int S_LOADS = (S_CHUNKS + NW - 1) / NW;
     static constexpr int LOADS = X_LOADS + W_LOADS + S_LOADS;
+    static constexpr int SLAB = 1024;                        // output staging of a wave: 16 tokens' 64 bytes
     template <int NST>
-    static constexpr int lds_bytes() { return NST * STAGE; }
+    static constexpr int lds_bytes() { return NST * STAGE + NW * SLAB; }
 };
 
 // f(integral_constant<int, I>) for each I of the sequence, in order
@@ -237,58 +238,57 @@ __device__ __forceinline__ void f8_tiles(const F8GemmArgs &a, F8Tile tile, Next 
                 for (int r = 0; r < 16; ++r) f[i][j][r] = 0.0f;
     };
     // ---- output: register r of a block is row 8(r/4) + 4kg + r%4 of the lane's
-    // token. FP32: four rows a lane and store. BF16: lanes l and l + 32 exchange
-    // half of a pair of such runs, so a lane stores eight rows ----
+    // token. BF16: 16 tokens at a time pass the wave's slab in LDS (64 bytes of
+    // each, its 16-byte piece c at c ^ (t / 4 % 4)) and go out 64 bytes a token,
+    // so a store meets 16 of the L2's half lines, not 32 quarters (8,192 tokens,
+    // 8,192 x 1,024: 98 us without the slab, 87). FP32: four rows a lane and
+    // store (through the slab 22.7 us became 24.3, 256 tokens, 5,120 x 5,120) ----
+    uint8_t *slab = smem + NST * STAGE + wave * S::SLAB;
     auto store = [&]() {
         const F8GemmWeight &W = a.w[tile.wi];
+        // (the lane's places are computed anew for each tile: kept over the steps
+        // they would spill)
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));
+        const int m32 = lane & 31, kg = lane >> 5, t16 = m32 & 15, swz = t16 >> 2;
         const int M = W.M, row0 = (tile.rg0 + wr * 2 * TB) * 16;
+        const bool part = !GRP && a.part;                    // (part of a sum: f8_join_kernel ends it)
 #pragma unroll
         for (int i = 0; i < TA; ++i) {
-            if (i >= na) continue;                               // (uniform)
-            const int t = tile.t0 + 32 * (WT * i + wt) + m32;
-            const bool mine = t < tile.t_end;
+            const int tb = tile.t0 + 32 * (WT * i + wt), t = tb + m32;
+            if (i >= na || tb >= tile.t_end) continue;       // (uniform)
 #pragma unroll
             for (int j = 0; j < TB; ++j) {
+                const int row = row0 + 32 * j;
+                if (row >= M) continue;                      // (uniform)
+                if (!GRP && a.residual && !part) {
+                    // (places past the ends read the last ones, for outputs that are not stored)
+                    const float *res = a.residual + (size_t)min(t, a.rows - 1) * M;
+                    v4f x[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {                // 16 rows
-                    const int row = row0 + 32 * j + 16 * h;
-                    if (row >= M) continue;                  // (uniform)
-                    v4f v[2];
+                    for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const v4f *>(res + min(row + 8 * q + 4 * kg, M - 4));
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
+                    for (int r = 0; r < 16; ++r) f[i][j][r] += x[r / 4][r % 4];
+                }
+                if (EX == 0 && !part) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[q][r] = f[i][j][4 * (2 * h + q) + r];
-                    if (!GRP && a.part) {                    // (part of a sum: f8_join_kernel ends it)
-                        float *to = a.part + W.part + ((size_t)tile.s * a.rows + t) * M + row;
-                        if (mine) {
+                    for (int h = 0; h < 2; ++h) {            // 16 tokens
+                        if ((m32 >> 4) == h) {
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) *reinterpret_cast<v4f *>(to + 8 * q + 4 * kg) = v[q];
+                            for (int q = 0; q < 4; ++q)
+                                *reinterpret_cast<v2u *>(slab + t16 * 64 + ((q ^ swz) * 16) + kg * 8) =
+                                    v2u{pack_bf16(f[i][j][4 * q], f[i][j][4 * q + 1]), pack_bf16(f[i][j][4 * q + 2], f[i][j][4 * q + 3])};
                         }
-                        continue;
+                        const int ts = tb + 16 * h + (lane >> 2), r = row + (lane & 3) * 8;
+                        const v4u v = *reinterpret_cast<const v4u *>(slab + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) * 16));
+                        if (ts < tile.t_end && r < M) *reinterpret_cast<v4u *>(static_cast<uint16_t *>(W.y) + (size_t)ts * M + r) = v;
                     }
-                    if (!GRP && a.residual && mine) {
+                } else {
+                    float *to = (part ? a.part + W.part + (size_t)tile.s * a.rows * M : static_cast<float *>(W.y)) + (size_t)t * M + row + 4 * kg;
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const v4f x = *reinterpret_cast<const v4f *>(a.residual + (size_t)t * M + row + 8 * q + 4 * kg);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) v[q][r] += x[r];
-                        }
-                    }
-                    if constexpr (EX == 0) {
-                        v4u o;
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const auto x = __builtin_amdgcn_permlane32_swap(pack_bf16(v[0][2 * r], v[0][2 * r + 1]),
-                                                                            pack_bf16(v[1][2 * r], v[1][2 * r + 1]), false, false);
-                            o[r] = x[0];
-                            o[2 + r] = x[1];
-                        }
-                        if (mine) *reinterpret_cast<v4u *>(static_cast<uint16_t *>(W.y) + (size_t)t * M + row + 8 * kg) = o;
-                    } else if (mine) {
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-                            *reinterpret_cast<v4f *>(static_cast<float *>(W.y) + (size_t)t * M + row + 8 * q + 4 * kg) = v[q];
-                    }
+                    for (int q = 0; q < 4; ++q)
+                        if (t < tile.t_end && row + 8 * q < M)
+                            *reinterpret_cast<v4f *>(to + 8 * q) = v4f{f[i][j][4 * q], f[i][j][4 * q + 1], f[i][j][4 * q + 2], f[i][j][4 * q + 3]};
                 }
             }
         }
@@ -492,7 +492,7 @@ __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void f8_gemm_kernel(const F8GemmA
 
 // The parts of split sums, added up in their order, plus the residual; four
 // outputs a thread.
-__global__ __launch_bounds__(256) inline void f8_join_kernel(const F8GemmArgs a) {
+__global__ __launch_bounds__(256) void f8_join_kernel(const F8GemmArgs a) {
     long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
     int wi = 0;
     for (; wi < a.count; ++wi) {
@@ -522,33 +522,29 @@ __global__ __launch_bounds__(256) inline void f8_join_kernel(const F8GemmArgs a)
 // The same over rows sorted by group: tiles of 32 TA WT places of one group, its
 // last one shorter (its steps run the token blocks it has).
 //
-// Column c = e * a.n_tiles + n is weight tile n of group e with the group's token
-// tiles; XCD c % 8 takes it, so its codes pass one L2 and the columns of every
-// group, long or short, are dealt to all XCDs. An XCD's work-groups take the
-// tiles of its columns in turn.
-struct F8Columns {
+// The tiles in order: groups, in each its weight tiles, of each the group's token
+// tiles. An XCD (blockIdx % 8) takes an eighth of them, one after another, and its
+// work-groups those in turn: at once they run the tiles of one or two groups,
+// whose tokens and codes each pass that XCD's L2 once (with each group's weight
+// tiles dealt over the XCDs every one of these read all the tokens: 2,048 x 8 rows
+// over 64 groups, 5,120 -> 2 x 1,024: 313 us, so 298).
+struct F8Scan {
     int first, end, before, total, begin, begin_end;         // a lane's run of groups, the tiles before it, all tiles; its first group's places
 };
 
-// Columns of group e that XCD x takes: n = n0, n0 + 8, ..
-__device__ __forceinline__ int f8_columns(int e, int x, int nnt, int &n0) {
-    n0 = (x - e * nnt) & 7;
-    return n0 < nnt ? (nnt - 1 - n0) / 8 + 1 : 0;
-}
-
 template <int BT>
-__device__ __forceinline__ F8Columns f8_scan(const int *offsets, int groups, int x, int nnt, int lane) {
+__device__ __forceinline__ F8Scan f8_scan(const int *offsets, int groups, int nnt, int lane) {
     const int run = (groups + 63) / 64;
-    F8Columns s;
+    F8Scan s;
     s.first = min(lane * run, groups);
     s.end = min(s.first + run, groups);
-    int sum = 0, n0, lo = offsets[s.first];
+    int sum = 0, lo = offsets[s.first];
     s.begin = lo;
     s.begin_end = lo;
     for (int e = s.first; e < s.end; ++e) {
         const int hi = offsets[e + 1];
         if (e == s.first) s.begin_end = hi;
-        sum += (hi - lo + BT - 1) / BT * f8_columns(e, x, nnt, n0);
+        sum += (hi - lo + BT - 1) / BT * nnt;
         lo = hi;
     }
     const int inc = wave_scan(sum);
@@ -557,25 +553,25 @@ __device__ __forceinline__ F8Columns f8_scan(const int *offsets, int groups, int
     return s;
 }
 
-// Tile u < s.total of an XCD: its group, places and weight tile.
+// Tile u < s.total: its group, places and weight tile.
 template <int BT>
-__device__ __forceinline__ F8Tile f8_column_tile(const F8Columns &s, const F8GemmArgs &a, int x, int brg, int u) {
+__device__ __forceinline__ F8Tile f8_group_tile(const F8Scan &s, const F8GemmArgs &a, int brg, int u) {
     // (lanes without tiles share the start of the next that has some, so the
     // last lane that starts at or before u has the tile)
     const int l = 63 - __builtin_clzll(__ballot(s.first < s.end && s.before <= u));
     int e = __builtin_amdgcn_readlane(s.first, l), before = __builtin_amdgcn_readlane(s.before, l);
     int begin = __builtin_amdgcn_readlane(s.begin, l), end = __builtin_amdgcn_readlane(s.begin_end, l);
-    int count, n0;
+    int count;
     for (;;) {
         count = (end - begin + BT - 1) / BT;
-        const int n = count * f8_columns(e, x, a.n_tiles, n0);
+        const int n = count * a.n_tiles;
         if (u < before + n) break;
         before += n;
         ++e;
         begin = end;
         end = __builtin_amdgcn_readfirstlane(a.offsets[e + 1]);
     }
-    const int column = (u - before) / count, t0 = begin + (u - before - column * count) * BT, ntg = n0 + 8 * column;
+    const int ntg = (u - before) / count, t0 = begin + (u - before - ntg * count) * BT;
     int wi = 0;
     for (int i = 1; i < a.count; ++i)
         if (ntg >= a.w[i].nt_begin) wi = i;
@@ -587,12 +583,13 @@ __global__ __launch_bounds__(64 * WT * WR)
 __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void f8_group_kernel(const F8GemmArgs a) {
     constexpr int BT = 32 * TA * WT, BRG = 2 * TB * WR;
     const int x = blockIdx.x % 8, first = blockIdx.x / 8, stride = gridDim.x / 8;      // (a multiple of eight)
-    const F8Columns s = f8_scan<BT>(a.offsets, a.groups, x, a.n_tiles, threadIdx.x & 63);
-    if (first >= s.total) return;
-    f8_tiles<TA, TB, WT, WR, NST, EX, true>(a, f8_column_tile<BT>(s, a, x, BRG, first), [&](F8Tile &t) {
-        const int n = t.n + 1, u = first + n * stride;
-        if (u >= s.total) return 0;
-        t = f8_column_tile<BT>(s, a, x, BRG, u);
+    const F8Scan s = f8_scan<BT>(a.offsets, a.groups, a.n_tiles, threadIdx.x & 63);
+    const int from = (int)((long long)s.total * x / 8), end = (int)((long long)s.total * (x + 1) / 8);
+    if (from + first >= end) return;
+    f8_tiles<TA, TB, WT, WR, NST, EX, true>(a, f8_group_tile<BT>(s, a, BRG, from + first), [&](F8Tile &t) {
+        const int n = t.n + 1, u = from + first + n * stride;
+        if (u >= end) return 0;
+        t = f8_group_tile<BT>(s, a, BRG, u);
         t.n = n;
         return 1;
     });
