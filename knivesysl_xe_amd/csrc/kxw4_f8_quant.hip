@@ -35,64 +35,48 @@ __device__ __forceinline__ void f8_load8(const void *p, size_t i, float (&v)[8])
     }
 }
 
-// 16 lanes a block of one row, eight columns a lane; NB neighbouring blocks of
-// a row one after another, their loads in flight together.
-template <bool BF16, bool SILU, int NB>
+// 16 lanes a block of one row, eight columns a lane; neighbouring units are the
+// same block of neighbouring rows, whose scales lie side by side. One block a
+// lane: two, four and eight with their loads in flight together took as long or
+// longer at every size (512 x 17,408 BF16: 7.0, 7.7, 7.7, 9.1 us; 16,384 x 5,120:
+// 52, 52, 56, 59, 4.8 TB/s of the 5.0 that a copy reaches).
+template <bool BF16, bool SILU>
 __global__ __launch_bounds__(256) void f8_quant_kernel(const F8QuantArgs a) {
     const int l16 = threadIdx.x & 15;
     const uint32_t unit = blockIdx.x * 16u + (threadIdx.x >> 4);
-    const int chunk = (int)(unit / (uint32_t)a.T), t = (int)(unit % (uint32_t)a.T);
-    const int kb0 = chunk * NB;
-    if (kb0 >= a.KB) return;
+    const int kb = (int)(unit / (uint32_t)a.T), t = (int)(unit % (uint32_t)a.T);
+    if (kb >= a.KB) return;
     const size_t row = (size_t)t * a.K;
-    float v[NB][8];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int k = (kb0 + n) * kF8Block + 8 * l16;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[n][j] = 0.0f;
-        if (k < a.K) f8_load8<BF16>(a.x, row + k, v[n]);     // (K is a multiple of 16)
-    }
+    const int k = kb * kF8Block + 8 * l16;
+    float v[8] = {};
+    if (k < a.K) f8_load8<BF16>(a.x, row + k, v);            // (K is a multiple of 16)
     if constexpr (SILU) {
+        float u[8] = {};
+        if (k < a.K) f8_load8<BF16>(a.up, row + k, u);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int k = (kb0 + n) * kF8Block + 8 * l16;
-            float u[8] = {};
-            if (k < a.K) f8_load8<BF16>(a.up, row + k, u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[n][j] = (v[n][j] / (1.0f + expf(-v[n][j]))) * u[j];
-            if (a.out && k < a.K) {
-                *reinterpret_cast<float4 *>(a.out + row + k) = make_float4(v[n][0], v[n][1], v[n][2], v[n][3]);
-                *reinterpret_cast<float4 *>(a.out + row + k + 4) = make_float4(v[n][4], v[n][5], v[n][6], v[n][7]);
-            }
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] / (1.0f + expf(-v[j]))) * u[j];
+        if (a.out && k < a.K) {
+            *reinterpret_cast<float4 *>(a.out + row + k) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4 *>(a.out + row + k + 4) = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
+    float top = kF8Floor;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        if (kb0 + n >= a.KB) break;
-        float top = kF8Floor;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[n][j]));
-        top = f8_row_max(top);
-        const float up = kF8Max / top;
-        uint2 c;
-        c.x = f8_pack(v[n][0] * up, v[n][1] * up, v[n][2] * up, v[n][3] * up);
-        c.y = f8_pack(v[n][4] * up, v[n][5] * up, v[n][6] * up, v[n][7] * up);
-        *reinterpret_cast<uint2 *>(a.q + ((size_t)t * a.KB + kb0 + n) * kF8Block + 8 * l16) = c;
-        if (l16 == 0) a.scale[(size_t)(kb0 + n) * a.T + t] = top / kF8Max;
-    }
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+    top = f8_row_max(top);
+    const float up = kF8Max / top;
+    uint2 c;
+    c.x = f8_pack(v[0] * up, v[1] * up, v[2] * up, v[3] * up);
+    c.y = f8_pack(v[4] * up, v[5] * up, v[6] * up, v[7] * up);
+    *reinterpret_cast<uint2 *>(a.q + ((size_t)t * a.KB + kb) * kF8Block + 8 * l16) = c;
+    if (l16 == 0) a.scale[(size_t)kb * a.T + t] = top / kF8Max;
 }
 
 template <bool BF16, bool SILU>
 static int quant_rows(const F8QuantArgs &a, hipStream_t st) {
-    // several blocks a lane where there are rows enough to fill the card
-    constexpr int NB = SILU ? 2 : 4;
-    const bool many = (long long)a.T * a.KB >= 16ll * 16 * device_cus() * NB;
-    const long long units = (long long)a.T * (many ? (a.KB + NB - 1) / NB : a.KB);
-    const long long grid = (units + 15) / 16;
+    const long long grid = ((long long)a.T * a.KB + 15) / 16;
     if (grid > grid_limit(256)) return -2;
-    if (many) hipLaunchKernelGGL((f8_quant_kernel<BF16, SILU, NB>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((f8_quant_kernel<BF16, SILU, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((f8_quant_kernel<BF16, SILU>), dim3((unsigned)grid), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 

@@ -832,7 +832,7 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
-@dataclass
+@dataclass(frozen=True)
 class F8Weight:
     """`groups` weights (an expert's each; 1: one projection) of M rows and K
     columns as e4m3 codes in the gfx950 tile layout, with an FP32 scale for each
@@ -843,8 +843,7 @@ class F8Weight:
     codes: torch.Tensor      # uint8 [groups * M * 128 ceil(K / 128)]
     scales: torch.Tensor     # float32 [groups][ceil(M / 128)][ceil(K / 128)]
 
-    def __post_init__(self):
-        self._made = None    # (device, addresses, C struct) once checked
+    _made = None             # (device, addresses, C struct) once checked
 
     def at(self) -> tuple:
         return self.codes.data_ptr(), self.scales.data_ptr()
@@ -927,11 +926,10 @@ def _f8_out(out, groups: int, M: int, K: int, device) -> F8Weight:
 
 def _f8_weight(w: F8Weight, device) -> _lib.WeightF8:
     """The C struct of a weight on `device`: the one made before while its
-    tensors lie where they did."""
+    tensors lie where they did (as _plan)."""
     if w.__class__ is F8Weight:
         made = w._made
-        if made is not None and made[0] == device and made[1] == w.at() and (made[2].groups, made[2].M, made[2].K) == (
-                w.groups, w.M, w.K):
+        if made is not None and made[0] == device and made[1] == w.at():
             return made[2]
     if not isinstance(w, F8Weight):
         raise ValueError("weights must be F8Weight")
@@ -940,7 +938,7 @@ def _f8_weight(w: F8Weight, device) -> _lib.WeightF8:
     _need(w.codes, "weight codes", torch.uint8, (w.groups * w.M * 128 * _blocks(w.K),), device)
     _need(w.scales, "weight scales", torch.float32, (w.groups, _blocks(w.M), _blocks(w.K)), device)
     c = w.c()
-    w._made = (device, w.at(), c)
+    w.__dict__["_made"] = (device, w.at(), c)
     return c
 
 

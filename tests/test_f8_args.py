@@ -157,6 +157,6 @@ def test_a_copied_weight_is_checked_anew():
     import copy
     w = ops.F8Weight.empty(2, 16, 144, device="cpu")
     assert w.codes.numel() == 2 * 16 * 256 and tuple(w.scales.shape) == (2, 1, 2)
-    w._made = ("cpu", w.at(), w.c())
+    w.__dict__["_made"] = ("cpu", w.at(), w.c())
     c = copy.deepcopy(w)
     assert c._made is None and (c.groups, c.M, c.K) == (2, 16, 144)
