@@ -412,8 +412,9 @@ int kxw4_quantize_act_f8(const void *x, int x_dtype, int T, int K, uint8_t *q, f
 int kxw4_silu_mul_quant_f8(float *out, const void *gate, const void *up, int dtype, int T, int K, uint8_t *q,
                            float *scale, void *stream);
 
-/* y[T][M] = the product (+ FP32 residual[T][M]) for up to 4 weights of one K
- * and groups = 1 over one activation. T may be 0. workspace:
+/* y[T][M] = the product (+ FP32 residual[T][M], for one weight; an FP32 y may be
+ * the residual) for up to 4 weights of one K and groups = 1 over one activation.
+ * T may be 0. workspace:
  * kxw4_gemm_f8_workspace bytes (asked with the call's device current; then it
  * may be NULL when that is 0), the call's own while it runs. 16-byte aligned
  * pointers (4 for scales). */

@@ -206,7 +206,8 @@ int kxw4_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, 
                  const float *residual, void *workspace, void *stream) {
     const int rc = check_product(ws, ys, count, a, 1, a ? a->T : 0, y_dtype);
     if (rc) return rc;
-    if (residual && (count != 1 || !aligned(residual, 16))) return KXW4_EARG;
+    // (an FP32 output may be the residual itself; a BF16 one would overwrite parts of it that are still to be read)
+    if (residual && (count != 1 || !aligned(residual, 16) || (y_dtype == KXW4_BF16 && ys[0] == residual))) return KXW4_EARG;
     if (a->T == 0) return KXW4_OK;
     if (!aligned(workspace, 16) || (!workspace && kxw4_gemm_f8_workspace(ws, count, a, y_dtype))) return KXW4_EARG;
     return product(ws, ys, count, a, y_dtype, residual, Rows{}, workspace, as_stream(stream));

@@ -279,9 +279,11 @@ __device__ __forceinline__ void f8_tiles(const F8GemmArgs &a, F8Tile tile, Next 
                                 *reinterpret_cast<v2u *>(slab + t16 * 64 + ((q ^ swz) * 16) + kg * 8) =
                                     v2u{pack_bf16(f[i][j][4 * q], f[i][j][4 * q + 1]), pack_bf16(f[i][j][4 * q + 2], f[i][j][4 * q + 3])};
                         }
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (other lanes' writes)
                         const int ts = tb + 16 * h + (lane >> 2), r = row + (lane & 3) * 8;
                         const v4u v = *reinterpret_cast<const v4u *>(slab + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) * 16));
                         if (ts < tile.t_end && r < M) *reinterpret_cast<v4u *>(static_cast<uint16_t *>(W.y) + (size_t)ts * M + r) = v;
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (their reads)
                     }
                 } else {
                     float *to = (part ? a.part + W.part + (size_t)tile.s * a.rows * M : static_cast<float *>(W.y)) + (size_t)t * M + row + 4 * kg;

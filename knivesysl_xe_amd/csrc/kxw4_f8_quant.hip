@@ -214,33 +214,46 @@ __global__ __launch_bounds__(256) void f8_transpose_kernel(const F8WeightArgs a,
     }
 }
 
-static dim3 f8_weight_grid(const F8WeightArgs &a, int groups) {
-    return dim3((unsigned)a.KB, (unsigned)a.MB, (unsigned)(groups < 1024 ? groups : 1024));
+// A work-group a block of 128 x 128, groups in turn where the blocks of all would
+// take 2^32 threads and more, which the runtime cuts without an error. False:
+// those of one group do.
+static bool f8_weight_grid(const F8WeightArgs &a, int groups, dim3 &grid) {
+    const long long most = grid_limit(256) / ((long long)a.KB * a.MB);
+    grid = dim3((unsigned)a.KB, (unsigned)a.MB, (unsigned)(groups < most ? groups : most));
+    return most > 0;
 }
 
 int launch_f8_pack(const uint8_t *codes, int groups, int M, int K, uint8_t *out, hipStream_t st) {
     const F8WeightArgs a{codes, out, nullptr, nullptr, M, K, f8_blocks(M), f8_blocks(K)};
-    hipLaunchKernelGGL(f8_pack_kernel<kF8Pack>, f8_weight_grid(a, groups), dim3(256), 0, st, a, groups);
+    dim3 grid;
+    if (!f8_weight_grid(a, groups, grid)) return -2;
+    hipLaunchKernelGGL(f8_pack_kernel<kF8Pack>, grid, dim3(256), 0, st, a, groups);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 int launch_f8_unpack(const uint8_t *tiles, int groups, int M, int K, uint8_t *codes, hipStream_t st) {
     const F8WeightArgs a{tiles, codes, nullptr, nullptr, M, K, f8_blocks(M), f8_blocks(K)};
-    hipLaunchKernelGGL(f8_pack_kernel<kF8Unpack>, f8_weight_grid(a, groups), dim3(256), 0, st, a, groups);
+    dim3 grid;
+    if (!f8_weight_grid(a, groups, grid)) return -2;
+    hipLaunchKernelGGL(f8_pack_kernel<kF8Unpack>, grid, dim3(256), 0, st, a, groups);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 int launch_f8_weight(const void *w, bool bf16, int groups, int M, int K, uint8_t *codes, float *scales, hipStream_t st) {
     const F8WeightArgs a{w, codes, nullptr, scales, M, K, f8_blocks(M), f8_blocks(K)};
-    if (bf16) hipLaunchKernelGGL(f8_weight_kernel<true>, f8_weight_grid(a, groups), dim3(256), 0, st, a, groups);
-    else hipLaunchKernelGGL(f8_weight_kernel<false>, f8_weight_grid(a, groups), dim3(256), 0, st, a, groups);
+    dim3 grid;
+    if (!f8_weight_grid(a, groups, grid)) return -2;
+    if (bf16) hipLaunchKernelGGL(f8_weight_kernel<true>, grid, dim3(256), 0, st, a, groups);
+    else hipLaunchKernelGGL(f8_weight_kernel<false>, grid, dim3(256), 0, st, a, groups);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 int launch_f8_transpose(const uint8_t *tiles, const float *scales, int groups, int M, int K, uint8_t *out, float *out_scales,
                         hipStream_t st) {
     const F8WeightArgs a{tiles, out, scales, out_scales, M, K, f8_blocks(M), f8_blocks(K)};
-    hipLaunchKernelGGL(f8_transpose_kernel, f8_weight_grid(a, groups), dim3(256), 0, st, a, groups);
+    dim3 grid;
+    if (!f8_weight_grid(a, groups, grid)) return -2;
+    hipLaunchKernelGGL(f8_transpose_kernel, grid, dim3(256), 0, st, a, groups);
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 

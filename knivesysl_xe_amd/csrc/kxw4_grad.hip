@@ -235,6 +235,7 @@ __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void grad_kernel(const GradArgs a
         const size_t base = (size_t)tile.grp * M * K;
         auto lines = [&](auto bytes, void *out, int m, int k) {          // the slab's rows to `out`
             constexpr int B = decltype(bytes)::value;        // of an output
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");               // (other lanes' writes)
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 const int r = it * 8 + (lane >> 3), c = lane & 7;
@@ -243,6 +244,7 @@ __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void grad_kernel(const GradArgs a
                 if (m + r < M && col < K)
                     *reinterpret_cast<v4u *>(static_cast<uint8_t *>(out) + (base + (size_t)(m + r) * K + col) * B) = v;
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");               // (their reads)
         };
 #pragma unroll
         for (int i = 0; i < AM; ++i) {

@@ -1066,9 +1066,12 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
     if outs is not None and len(outs) != n:
         raise ValueError(f"outs has {len(outs)} tensors for {n} weights")
     ys = [_out(N, w.M, dtype, dev, None if outs is None else outs[i], _OUTS[i]) for i, w in enumerate(ws)]
+    _residual(residual, T, ws[0].M, dev)
     for y in ys:
         if y.requires_grad:
             _detached(name)
+    if residual is not None and residual.requires_grad:
+        _detached(name)
     code = _dtype_code(dtype)
     nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, codes, code,
                        None if route is None else (route.T, route.k, route.groups, bool(sorted_rows)))
@@ -1077,7 +1080,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
     yarr = _POINTER_ARRAYS[n](*[y.data_ptr() for y in ys])
     at = scratch.data_ptr() if nbytes else None
     if route is None:
-        _launch("kxw4_gemm_f8", dev, warr, yarr, n, C.byref(ac), code, _ptr(_residual(residual, T, ws[0].M, dev)), at)
+        _launch("kxw4_gemm_f8", dev, warr, yarr, n, C.byref(ac), code, _ptr(residual), at)
     else:
         _launch("kxw4_expert_gemm_f8", dev, warr, yarr, n, C.byref(ac), plan, bool(sorted_rows), code, at)
     return ys
@@ -1093,7 +1096,8 @@ def gemm_f8_fanout(ws: Sequence[F8Weight], a, dtype=torch.float32, outs=None):
 
 
 def gemm_f8(w: F8Weight, a, dtype=torch.float32, residual=None, out=None) -> torch.Tensor:
-    """One weight of gemm_f8_fanout, plus an optional f32 residual [T][M]."""
+    """One weight of gemm_f8_fanout, plus an optional f32 residual [T][M], which
+    an f32 `out` may be."""
     return _f8_product("gemm_f8", [w], a, dtype, None if out is None else [out], residual, None, False)[0]
 
 

@@ -59,6 +59,7 @@ def test_product_refusals():
     assert gemm(ys=[2 * AT]) == arg                           # the rows' codes
     assert gemm(a=A(q=None, x=4 * AT)) == arg                 # the rows' values
     assert gemm([W(), W()], residual=AT) == arg and gemm(residual=AT + 4) == arg
+    assert gemm(residual=4 * AT, dtype=1) == arg              # a BF16 output over its residual
     assert gemm(a=A(T=0, q=None, scale=None)) == 0            # no rows: nothing is read or launched
     assert _lib.lib().kxw4_gemm_f8(None, None, 1, C.byref(A()), 0, None, None, None) == arg
     assert _lib.lib().kxw4_gemm_f8(array([W()]), (C.c_void_p * 1)(AT), 1, None, 0, None, None, None) == arg
