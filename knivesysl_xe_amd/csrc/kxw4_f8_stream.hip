@@ -10,6 +10,12 @@
 // the cut that the f8 MFMA makes (kxw4_f8_gemm.hpp), and the rate of either is
 // far above what the weights' stream needs. Rows that come as values are
 // quantized by each wave for the blocks it takes, which saves a launch.
+//
+// Bound: HBM, where there are weights enough (8 rows, 2 x 17,408 x 5,120: 178 MB
+// in 30 to 32 us, 5.6 to 5.9 TB/s; 16 x 8 rows over 64 experts, 2 x 1,024 x 5,120:
+// 582 MB, of which 499 from HBM, in 73 to 79 us; a pure read reaches 6.3); below
+// that the chain of round trips of one launch (one row, 4,096 x 4,096: 16.8 MB in
+// 8.1 us).
 #include "kxw4_f8.hpp"
 #include "kxw4_groups.hpp"
 

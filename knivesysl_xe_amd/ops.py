@@ -843,7 +843,7 @@ class F8Weight:
     codes: torch.Tensor      # uint8 [groups * M * 128 ceil(K / 128)]
     scales: torch.Tensor     # float32 [groups][ceil(M / 128)][ceil(K / 128)]
 
-    _made = None             # (device, addresses, C struct) once checked
+    _made = None             # (device, addresses, pointer to the C struct) once checked
 
     def at(self) -> tuple:
         return self.codes.data_ptr(), self.scales.data_ptr()
@@ -897,7 +897,7 @@ class F8Weight:
         """The transposed weights, the same values: gemm_f8 of them and of dy's
         rows is the gradient of the projection's input."""
         dev = self.codes.device
-        ref = C.byref(_f8_weight(self, dev))
+        ref = _f8_weight(self, dev)
         o = _f8_out(out, self.groups, self.K, self.M, dev)
         _launch("kxw4_transpose_weight_f8", dev, ref, o.codes.data_ptr(), o.scales.data_ptr())
         return o
@@ -905,7 +905,7 @@ class F8Weight:
     def unpack(self):
         """(codes as float8_e4m3fn [groups][M][K], scales)."""
         dev = self.codes.device
-        ref = C.byref(_f8_weight(self, dev))
+        ref = _f8_weight(self, dev)
         codes = torch.empty(self.groups, self.M, self.K, dtype=torch.uint8, device=dev)
         _launch("kxw4_unpack_weight_f8", dev, ref, codes.data_ptr())
         return codes.view(torch.float8_e4m3fn), self.scales
@@ -924,9 +924,9 @@ def _f8_out(out, groups: int, M: int, K: int, device) -> F8Weight:
     return out
 
 
-def _f8_weight(w: F8Weight, device) -> _lib.WeightF8:
-    """The C struct of a weight on `device`: the one made before while its
-    tensors lie where they did (as _plan)."""
+def _f8_weight(w: F8Weight, device):
+    """The C struct of a weight on `device`, by reference: the one made before
+    while its tensors lie where they did (as _plan)."""
     if w.__class__ is F8Weight:
         made = w._made
         if made is not None and made[0] == device and made[1] == w.at():
@@ -937,9 +937,9 @@ def _f8_weight(w: F8Weight, device) -> _lib.WeightF8:
         raise ValueError("weights must be on the GPU")
     _need(w.codes, "weight codes", torch.uint8, (w.groups * w.M * 128 * _blocks(w.K),), device)
     _need(w.scales, "weight scales", torch.float32, (w.groups, _blocks(w.M), _blocks(w.K)), device)
-    c = w.c()
-    w.__dict__["_made"] = (device, w.at(), c)
-    return c
+    ref = C.pointer(w.c())
+    w.__dict__["_made"] = (device, w.at(), ref)
+    return ref
 
 
 @dataclass
@@ -1030,7 +1030,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
     if not 1 <= n <= 4:
         raise ValueError(f"one to four weights, got {n}")
     dev = ws[0].codes.device
-    cs = [_f8_weight(w, dev) for w in ws]
+    refs = [_f8_weight(w, dev) for w in ws]
     plan = None
     if route is not None:
         plan = _plan(route, dev)
@@ -1067,16 +1067,13 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         raise ValueError(f"outs has {len(outs)} tensors for {n} weights")
     ys = [_out(N, w.M, dtype, dev, None if outs is None else outs[i], _OUTS[i]) for i, w in enumerate(ws)]
     _residual(residual, T, ws[0].M, dev)
-    for y in ys:
-        if y.requires_grad:
-            _detached(name)
-    if residual is not None and residual.requires_grad:
+    if any([y.requires_grad for y in ys]) or (residual is not None and residual.requires_grad):
         _detached(name)
     code = _dtype_code(dtype)
     nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, codes, code,
                        None if route is None else (route.T, route.k, route.groups, bool(sorted_rows)))
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    warr = _F8_ARRAYS[n](*[C.pointer(c) for c in cs])
+    warr = _F8_ARRAYS[n](*refs)
     yarr = _POINTER_ARRAYS[n](*[y.data_ptr() for y in ys])
     at = scratch.data_ptr() if nbytes else None
     if route is None:
