@@ -155,4 +155,14 @@ __device__ __forceinline__ float clampf(float x, float lo, float hi) {
     return fminf(fmaxf(x, lo), hi);
 }
 
+// A non-temporal store. (Between empty asm statements: beside a plain store of
+// the same value in another branch the compiler would make one plain store of
+// both.)
+template <class V>
+__device__ __forceinline__ void store_past(const V &v, V *to) {
+    asm volatile("");
+    __builtin_nontemporal_store(v, to);
+    asm volatile("");
+}
+
 }  // namespace kxw4

@@ -100,6 +100,11 @@ int launch_f8_gemm(F8GemmArgs &a, hipStream_t st) {
             outputs += (long long)a.rows * a.w[i].M;
         }
         if (a.splits == 1) a.part = nullptr;
+        // Outputs of twice the L2s (4 MB an XCD) and more go past them, which leaves
+        // them to the codes: 8,192 rows, 1,024 -> 16,384 (268 MB): 168 us, else 221;
+        // 4,096 -> 16,384: 487, 504; 2 x 17,408 of 3,965 rows: 685, 697; 33 MB: as
+        // long. (By group 1,024 -> 5,120 took 313 us so, else 291.)
+        a.stream = outputs * 2 >= 64ll << 20;
         const int rc = f8_config(a, c.id, st);
         if (rc || a.splits == 1) return rc;
         const long long grid = (outputs / 4 + 255) / 256;

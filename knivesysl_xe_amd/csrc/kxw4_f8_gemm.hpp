@@ -293,7 +293,11 @@ __device__ __forceinline__ void f8_tiles(const F8GemmArgs &a, F8Tile tile, Next 
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (other lanes' writes)
                         const int ts = tb + 16 * h + (lane >> 2), r = row + (lane & 3) * 8;
                         const v4u v = *reinterpret_cast<const v4u *>(slab + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) * 16));
-                        if (ts < tile.t_end && r < M) *reinterpret_cast<v4u *>(static_cast<uint16_t *>(W.y) + (size_t)ts * M + r) = v;
+                        if (ts < tile.t_end && r < M) {
+                            v4u *to = reinterpret_cast<v4u *>(static_cast<uint16_t *>(W.y) + (size_t)ts * M + r);
+                            if (!GRP && a.stream) store_past(v, to);
+                            else *to = v;
+                        }
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (their reads)
                     }
                 } else {

@@ -227,7 +227,10 @@ __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void grad_kernel(const GradArgs a
     // 4 (l/32) + r%4 of the lane's row. 32 rows at a time pass the wave's own slab
     // in LDS (rows of 128 bytes, 16-byte chunk c of row m at c ^ (m % 8)) and go
     // out as whole lines: stores of 32 bytes a row reached 2.1 TB/s of BF16, these
-    // 8 times 128 bytes a store ----
+    // 8 times 128 bytes a store. Non-temporal, which leaves the L2s to dy and x (64
+    // groups of 256 rows, 1,024 x 2,048, BF16: 136 us for 153; 2,048 rows, 5,120 x
+    // 5,120: 136 for 141), but for parts of a sum, which are read again at once
+    // (8,192 rows, 512 x 512: 22.4 us for 21.0) ----
     const int m32 = lane & 31, kg = lane >> 5;
     const size_t outputs = (size_t)a.groups * M * K;
     uint8_t *slab = smem + NST * STAGE + wave * S::SLAB;
@@ -241,8 +244,11 @@ __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void grad_kernel(const GradArgs a
                 const int r = it * 8 + (lane >> 3), c = lane & 7;
                 const v4u v = *reinterpret_cast<const v4u *>(slab + r * 128 + ((c ^ (r & 7)) * 16));
                 const int col = k + c * (16 / B);
-                if (m + r < M && col < K)
-                    *reinterpret_cast<v4u *>(static_cast<uint8_t *>(out) + (base + (size_t)(m + r) * K + col) * B) = v;
+                if (m + r < M && col < K) {
+                    v4u *to = reinterpret_cast<v4u *>(static_cast<uint8_t *>(out) + (base + (size_t)(m + r) * K + col) * B);
+                    if (a.splits > 1) *to = v;
+                    else store_past(v, to);
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");               // (their reads)
         };

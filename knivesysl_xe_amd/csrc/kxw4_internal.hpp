@@ -283,7 +283,7 @@ struct F8GemmArgs {
     const int *offsets, *order;
     int N, groups, k;
     float *part;                      // scratch of f8_gemm_scratch bytes
-    int n_tiles, splits;              // (set by the launcher)
+    int n_tiles, splits, stream;      // (set by the launcher; stream: non-temporal BF16 stores)
 };
 size_t f8_gemm_scratch(const F8GemmArgs &a);
 int launch_f8_gemm(F8GemmArgs &a, hipStream_t st);
