@@ -15,9 +15,9 @@
 // 1,265 TF): the matrix units, at the clock that the power limit leaves them, for
 // many rows of a group (4,096 rows, 5,120 x 5,120, FP32 out: 224 us, 957 TF; 2,048
 // rows, 17,408 x 5,120, BF16 out: 345 us, 1,058 TF); the last round of tiles where
-// these are few (2,048 rows, 5,120 x 5,120: 400 tiles on 256 CUs, 143 us, 749 TF);
-// the stores where a group has few rows (64 groups of 256 rows, 1,024 x 2,048,
-// BF16 out: 150 us, 457 TF). A first version with a tile per work-group and 32-byte
+// these are few (2,048 rows, 5,120 x 5,120: 400 tiles on 256 CUs, 136 to 143 us,
+// 749 TF and more); the stores where a group has few rows (64 groups of 256 rows,
+// 1,024 x 2,048, BF16 out: 134 us, 512 TF). A first version with a tile per work-group and 32-byte
 // stores took 177 us for the 2,048 rows and 290 for 8 groups of 1,000 rows, 2,048 x
 // 4,096 (now 168: 800 TF).
 #include "kxw4_device.hpp"
@@ -452,7 +452,7 @@ int launch_grad(GradArgs &a, hipStream_t st) {
     // 256 x 256 outputs a work-group read half the bytes of 128 x 128 from LDS and
     // the caches; they need a tile for each CU. Measured on 256 CUs (this, then
     // 128 x 128, us): 4,096 rows 5,120 x 5,120 224 / 241; 2,048 rows 17,408 x 5,120
-    // 345 / 388; 64 groups of 256 rows 1,024 x 2,048 150 / 167; 16 groups of 512
+    // 345 / 388; 64 groups of 256 rows 1,024 x 2,048 150 / 167 (134 now); 16 groups of 512
     // rows 63 / 62.
     const long long big = (long long)a.groups * ((a.M + 255) / 256) * ((a.K + 255) / 256);
     const int rc = a.splits == 1 && big >= device_cus() ? grad_launch<4, 2, 2, 4, 4, 2>(a, st)

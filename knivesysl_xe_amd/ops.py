@@ -873,6 +873,8 @@ class F8Weight:
         groups, (M, K) = codes.shape[0] if codes.dim() == 3 else 1, codes.shape[-2:]
         w = cls.empty(groups, M, K, dev)
         _need(scales, "scales", torch.float32, codes.shape[:-2] + (_blocks(M), _blocks(K)), dev)
+        if scales.requires_grad:
+            _detached("F8Weight.from_codes")
         w.scales.copy_(scales.view_as(w.scales))
         _launch("kxw4_pack_weight_f8", dev, codes.data_ptr(), groups, M, K, w.codes.data_ptr())
         return w

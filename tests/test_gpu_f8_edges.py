@@ -48,6 +48,9 @@ def test_residuals_that_are_refused():
         ops.gemm_f8(w, x, residual=r.clone().requires_grad_())
     with pytest.raises(ValueError, match="residual must be torch.float32"):
         ops.gemm_f8(w, x, residual=r.to(BF16))
+    codes, scales = [t[0] for t in exact_weight(1, 32, 128, 1)]
+    with pytest.raises(ValueError, match="records no gradient"):
+        ops.F8Weight.from_codes(codes, scales.clone().requires_grad_())
 
 
 def test_gradients_on_two_streams_at_once():
