@@ -85,9 +85,10 @@ Way way_of(const F8GemmArgs &x, const kxw4_act_f8_t *a) {
     F8Sizes s{device_cus(), x.groups ? x.N : x.rows, x.KB, x.count, {}, x.groups, x.y_bf16 != 0};
     for (int i = 0; i < x.count; ++i) s.M[i] = x.w[i].M;
     Way w{f8_stream_rows(s), false};
-    // (the stream kernel takes values with 32-bit offsets, in tiles of 16)
+    // (the stream kernel takes values with 32-bit offsets)
     if (!a->q)
-        w.quantizes = !(w.rows == 16 && f8_stream_quantizes(s) && (long long)a->T * a->K * elem_bytes(a->x_dtype) < (1ll << 31));
+        w.quantizes = !(w.rows && (w.rows == 16 ? f8_stream_quantizes(s) : f8_stream32_quantizes(s, elem_bytes(a->x_dtype))) &&
+                        (long long)a->T * a->K * elem_bytes(a->x_dtype) < (1ll << 31));
     return w;
 }
 

@@ -19,6 +19,11 @@ inline long long f8_row_groups(const F8Sizes &s) {
     return rgs;
 }
 
+// Tiles of 32 rows, at most, of all groups.
+inline long long f8_tiles32(const F8Sizes &s) {
+    return s.groups ? s.rows / 32 + std::min<long long>(s.rows, s.groups) : (s.rows + 31) / 32;
+}
+
 // Rows of a stream tile (16 or 32; kxw4_f8_stream.hip), 0 for the large tiles.
 // Up to 16 rows a weight the weights' stream bounds the product and one tile
 // reads it once (16 rows, 5120 x 5120: 9.8 us, large tiles 13; 128 rows over 64
@@ -29,8 +34,7 @@ inline long long f8_row_groups(const F8Sizes &s) {
 inline int f8_stream_rows(const F8Sizes &s) {
     const long long groups = std::max(s.groups, 1);
     if (s.rows <= 16 * groups) return 16;
-    const long long tiles = s.groups ? s.rows / 32 + std::min<long long>(s.rows, groups) : (s.rows + 31) / 32;
-    return tiles * f8_row_groups(s) * s.kb <= 13000 ? 32 : 0;
+    return f8_tiles32(s) * f8_row_groups(s) * s.kb <= 13000 ? 32 : 0;
 }
 
 // Whether the stream kernel quantizes values itself: each wave does so for the
@@ -40,6 +44,19 @@ inline int f8_stream_rows(const F8Sizes &s) {
 inline bool f8_stream_quantizes(const F8Sizes &s) {
     const long long used = s.groups ? std::min(s.rows, s.groups) : 1;
     return used * f8_row_groups(s) * s.kb <= (32ll << 20) / 2048;
+}
+
+// The same in tiles of 32 rows, of x_bytes a value: where the four waves hold all
+// blocks of FP32 rows in flight (BF16: half of them), and the work-groups' reads of
+// the same rows are few. Launches of both, then of one, replayed / called in turn:
+// FP32, 256 rows, 1,024 x 1,024: 8.9 / 12.0, then 9.6 / 8.1; 200, 768 -> 1,024: 8.7 /
+// 12.2, 9.0 / 8.0; 150 x 3 rows over 5 experts, 208 -> 336: 8.2 / 12.2, 6.6 / 8.7;
+// past it 64 rows, 2,048 x 2,048: 9.9 / 11.8, 12.8 / 11.1; 97, 1,456 -> 2,064: 11.5 /
+// 11.9, 14.4 / 12.9. BF16, 97 rows, 1,456 -> 2,064: 11.4 / 11.8, 11.5 / 9.9; 64 x 4
+// over 8, 1,024 x 1,024: 11.4 / 12.5, 10.9 / 9.2; past it 32 rows, 4,096 x 4,096:
+// 12.8 / 11.8, 14.4 / 12.9.
+inline bool f8_stream32_quantizes(const F8Sizes &s, int x_bytes) {
+    return s.kb * x_bytes <= 32 && f8_tiles32(s) * f8_row_groups(s) * s.kb * x_bytes <= 17500;
 }
 
 // The tiles of the dense launch and what a step (128 columns) of one takes, in

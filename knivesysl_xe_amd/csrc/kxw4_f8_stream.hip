@@ -277,8 +277,8 @@ static int f8_stream_shape(F8StreamArgs &a, hipStream_t st) {
 
 template <bool GRP>
 static int f8_stream_rows(F8StreamArgs &a, int x, int rows, hipStream_t st) {
-    if (x == kF8Bf16) return f8_stream_shape<1, kF8Bf16, GRP>(a, st);
-    if (x == kF8F32) return f8_stream_shape<1, kF8F32, GRP>(a, st);
+    if (x == kF8Bf16) return rows == 16 ? f8_stream_shape<1, kF8Bf16, GRP>(a, st) : f8_stream_shape<2, kF8Bf16, GRP>(a, st);
+    if (x == kF8F32) return rows == 16 ? f8_stream_shape<1, kF8F32, GRP>(a, st) : f8_stream_shape<2, kF8F32, GRP>(a, st);
     return rows == 16 ? f8_stream_shape<1, kF8Codes, GRP>(a, st) : f8_stream_shape<2, kF8Codes, GRP>(a, st);
 }
 

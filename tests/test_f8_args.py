@@ -67,13 +67,15 @@ def test_product_refusals():
 
 def test_rows_of_values_ask_for_scratch():
     L = _lib.lib()
-    a = A(T=1000, q=None, scale=None, x=2 * AT)
-    assert L.kxw4_gemm_f8_workspace(array([W()]), 1, C.byref(a), 0) >= 1000 * 512 + 4 * 1000 * 4
-    assert gemm(a=a, ws_at=None) == _lib.EARG and gemm(a=a, ws_at=AT + 8) == _lib.EARG
+    a, w = A(T=1000, q=None, scale=None, x=2 * AT), W(M=1024)
+    assert L.kxw4_gemm_f8_workspace(array([w]), 1, C.byref(a), 0) >= 1000 * 512 + 4 * 1000 * 4
+    assert gemm([w], a=a, ws_at=None) == _lib.EARG and gemm([w], a=a, ws_at=AT + 8) == _lib.EARG
+    # (a short launch quantizes by itself)
+    assert L.kxw4_gemm_f8_workspace(array([W()]), 1, C.byref(a), 0) == 0
     assert L.kxw4_gemm_f8_workspace(array([W()]), 1, C.byref(A(T=0)), 0) == 0
-    e = W(groups=4)
+    e = W(M=1024, groups=4)
     assert L.kxw4_expert_gemm_f8_workspace(array([e]), 1, C.byref(a), C.byref(R(T=1000)), 0, 0) >= 1000 * 512
-    assert expert(a=a, r=R(T=1000), ws_at=None) == _lib.EARG
+    assert expert(w=e, a=a, r=R(T=1000), ws_at=None) == _lib.EARG
 
 
 def test_expert_product_refusals():

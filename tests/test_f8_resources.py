@@ -7,7 +7,7 @@ def test_the_tiles_keep_nothing_in_scratch(records):  # noqa: F811
     # a value kept in private memory is waited for together with the loads into LDS, which are meant to stay in flight
     mine = [k for k in records if any(n in k[".name"] for n in ("f8_gemm_kernel", "f8_group_kernel", "f8_stream_kernel",
                                                               "4kxw411grad_kernel"))]
-    assert len(mine) >= 6 + 4 + 16 + 2
+    assert len(mine) >= 6 + 4 + 24 + 2
     bad = {k[".name"]: k[".private_segment_fixed_size"] for k in mine if k[".private_segment_fixed_size"]}
     assert not bad
 

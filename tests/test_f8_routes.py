@@ -23,6 +23,7 @@ def rules(tmp_path_factory):
                    '}\n'
                    'extern "C" int stream(int rows, int K, int count, int M, int groups) { return f8_stream_rows(sizes(rows, K, count, M, groups, 1)); }\n'
                    'extern "C" int fused(int rows, int K, int count, int M, int groups) { return f8_stream_quantizes(sizes(rows, K, count, M, groups, 1)); }\n'
+                   'extern "C" int fused32(int rows, int K, int M, int groups, int bytes) { return f8_stream32_quantizes(sizes(rows, K, 1, M, groups, 1), bytes); }\n'
                    'extern "C" int longer(int rows, int groups) { return f8_long_groups(sizes(rows, 128, 1, 128, groups, 1)); }\n'
                    'extern "C" int choose(int rows, int K, int count, int M, int bf16, int *splits) {\n'
                    '    const F8Choice c = f8_choose(sizes(rows, K, count, M, 0, bf16));\n'
@@ -52,6 +53,14 @@ def test_small_weights_are_streamed_by_one_launch(rules):
     assert rules.fused(1, 4096, 1, 4096, 0) and rules.fused(4, 1024, 1, 5120, 32)
     assert not rules.fused(1, 17408, 1, 5120, 0) and not rules.fused(8, 5120, 2, 17408, 0)
     assert not rules.fused(128, 5120, 2, 1024, 64)
+
+
+def test_short_launches_of_32_rows_quantize_by_themselves(rules):
+    # rows, K, M, groups
+    for case, f32, bf16 in (((256, 1024, 1024, 0), 1, 1), ((200, 768, 1024, 0), 1, 1), ((450, 208, 336, 5), 1, 1),
+                            ((64, 2048, 2048, 0), 0, 1), ((97, 1456, 2064, 0), 0, 1), ((256, 1024, 1024, 8), 0, 1),
+                            ((32, 4096, 4096, 0), 0, 0), ((32, 5120, 5120, 0), 0, 0)):
+        assert (rules.fused32(*case, 4), rules.fused32(*case, 2)) == (f32, bf16), case
 
 
 def test_dense_tiles(rules):
