@@ -417,7 +417,8 @@ int kxw4_silu_mul_quant_f8(float *out, const void *gate, const void *up, int dty
  * T may be 0. workspace:
  * kxw4_gemm_f8_workspace bytes (asked with the call's device current; then it
  * may be NULL when that is 0), the call's own while it runs. 16-byte aligned
- * pointers (4 for scales). */
+ * pointers (4 for scales). Outputs overlap nothing else that a call reads or
+ * writes (here and below). */
 size_t kxw4_gemm_f8_workspace(const kxw4_weight_f8_t *const *ws, int count, const kxw4_act_f8_t *a, int y_dtype);
 int kxw4_gemm_f8(const kxw4_weight_f8_t *const *ws, void *const *ys, int count, const kxw4_act_f8_t *a, int y_dtype,
                  const float *residual, void *workspace, void *stream);

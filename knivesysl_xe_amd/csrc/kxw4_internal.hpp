@@ -263,7 +263,7 @@ struct F8StreamArgs {
     int N, groups, k;
     int row_blocks;                   // (set by the launcher)
 };
-// x: what the rows come as (codes, BF16, FP32); rows: of a tile, 16 or (codes) 32
+// x: what the rows come as (codes, BF16, FP32); rows: of a tile, 16 or 32
 int launch_f8_stream(F8StreamArgs &a, int x, int rows, hipStream_t st);
 
 struct F8GemmWeight {
