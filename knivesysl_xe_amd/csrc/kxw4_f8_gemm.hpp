@@ -433,7 +433,8 @@ __device__ __forceinline__ void f8_tiles(const F8GemmArgs &a, F8Tile tile, Next 
             clear();
         }
     } else {
-        for (;;) {
+        auto steps = [&](auto NA) {
+            constexpr int N = decltype(NA)::value;
             for (int kb = tile.k0; kb < tile.k1; ++kb) {
                 arrive();
                 issue(st == 0 ? NST - 1 : st - 1);
@@ -444,8 +445,7 @@ __device__ __forceinline__ void f8_tiles(const F8GemmArgs &a, F8Tile tile, Next 
 #pragma unroll
                 for (int j = 0; j < TB; ++j) read_w(base, j, w[j]);
 #pragma unroll
-                for (int i = 0; i < TA; ++i) {
-                    if (i >= na) continue;
+                for (int i = 0; i < N; ++i) {
                     v4u x[4];
                     read_x(base, i, x);
                     const float s = read_s(base, i) * g;
@@ -463,6 +463,10 @@ __device__ __forceinline__ void f8_tiles(const F8GemmArgs &a, F8Tile tile, Next 
                 }
                 st = st == NST - 1 ? 0 : st + 1;
             }
+        };
+        for (;;) {
+            if (TA != 2 || na == 2) steps(std::integral_constant<int, TA>{});
+            else steps(std::integral_constant<int, 1>{});
             store();
             if (!more) break;
             tile = ahead;
