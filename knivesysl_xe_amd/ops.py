@@ -1014,12 +1014,13 @@ _F8_ARRAYS = tuple(C.POINTER(_lib.WeightF8) * n for n in range(5))
 
 
 @functools.lru_cache(maxsize=4096)
-def _f8_bytes(device: int, Ms: tuple, K: int, T: int, codes: bool, dtype: int, plan: Optional[tuple]) -> int:
-    """Scratch of a product on a device (it goes by the CUs)."""
+def _f8_bytes(device: int, Ms: tuple, K: int, T: int, x: Optional[int], dtype: int, plan: Optional[tuple]) -> int:
+    """Scratch of a product on a device (it goes by the CUs); x: the values'
+    type, None for codes."""
     groups = plan[2] if plan else 1
     ws = [_lib.WeightF8(groups, M, K) for M in Ms]
     warr = _F8_ARRAYS[len(ws)](*[C.pointer(w) for w in ws])
-    a = _lib.ActF8(T, K, 0, 1 if codes else None)
+    a = _lib.ActF8(T, K, x or 0, 1 if x is None else None)
     with torch.cuda.device(device):
         if plan:
             r = _lib.Route(plan[0], plan[1], groups)
@@ -1045,7 +1046,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         T, K = a.T, a.K
         _check_act_f8(a, dev)
         ac = _lib.ActF8(T, K, 0, a.q.data_ptr(), a.scale.data_ptr(), None)
-        codes = True
+        xt = None
     else:
         if not isinstance(a, torch.Tensor) or a.dim() != 2:
             raise ValueError("the activation must be a QuantActF8 or a tensor (T, K)")
@@ -1055,7 +1056,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         if a.requires_grad:
             _detached(name)
         ac = _lib.ActF8(T, K, _DTYPE_CODES[a.dtype], None, None, a.data_ptr())
-        codes = False
+        xt = ac.x_dtype
     if T > _MAX_SLOTS:
         raise ValueError(f"up to 2^30 rows, got {T}")
     if route is None:
@@ -1072,7 +1073,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
     if any([y.requires_grad for y in ys]) or (residual is not None and residual.requires_grad):
         _detached(name)
     code = _dtype_code(dtype)
-    nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, codes, code,
+    nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, xt, code,
                        None if route is None else (route.T, route.k, route.groups, bool(sorted_rows)))
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     warr = _F8_ARRAYS[n](*refs)
