@@ -19,9 +19,9 @@ inline long long f8_row_groups(const F8Sizes &s) {
     return rgs;
 }
 
-// Tiles of 32 rows, at most, of all groups.
-inline long long f8_tiles32(const F8Sizes &s) {
-    return s.groups ? s.rows / 32 + std::min<long long>(s.rows, s.groups) : (s.rows + 31) / 32;
+// Tiles of `rows` rows, at most, of all groups.
+inline long long f8_tiles_of(const F8Sizes &s, int rows) {
+    return s.groups ? s.rows / rows + std::min(s.rows, s.groups) : (s.rows + rows - 1) / rows;
 }
 
 // Rows of a stream tile (16 or 32; kxw4_f8_stream.hip), 0 for the large tiles.
@@ -34,7 +34,7 @@ inline long long f8_tiles32(const F8Sizes &s) {
 inline int f8_stream_rows(const F8Sizes &s) {
     const long long groups = std::max(s.groups, 1);
     if (s.rows <= 16 * groups) return 16;
-    return f8_tiles32(s) * f8_row_groups(s) * s.kb <= 13000 ? 32 : 0;
+    return f8_tiles_of(s, 32) * f8_row_groups(s) * s.kb <= 13000 ? 32 : 0;
 }
 
 // Whether the stream kernel quantizes values itself: each wave does so for the
@@ -56,7 +56,20 @@ inline bool f8_stream_quantizes(const F8Sizes &s) {
 // over 8, 1,024 x 1,024: 11.4 / 12.5, 10.9 / 9.2; past it 32 rows, 4,096 x 4,096:
 // 12.8 / 11.8, 14.4 / 12.9.
 inline bool f8_stream32_quantizes(const F8Sizes &s, int x_bytes) {
-    return s.kb * x_bytes <= 32 && f8_tiles32(s) * f8_row_groups(s) * s.kb * x_bytes <= 17500;
+    return s.kb * x_bytes <= 32 && f8_tiles_of(s, 32) * f8_row_groups(s) * s.kb * x_bytes <= 17500;
+}
+
+// A stream work-group's row-groups and waves, for tiles of `rows` rows: two
+// row-groups, or one where they do not fill the CUs; four waves, or eight for long
+// sums of few work-groups (codes, one row: 5120 x 17408 19 us for 25, 17408 x 5120
+// 33 for 35, 4096 x 4096 6.2 either way).
+struct F8StreamShape {
+    int row_groups, waves;
+};
+inline F8StreamShape f8_stream_shape(const F8Sizes &s, int rows) {
+    const long long rgs = f8_tiles_of(s, rows) * f8_row_groups(s);
+    if (rgs <= s.cus) return {1, 4};
+    return {2, s.kb >= 64 && rgs < 4ll * s.cus ? 8 : 4};
 }
 
 // The tiles of the dense launch and what a step (128 columns) of one takes, in

@@ -17,6 +17,7 @@
 // that the chain of round trips of one launch (one row, 4,096 x 4,096: 16.8 MB in
 // 8.1 us).
 #include "kxw4_f8.hpp"
+#include "kxw4_f8_route.hpp"
 #include "kxw4_groups.hpp"
 
 namespace kxw4 {
@@ -261,29 +262,23 @@ static int f8_stream(F8StreamArgs &a, int nw, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-// Two row-groups a work-group, or one where they do not fill the CUs; four waves,
-// or eight for long sums of few work-groups (codes, one row: 5120 x 17408 19 us
-// for 25, 17408 x 5120 33 for 35, 4096 x 4096 6.2 either way).
 template <int TB, int X, bool GRP>
-static int f8_stream_shape(F8StreamArgs &a, hipStream_t st) {
-    long long rgs = 0;
-    for (int i = 0; i < a.count; ++i) rgs += a.w[i].M / 16;
-    rgs *= GRP ? tiles_at_most(a.N, a.groups, 16 * TB) : (a.rows + 16 * TB - 1) / (16 * TB);
-    const long long cus = device_cus();
-    if (rgs <= cus) return f8_stream<1, TB, X, GRP, 2>(a, 4, st);
-    if (a.KB >= 64 && rgs < 4 * cus) return f8_stream<2, TB, X, GRP, 2>(a, 8, st);
-    return f8_stream<2, TB, X, GRP, 2>(a, 4, st);
+static int f8_stream_shaped(F8StreamArgs &a, hipStream_t st) {
+    F8Sizes s{device_cus(), GRP ? a.N : a.rows, a.KB, a.count, {}, a.groups, a.y_bf16 != 0};
+    for (int i = 0; i < a.count; ++i) s.M[i] = a.w[i].M;
+    const F8StreamShape shape = f8_stream_shape(s, 16 * TB);
+    return shape.row_groups == 1 ? f8_stream<1, TB, X, GRP, 2>(a, shape.waves, st) : f8_stream<2, TB, X, GRP, 2>(a, shape.waves, st);
 }
 
 template <bool GRP>
-static int f8_stream_rows(F8StreamArgs &a, int x, int rows, hipStream_t st) {
-    if (x == kF8Bf16) return rows == 16 ? f8_stream_shape<1, kF8Bf16, GRP>(a, st) : f8_stream_shape<2, kF8Bf16, GRP>(a, st);
-    if (x == kF8F32) return rows == 16 ? f8_stream_shape<1, kF8F32, GRP>(a, st) : f8_stream_shape<2, kF8F32, GRP>(a, st);
-    return rows == 16 ? f8_stream_shape<1, kF8Codes, GRP>(a, st) : f8_stream_shape<2, kF8Codes, GRP>(a, st);
+static int f8_stream_typed(F8StreamArgs &a, int x, int rows, hipStream_t st) {
+    if (x == kF8Bf16) return rows == 16 ? f8_stream_shaped<1, kF8Bf16, GRP>(a, st) : f8_stream_shaped<2, kF8Bf16, GRP>(a, st);
+    if (x == kF8F32) return rows == 16 ? f8_stream_shaped<1, kF8F32, GRP>(a, st) : f8_stream_shaped<2, kF8F32, GRP>(a, st);
+    return rows == 16 ? f8_stream_shaped<1, kF8Codes, GRP>(a, st) : f8_stream_shaped<2, kF8Codes, GRP>(a, st);
 }
 
 int launch_f8_stream(F8StreamArgs &a, int x, int rows, hipStream_t st) {
-    return a.groups ? f8_stream_rows<true>(a, x, rows, st) : f8_stream_rows<false>(a, x, rows, st);
+    return a.groups ? f8_stream_typed<true>(a, x, rows, st) : f8_stream_typed<false>(a, x, rows, st);
 }
 
 }  // namespace kxw4

@@ -1,5 +1,5 @@
-"""Shapes that reach each kernel of the large tiles of the 8-bit floating tier, on 256 CUs. test_f8_coverage.py holds them to
-the rules of csrc/kxw4_f8_route.hpp; the GPU tests of test_gpu_f8_tiles.py run them."""
+"""Shapes that reach each kernel of the products of the 8-bit floating tier, on 256 CUs. test_f8_coverage.py holds them to the
+rules of csrc/kxw4_f8_route.hpp; the GPU tests of test_gpu_f8_tiles.py and test_gpu_f8_stream.py run them."""
 
 CUS = 256
 
@@ -32,6 +32,17 @@ GROUPED = {
 }
 # Weights past 2^32 bytes, by group: groups, K, M, and the rows of one slot each that make their runs short or long
 PAST_32 = (70, 16384, 4096, {"short": 1200, "long": 9000})
+
+# The kernel for few rows: rows of a tile, row-groups and waves of a work-group -> shapes (T, k, groups, K, the weights' M),
+# groups 0 for one weight
+STREAM = {
+    (16, 1, 4): [(1, 1, 0, 400, (272,)), (16, 1, 0, 1040, (144, 272)), (5, 2, 9, 400, (144,)), (16, 1, 0, 8208, (272,))],
+    (16, 2, 4): [(1, 1, 0, 400, (4112,)), (15, 1, 0, 528, (4112, 4240)), (9, 1, 0, 2064, (8208,)), (8, 1, 0, 5136, (8208, 16, 4112)),
+                 (7, 4, 30, 400, (272,)), (60, 8, 64, 1040, (528, 272))],
+    (16, 2, 8): [(13, 1, 0, 8208, (4112,)), (1, 1, 0, 14992, (5136,)), (4, 2, 8, 8208, (528,)), (16, 1, 16, 8192, (256,))],
+    (32, 1, 4): [(33, 1, 0, 400, (272,)), (17, 1, 0, 2064, (1040,)), (50, 2, 3, 336, (272,))],
+    (32, 2, 4): [(130, 1, 0, 400, (1040,)), (97, 1, 0, 1456, (2064,)), (100, 3, 5, 400, (528,)), (100, 3, 5, 400, (528, 16, 272))],
+}
 
 
 def cases(table):
