@@ -888,9 +888,9 @@ class F8Weight:
             raise ValueError(f"w must have shape (M, K) or (groups, M, K), got {tuple(w.shape)}")
         _need(w, "w", _FLOATS, w.shape, dev)
         groups, (M, K) = w.shape[0] if w.dim() == 3 else 1, w.shape[-2:]
-        if w.requires_grad:
-            _detached("F8Weight.quantize")
         o = _f8_out(out, groups, M, K, dev)
+        if w.requires_grad or o.scales.requires_grad:
+            _detached("F8Weight.quantize")
         _launch("kxw4_quantize_weight_f8", dev, w.data_ptr(), _DTYPE_CODES[w.dtype], groups, M, K, o.codes.data_ptr(),
                 o.scales.data_ptr())
         return o
@@ -901,6 +901,8 @@ class F8Weight:
         dev = self.codes.device
         ref = _f8_weight(self, dev)
         o = _f8_out(out, self.groups, self.K, self.M, dev)
+        if self.scales.requires_grad or o.scales.requires_grad:
+            _detached("F8Weight.transposed")
         _launch("kxw4_transpose_weight_f8", dev, ref, o.codes.data_ptr(), o.scales.data_ptr())
         return o
 
@@ -985,9 +987,9 @@ def quantize_act_f8(x: torch.Tensor, out: Optional[QuantActF8] = None) -> QuantA
         raise ValueError("x must have shape (T, K)")
     T, K = x.shape
     _need(x, "x", _FLOATS, (T, K), dev)
-    if x.requires_grad:
-        _detached("quantize_act_f8")
     a = _f8_rows(T, K, dev, out)
+    if x.requires_grad or a.scale.requires_grad:
+        _detached("quantize_act_f8")
     _launch("kxw4_quantize_act_f8", dev, x.data_ptr(), _DTYPE_CODES[x.dtype], T, K, a.q.data_ptr(), a.scale.data_ptr())
     return a
 
@@ -1001,9 +1003,9 @@ def silu_mul_quant_f8(gate: torch.Tensor, up: torch.Tensor, keep_hidden=True, ou
     T, K = gate.shape
     _need(gate, "gate", _FLOATS, (T, K), dev)
     _need(up, "up", gate.dtype, (T, K), dev)
-    if gate.requires_grad or up.requires_grad:
-        _detached("silu_mul_quant_f8")
     a = _f8_rows(T, K, dev, out)
+    if gate.requires_grad or up.requires_grad or a.scale.requires_grad:
+        _detached("silu_mul_quant_f8")
     hidden = torch.empty(T, K, dtype=torch.float32, device=dev) if keep_hidden else None
     _launch("kxw4_silu_mul_quant_f8", dev, hidden.data_ptr() if keep_hidden else None, gate.data_ptr(), up.data_ptr(),
             _DTYPE_CODES[gate.dtype], T, K, a.q.data_ptr(), a.scale.data_ptr())
@@ -1045,6 +1047,8 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
     if isinstance(a, QuantActF8):
         T, K = a.T, a.K
         _check_act_f8(a, dev)
+        if a.scale.requires_grad:
+            _detached(name)
         ac = _lib.ActF8(T, K, 0, a.q.data_ptr(), a.scale.data_ptr(), None)
         xt = None
     else:
@@ -1070,7 +1074,8 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         raise ValueError(f"outs has {len(outs)} tensors for {n} weights")
     ys = [_out(N, w.M, dtype, dev, None if outs is None else outs[i], _OUTS[i]) for i, w in enumerate(ws)]
     _residual(residual, T, ws[0].M, dev)
-    if any([y.requires_grad for y in ys]) or (residual is not None and residual.requires_grad):
+    if (any([t.requires_grad for t in ys]) or any([w.scales.requires_grad for w in ws])
+            or (residual is not None and residual.requires_grad)):
         _detached(name)
     code = _dtype_code(dtype)
     nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, xt, code,
