@@ -28,7 +28,8 @@ expert_gemm[_fanout] projects each by its expert, adapter_add adds a low-rank
 adapter per request to a projection's output. None of these calls records a
 gradient: dispatch_rows, combine_rows (the gradients of both are calls of their
 own) and adapter_add (which has none) refuse tensors that require grad unless
-gradients are off, as they are in a torch.autograd.Function.
+gradients are off, as they are in a torch.autograd.Function, and tensors that
+carry a tangent of forward-mode differentiation.
 
 The 8-bit floating tier has none either (its tiers are integer): F8Weight holds
 e4m3 codes with a scale for each 128 x 128 block, gemm_f8[_fanout] and
@@ -49,6 +50,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import BF16, F32, SCALE_FP16, SCALE_FP16_ZP4, SCALE_W8, check, lib
@@ -533,12 +535,23 @@ def _launch(name: str, device: torch.device, *args) -> None:
         check(name, rc)
 
 
-def _detached(call: str) -> None:
-    """A tensor of `call` requires grad: refused while gradients are recorded,
-    since these calls record none and its own would be lost without a word."""
-    if torch.is_grad_enabled():
+def _dual() -> bool:
+    """Whether tensors may carry a tangent: inside a torch.autograd.forward_ad.dual_level."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def _detached(call: str, *tensors) -> None:
+    """Some of the floating `tensors` of `call` may require grad or carry a
+    tangent: refused while either is recorded, since these calls record none and
+    theirs would be lost without a word."""
+    tensors = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise ValueError(f"{call} records no gradient, but one of its tensors requires grad: call it under "
                          "torch.no_grad() or in the forward and backward of a torch.autograd.Function")
+    # (in a Function's forward its tensors have none)
+    if _dual() and any([forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        raise ValueError(f"{call} carries no tangent on, but one of its tensors has one: call it in the forward of a "
+                         "torch.autograd.Function with a jvp")
 
 
 # (the C calls take 32-bit sizes, and ctypes cuts a longer one to that unseen)
@@ -661,8 +674,8 @@ def dispatch_rows(x: torch.Tensor, route: RowRoute, out=None) -> torch.Tensor:
         _need(x, "x", _FLOATS, (route.T, H), dev)
     N = route.T * route.k
     rows = _need(out, "out", x.dtype, (N, H), dev) if out is not None else torch.empty(N, H, dtype=x.dtype, device=dev)
-    if x.requires_grad or rows.requires_grad:
-        _detached("dispatch_rows")
+    if x.requires_grad or rows.requires_grad or _dual():
+        _detached("dispatch_rows", x, rows)
     if N:
         _launch("kxw4_dispatch_rows", dev, x.data_ptr(), _DTYPE_CODES[x.dtype], H, plan, rows.data_ptr())
     return rows
@@ -685,8 +698,8 @@ def combine_rows(rows: torch.Tensor, route: RowRoute, weights: Optional[torch.Te
     if weights is not None:
         _need(weights, "weights", torch.float32, (route.T, route.k), dev)
     y = _out(route.T, H, dtype or (out.dtype if out is not None else rows.dtype), dev, out)
-    if rows.requires_grad or (weights is not None and weights.requires_grad) or y.requires_grad:
-        _detached("combine_rows")
+    if rows.requires_grad or (weights is not None and weights.requires_grad) or y.requires_grad or _dual():
+        _detached("combine_rows", rows, weights, y)
     if route.T:
         _launch("kxw4_combine_rows", dev, rows.data_ptr(), _DTYPE_CODES[rows.dtype], H,
                 None if weights is None else weights.data_ptr(), plan, y.data_ptr(), _DTYPE_CODES[y.dtype])
@@ -708,8 +721,8 @@ def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, route: RowRoute,
     _need(dy, "dy", _FLOATS, (route.T, H), dev)
     _need(weights, "weights", torch.float32, (route.T, route.k), dev)
     drows = _need(out, "out", rows.dtype, (N, H), dev) if out is not None else torch.empty_like(rows)
-    if dy.requires_grad or rows.requires_grad or weights.requires_grad or drows.requires_grad:
-        _detached("combine_rows_backward")
+    if dy.requires_grad or rows.requires_grad or weights.requires_grad or drows.requires_grad or _dual():
+        _detached("combine_rows_backward", dy, rows, weights, drows)
     dweights = torch.empty(route.T, route.k, dtype=torch.float32, device=dev)
     if N:
         _launch("kxw4_combine_rows_backward", dev, dy.data_ptr(), _DTYPE_CODES[dy.dtype], rows.data_ptr(),
@@ -815,8 +828,8 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, route: Row
     _need(scale, "adapters.scale", torch.float32, (n,), dev)
     o = _need(out, "out", y.dtype, (T, M), dev) if out is not None else torch.empty_like(y)
     if (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad or scale.requires_grad
-            or o.requires_grad):
-        _detached("adapter_add")
+            or o.requires_grad or _dual()):
+        _detached("adapter_add", y, x, a, b, scale, o)
     ref = C.byref(adapters.c())
     nbytes = _adapter_bytes(dev.index, n, r, K, M, T)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
@@ -873,8 +886,8 @@ class F8Weight:
         groups, (M, K) = codes.shape[0] if codes.dim() == 3 else 1, codes.shape[-2:]
         w = cls.empty(groups, M, K, dev)
         _need(scales, "scales", torch.float32, codes.shape[:-2] + (_blocks(M), _blocks(K)), dev)
-        if scales.requires_grad:
-            _detached("F8Weight.from_codes")
+        if scales.requires_grad or _dual():
+            _detached("F8Weight.from_codes", scales)
         w.scales.copy_(scales.view_as(w.scales))
         _launch("kxw4_pack_weight_f8", dev, codes.data_ptr(), groups, M, K, w.codes.data_ptr())
         return w
@@ -889,8 +902,8 @@ class F8Weight:
         _need(w, "w", _FLOATS, w.shape, dev)
         groups, (M, K) = w.shape[0] if w.dim() == 3 else 1, w.shape[-2:]
         o = _f8_out(out, groups, M, K, dev)
-        if w.requires_grad or o.scales.requires_grad:
-            _detached("F8Weight.quantize")
+        if w.requires_grad or o.scales.requires_grad or _dual():
+            _detached("F8Weight.quantize", w, o.scales)
         _launch("kxw4_quantize_weight_f8", dev, w.data_ptr(), _DTYPE_CODES[w.dtype], groups, M, K, o.codes.data_ptr(),
                 o.scales.data_ptr())
         return o
@@ -901,8 +914,8 @@ class F8Weight:
         dev = self.codes.device
         ref = _f8_weight(self, dev)
         o = _f8_out(out, self.groups, self.K, self.M, dev)
-        if self.scales.requires_grad or o.scales.requires_grad:
-            _detached("F8Weight.transposed")
+        if self.scales.requires_grad or o.scales.requires_grad or _dual():
+            _detached("F8Weight.transposed", self.scales, o.scales)
         _launch("kxw4_transpose_weight_f8", dev, ref, o.codes.data_ptr(), o.scales.data_ptr())
         return o
 
@@ -988,8 +1001,8 @@ def quantize_act_f8(x: torch.Tensor, out: Optional[QuantActF8] = None) -> QuantA
     T, K = x.shape
     _need(x, "x", _FLOATS, (T, K), dev)
     a = _f8_rows(T, K, dev, out)
-    if x.requires_grad or a.scale.requires_grad:
-        _detached("quantize_act_f8")
+    if x.requires_grad or a.scale.requires_grad or _dual():
+        _detached("quantize_act_f8", x, a.scale)
     _launch("kxw4_quantize_act_f8", dev, x.data_ptr(), _DTYPE_CODES[x.dtype], T, K, a.q.data_ptr(), a.scale.data_ptr())
     return a
 
@@ -1004,8 +1017,8 @@ def silu_mul_quant_f8(gate: torch.Tensor, up: torch.Tensor, keep_hidden=True, ou
     _need(gate, "gate", _FLOATS, (T, K), dev)
     _need(up, "up", gate.dtype, (T, K), dev)
     a = _f8_rows(T, K, dev, out)
-    if gate.requires_grad or up.requires_grad or a.scale.requires_grad:
-        _detached("silu_mul_quant_f8")
+    if gate.requires_grad or up.requires_grad or a.scale.requires_grad or _dual():
+        _detached("silu_mul_quant_f8", gate, up, a.scale)
     hidden = torch.empty(T, K, dtype=torch.float32, device=dev) if keep_hidden else None
     _launch("kxw4_silu_mul_quant_f8", dev, hidden.data_ptr() if keep_hidden else None, gate.data_ptr(), up.data_ptr(),
             _DTYPE_CODES[gate.dtype], T, K, a.q.data_ptr(), a.scale.data_ptr())
@@ -1047,8 +1060,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
     if isinstance(a, QuantActF8):
         T, K = a.T, a.K
         _check_act_f8(a, dev)
-        if a.scale.requires_grad:
-            _detached(name)
+        values = a.scale
         ac = _lib.ActF8(T, K, 0, a.q.data_ptr(), a.scale.data_ptr(), None)
         xt = None
     else:
@@ -1057,8 +1069,7 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         T, K = a.shape
         if a.dtype not in _FLOATS or not a.is_contiguous() or a.device != dev:
             _need(a, "x", _FLOATS, (T, K), dev)
-        if a.requires_grad:
-            _detached(name)
+        values = a
         ac = _lib.ActF8(T, K, _DTYPE_CODES[a.dtype], None, None, a.data_ptr())
         xt = ac.x_dtype
     if T > _MAX_SLOTS:
@@ -1074,9 +1085,9 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         raise ValueError(f"outs has {len(outs)} tensors for {n} weights")
     ys = [_out(N, w.M, dtype, dev, None if outs is None else outs[i], _OUTS[i]) for i, w in enumerate(ws)]
     _residual(residual, T, ws[0].M, dev)
-    if (any([t.requires_grad for t in ys]) or any([w.scales.requires_grad for w in ws])
-            or (residual is not None and residual.requires_grad)):
-        _detached(name)
+    if (values.requires_grad or any([t.requires_grad for t in ys]) or any([w.scales.requires_grad for w in ws])
+            or (residual is not None and residual.requires_grad) or _dual()):
+        _detached(name, values, residual, *ys, *[w.scales for w in ws])
     code = _dtype_code(dtype)
     nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, xt, code,
                        None if route is None else (route.T, route.k, route.groups, bool(sorted_rows)))
@@ -1146,8 +1157,8 @@ def _grad_weight(name: str, dy, x, route, dtype, add, out):
     if add is not None:
         _need(add, "add", dtype, shape, dev)
     dw = _need(out, "out", dtype, shape, dev) if out is not None else torch.empty(shape, dtype=dtype, device=dev)
-    if dy.requires_grad or x.requires_grad or dw.requires_grad or (add is not None and add.requires_grad):
-        _detached(name)
+    if dy.requires_grad or x.requires_grad or dw.requires_grad or (add is not None and add.requires_grad) or _dual():
+        _detached(name, dy, x, dw, add)
     nbytes = _grad_bytes(dev.index, N, groups, M, K)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("kxw4_grad_weight", dev, dy.data_ptr(), x.data_ptr(), N, M, K, plan, None if add is None else add.data_ptr(),
