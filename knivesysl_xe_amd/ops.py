@@ -1085,8 +1085,10 @@ def _f8_product(name: str, ws, a, dtype, outs, residual, route, sorted_rows: boo
         raise ValueError(f"outs has {len(outs)} tensors for {n} weights")
     ys = [_out(N, w.M, dtype, dev, None if outs is None else outs[i], _OUTS[i]) for i, w in enumerate(ws)]
     _residual(residual, T, ws[0].M, dev)
-    if (values.requires_grad or any([t.requires_grad for t in ys]) or any([w.scales.requires_grad for w in ws])
-            or (residual is not None and residual.requires_grad) or _dual()):
+    tracked = values.requires_grad or (residual is not None and residual.requires_grad) or _dual()
+    for w, y in zip(ws, ys):
+        tracked = tracked or w.scales.requires_grad or y.requires_grad
+    if tracked:
         _detached(name, values, residual, *ys, *[w.scales for w in ws])
     code = _dtype_code(dtype)
     nbytes = _f8_bytes(dev.index, tuple([w.M for w in ws]), K, T, xt, code,
