@@ -4,7 +4,9 @@
 // code = e4m3(x * (448 / top)), each operation rounded once. The floor keeps
 // 448 / top finite; a block below it (zeros among them) has codes of a relative
 // error past e4m3's. A NaN or an infinity in a block makes a NaN code, so a
-// product of that row is NaN. Bound: memory, one read and one write.
+// product of that row is NaN. Bound: memory, one read and one write; with SiLU of
+// BF16 rows and no values out, its arithmetic (3,965 x 17,408: 94 us, 3.7 TB/s, VALU
+// 88 % of the cycles; values too 131 us, 4.7; 4,096 x 17,408 of FP32 134 us, 4.8).
 #include "kxw4_f8.hpp"
 
 namespace kxw4 {
@@ -130,6 +132,8 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const F8WeightArgs a, int 
     }
 }
 
+// Weights' values to codes: 5,120 x 5,120 of BF16 in 20 us (3.9 TB/s), 17,408 x 5,120
+// in 55 (4.9); of FP32 the first in 29 (4.5).
 template <bool BF16>
 __global__ __launch_bounds__(256) void f8_weight_kernel(const F8WeightArgs a, int groups) {
     __shared__ float red[4];

@@ -14,8 +14,8 @@
 // Bound: HBM, where there are weights enough (8 rows, 2 x 17,408 x 5,120: 178 MB
 // in 30 to 32 us, 5.6 to 5.9 TB/s; 16 x 8 rows over 64 experts, 2 x 1,024 x 5,120:
 // 582 MB, of which 499 from HBM, in 73 to 79 us; a pure read reaches 6.3); below
-// that the chain of round trips of one launch (one row, 4,096 x 4,096: 16.8 MB in
-// 8.1 us).
+// that a wave's round trips, one after another (one row, 4,096 x 4,096: eight
+// blocks a wave, two of them in flight: 16.8 MB in 8.0 us).
 #include "kxw4_f8.hpp"
 #include "kxw4_f8_route.hpp"
 #include "kxw4_groups.hpp"

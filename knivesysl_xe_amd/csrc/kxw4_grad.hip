@@ -13,13 +13,14 @@
 //
 // Bounds and measurements (256 CUs; a large BF16 library product reaches 1,176 to
 // 1,265 TF): the matrix units, at the clock that the power limit leaves them, for
-// many rows of a group (4,096 rows, 5,120 x 5,120, FP32 out: 224 us, 957 TF; 2,048
-// rows, 17,408 x 5,120, BF16 out: 345 us, 1,058 TF); the last round of tiles where
-// these are few (2,048 rows, 5,120 x 5,120: 400 tiles on 256 CUs, 136 to 143 us,
-// 749 TF and more); the stores where a group has few rows (64 groups of 256 rows,
-// 1,024 x 2,048, BF16 out: 134 us, 512 TF). A first version with a tile per work-group and 32-byte
-// stores took 177 us for the 2,048 rows and 290 for 8 groups of 1,000 rows, 2,048 x
-// 4,096 (now 168: 800 TF).
+// many rows of a group (4,096 rows, 5,120 x 5,120, FP32 out: 218 to 224 us, 957 TF
+// and more; 2,048 rows, 17,408 x 5,120, BF16 out: 320 to 345 us, 1,058 TF and more);
+// the last round of tiles where these are few (2,048 rows, 5,120 x 5,120, FP32 out:
+// 400 tiles on 256 CUs, 122 to 143 us, 749 TF and more; with `add` 147 for 122); the
+// stores where a group has few rows (64 groups of 256 rows, 1,024 x 2,048, BF16 out:
+// 134 us, 512 TF). A first version with a tile per work-group and 32-byte stores took
+// 177 us for the 2,048 rows and 290 for 8 groups of 1,000 rows, 2,048 x 4,096 (now
+// 168: 800 TF).
 #include "kxw4_device.hpp"
 #include "kxw4_internal.hpp"
 
